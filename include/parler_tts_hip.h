@@ -279,6 +279,81 @@ int ptts_test_gemm(int32_t dtype, int32_t M, int32_t N, int32_t K, const float* 
                    const float* gamma, const float* beta, float eps, int32_t act, const float* bias, float* Y,
                    void* stream);
 
+/* ---- operators over a CALLER'S paged KV cache (no engine; python: parler_tts_amd.paged) ----------------------------------------
+ * What the engine does inside its decode step and its batched prefill, for a cache, a page table and a ragged batch that the caller
+ * owns: rotary positions, the append of new keys and values with the rotation applied on the way, the attention of the new tokens
+ * over the cache.  Extensions: the reference has no paged cache and no rotary positions (its cache: modeling_parler_tts.py:285-306,
+ * its attention: :264-382).
+ *   - re-entrant and stateless; work is enqueued on `stream` of the CURRENT device, which owns every pointer.  Here NULL is the
+ *     legacy default stream itself (asynchronous, as everywhere else in HIP).  All calls can be captured into a hipGraph.
+ *   - page ids, lengths, starts and positions are read on the device, at the time the work runs.  Values that lead outside the
+ *     cache, the tables or the batch are never followed: the call sets bits of *status (device int32, caller-owned, only ever or-ed)
+ *     and returns what is said below for such rows.
+ *   - tokens behind the last sequence (>= starts[n_seqs]) are padding: nothing of theirs is read or written.
+ *   - a slot that two tokens of one call are appended to (a page listed twice) holds one of the two afterwards. */
+enum {
+    PTTS_PAGED_BAD_POSITION = 1,    /* a position outside the rotary table */
+    PTTS_PAGED_BAD_PAGE = 2,        /* a page id outside the cache */
+    PTTS_PAGED_BAD_LENGTH = 4,      /* past < 0, or a token behind the last page of its table row */
+    PTTS_PAGED_BAD_STARTS = 8       /* starts outside [0, tokens] or descending */
+};
+
+/* element [page][head][slot][feature], features contiguous; strides in elements, so that any order of the first three fits */
+typedef struct ptts_paged_kv {
+    void* k;
+    void* v;
+    int64_t k_strides[3], v_strides[3];    /* page, head, slot; every row starts at a multiple of 16 bytes */
+    int32_t dtype;                         /* PTTS_DTYPE_* */
+    int32_t n_pages, kv_heads;
+    int32_t page_tokens;                   /* power of two, 16 .. 4096 */
+    int32_t head_dim;                      /* 64 or 128 */
+} ptts_paged_kv;
+
+/* new tokens of n_seqs sequences, one behind the other: tokens starts[s] .. starts[s + 1] - 1 are sequence s's (starts NULL: one each) */
+typedef struct ptts_paged_batch {
+    const int32_t* table;                  /* [n_seqs][table_stride]: page ids of the slots 0 .. of every sequence */
+    int64_t table_stride;
+    const int32_t* past;                   /* [n_seqs]: tokens in the cache before these */
+    const int32_t* starts;                 /* [n_seqs + 1] ascending, or NULL */
+    int32_t max_pages;                     /* used width of the table */
+    int32_t n_seqs, tokens;                /* tokens: rows of q / k / v (>= starts[n_seqs]) */
+} ptts_paged_batch;
+
+/* cos / sin [positions][dims / 2] fp32; the first `dims` (even) features of a head turn, pairs (i, i + dims / 2) or (2 i, 2 i + 1) */
+typedef struct ptts_rotary {
+    const float* cos_t;
+    const float* sin_t;
+    int32_t positions, dims, interleaved;
+} ptts_rotary;
+
+/* out = x turned by positions [tokens] int32; x, out [tokens][heads][head_dim] (features contiguous) of `dtype`; out may be x.
+ * A row whose position is outside the table becomes zero. */
+int ptts_rotary_embed(const ptts_rotary* rot, int32_t dtype, int32_t tokens, int32_t heads, int32_t head_dim, const void* x,
+                      int64_t x_token_stride, int64_t x_head_stride, const int32_t* positions, void* out, int64_t out_token_stride,
+                      int64_t out_head_stride, int32_t* status, void* stream);
+
+/* Token i of sequence s goes to slot past[s] + i: k turned by `rot` (NULL: as it is) at its slot, or at positions[token] where
+ * positions is given; v as it is.  q (optional: q_heads > 0) is turned at the same positions into q_out, which may be q.
+ * dtype is that of k, v and q; f32 rows may go into a bf16 cache (rounded once, behind the rotation).  A token that cannot be placed
+ * leaves the cache as it is and its row of q_out becomes zero. */
+int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, int32_t dtype, const void* k, int64_t k_token_stride,
+                   int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, const ptts_rotary* rot,
+                   const int32_t* positions, int32_t q_heads, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
+                   int64_t q_out_token_stride, int64_t q_out_head_stride, int32_t* status, void* stream);
+
+/* out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j].  causal: token i of sequence s sees the keys 0 .. past[s] + i (the new tokens are in
+ * the cache); else all of 0 .. past[s] - 1 (encoder states, say).  key_mask [n_seqs][mask_stride] bytes: keys j < mask_width with a zero
+ * are no keys; whatever they hold does not reach the output.  A token that sees no key gets zeros; rows that a bad page, length or start
+ * concerns get NaN.  Query head h reads key head h / (q_heads / kv_heads).  q, out: [tokens][q_heads][head_dim] of the cache's type.
+ * max_new: an upper bound of the new tokens of one sequence, 0 = not known; it picks the kernel, never the result's validity.
+ * workspace: ptts_paged_attention_workspace() bytes (may be 0; negative = PTTS_E_*) at a multiple of 16, not shared with another call
+ * in flight. */
+int64_t ptts_paged_attention_workspace(const ptts_paged_kv* cache, const ptts_paged_batch* batch, int32_t q_heads, int32_t max_new);
+int ptts_paged_attention(const ptts_paged_kv* cache, const ptts_paged_batch* batch, int32_t q_heads, const void* q, int64_t q_token_stride,
+                         int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride, float scale, int32_t causal,
+                         const uint8_t* key_mask, int64_t mask_stride, int32_t mask_width, int32_t max_new, void* workspace,
+                         int64_t workspace_bytes, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,4 +29,8 @@ def __getattr__(name):
         from .streamer import AudioStreamer
 
         return AudioStreamer
+    if name in ("PagedKVCache", "RotaryTable", "rotary_embed", "kv_append", "paged_attention"):
+        from . import paged
+
+        return getattr(paged, name)
     raise AttributeError(name)

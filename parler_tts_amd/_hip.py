@@ -21,6 +21,7 @@ EXPORTS = [
     "ptts_t5_encode", "ptts_dac_decode", "ptts_dac_encode", "ptts_set_prompt_embeds", "ptts_set_decoder_mask", "ptts_prefill", "ptts_decode_steps", "ptts_forward_step", "ptts_select_step", "ptts_get_state", "ptts_state_snapshot", "ptts_state_poll", "ptts_last_logits",
     "ptts_set_block_table", "ptts_pool_info", "ptts_set_forced_tokens", "ptts_set_forced_sequence", "ptts_profile_read", "ptts_test_gemm",
     "ptts_debug_stop_after", "ptts_debug_buffer", "ptts_dac_kernel_counts",
+    "ptts_rotary_embed", "ptts_kv_append", "ptts_paged_attention_workspace", "ptts_paged_attention",
 ]
 
 # kernel families of ptts_dac_kernel_counts (include/parler_tts_hip.h)
@@ -63,6 +64,25 @@ class PttsState(C.Structure):
 class PttsProfile(C.Structure):
     _fields_ = [("launches", C.c_int64), ("total_ms", C.c_double), ("algo_bytes", C.c_double), ("steps", C.c_int64),
                 ("step_ms", C.c_double), ("fused_launches", C.c_int64)]
+
+
+class PttsPagedKV(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3), ("dtype", C.c_int32),
+                ("n_pages", C.c_int32), ("kv_heads", C.c_int32), ("page_tokens", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class PttsPagedBatch(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("table_stride", C.c_int64), ("past", C.c_void_p), ("starts", C.c_void_p),
+                ("max_pages", C.c_int32), ("n_seqs", C.c_int32), ("tokens", C.c_int32)]
+
+
+class PttsRotary(C.Structure):
+    _fields_ = [("cos_t", C.c_void_p), ("sin_t", C.c_void_p), ("positions", C.c_int32), ("dims", C.c_int32), ("interleaved", C.c_int32)]
+
+
+# bits of a paged operator's status word (PTTS_PAGED_*)
+PAGED_STATUS = {1: "a position outside the rotary table", 2: "a page id outside the cache",
+                4: "a sequence longer than its row of the page table (or of negative length)", 8: "starts outside the batch or descending"}
 
 
 class HipLibraryMissing(RuntimeError):
@@ -115,9 +135,15 @@ def load_library() -> C.CDLL:
     lib.ptts_debug_buffer.argtypes = [vp, C.c_char_p, C.POINTER(vp), C.POINTER(C.c_int64)]
     lib.ptts_dac_kernel_counts.argtypes = [i64p, i32, i32]
     lib.ptts_test_gemm.argtypes = [i32, i32, i32, i32, vp, vp, i32, vp, vp, C.c_float, i32, vp, vp, vp]
+    f32, i64 = C.c_float, C.c_int64
+    lib.ptts_rotary_embed.argtypes = [vp, i32, i32, i32, i32, vp, i64, i64, vp, vp, i64, i64, vp, vp]
+    lib.ptts_kv_append.argtypes = [vp, vp, i32, vp, i64, i64, vp, i64, i64, vp, vp, i32, vp, i64, i64, vp, i64, i64, vp, vp]
+    lib.ptts_paged_attention_workspace.argtypes = [vp, vp, i32, i32]
+    lib.ptts_paged_attention.argtypes = [vp, vp, i32, vp, i64, i64, vp, i64, i64, f32, i32, vp, i64, i32, i32, vp, i64, vp, vp]
     for name in EXPORTS:
         if name not in ("ptts_last_error",):
             getattr(lib, name).restype = i32
+    lib.ptts_paged_attention_workspace.restype = i64
     lib.ptts_last_error.restype = C.c_char_p
     if lib.ptts_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{LIB_PATH}: ABI version {lib.ptts_abi_version()} != binding {ABI_VERSION}; rebuild")

@@ -21,6 +21,7 @@
 #include "fused.h"
 #include "gemm.h"
 #include "misc.h"
+#include "paged.h"
 
 namespace {
 
@@ -873,6 +874,16 @@ int load_dac_tensor(ptts_engine* e, const std::string& n, const float* data, con
 }
 
 }  // namespace
+
+int ptts_set_error(int code, const char* fmt, ...) {
+    char buf[1024];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    g_err = buf;
+    return code;
+}
 
 extern "C" {
 

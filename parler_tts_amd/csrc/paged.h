@@ -1,0 +1,74 @@
+// Host-side interface of paged.hip / paged_attn.hip (internal): the operators over a caller's paged KV cache.
+#pragma once
+#include "ptts_common.h"
+
+// the text behind ptts_last_error(); returns `code` (engine.hip)
+int ptts_set_error(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+
+// bits of the caller's status word (PTTS_PAGED_* of the C ABI)
+enum { PAGED_BAD_POSITION = 1, PAGED_BAD_PAGE = 2, PAGED_BAD_LENGTH = 4, PAGED_BAD_STARTS = 8 };
+
+struct PagedBatchArgs {
+    const int* table;        // [n_seqs][table_stride] page ids
+    int64_t table_stride;
+    const int* past;         // [n_seqs] tokens cached before the call
+    const int* starts;       // [n_seqs + 1] first token of every sequence, or null: token t belongs to sequence t
+    int max_pages, n_pages, page_shift, n_seqs, tokens;
+};
+
+#if defined(__HIPCC__)
+// starts must ascend within [0, tokens]; one workgroup of a launch looks at all of them
+__device__ inline void check_starts(const int* starts, int n_seqs, int tokens, int* status) {
+    for (int i = threadIdx.x; i < n_seqs; i += blockDim.x)
+        if (starts[i] < 0 || starts[i] > starts[i + 1] || starts[i + 1] > tokens) atomicOr(status, PAGED_BAD_STARTS);
+}
+#endif
+
+struct RotaryArgs {
+    const float *cos_t, *sin_t;   // [positions][dims / 2]
+    int positions, dims, interleaved;
+};
+
+struct RotaryEmbedArgs {
+    const void* x;
+    void* out;
+    int64_t xs[2], os[2];    // token, head strides (elements)
+    const int* pos;          // [tokens]
+    RotaryArgs rot;
+    int* status;
+    int tokens, heads, head_dim;
+};
+
+struct AppendArgs {
+    const void *q, *k, *v;
+    void *q_out, *k_cache, *v_cache;
+    int64_t qs[2], qos[2], ks[2], vs[2];     // token, head
+    int64_t kc[3], vc[3];                    // page, head, slot
+    PagedBatchArgs b;
+    RotaryArgs rot;                          // cos_t null: no rotation
+    const int* pos;                          // [tokens] or null: the position is the slot
+    int* status;
+    int q_heads, kv_heads, head_dim;         // q_heads 0: no q
+};
+
+struct PagedAttnArgs {
+    const void *q, *k, *v;
+    void* out;
+    const int* table;
+    const int* past;
+    const int* starts;
+    const uint8_t* mask;     // [n_seqs][mask_stride], keys < mask_width with 0 are no keys; null: none
+    int* status;
+    float* part;             // partial results of a split launch: [split][row][D + 2]
+    int64_t qs[2], os[2], kc[3], vc[3];
+    int64_t table_stride, mask_stride;
+    float scale_log2;        // softmax scale * log2(e)
+    int max_pages, n_pages, page_shift, n_seqs, tokens, mask_width, causal;
+    int q_heads, kv_heads, group, splits;
+};
+
+hipError_t rotary_embed_launch(const RotaryEmbedArgs& a, int dtype, hipStream_t s);
+hipError_t kv_append_launch(const AppendArgs& a, int in_dtype, int cache_dtype, hipStream_t s);
+// rows of one sequence never exceed max_new * group; the choice of kernel and split follows from it and from max_pages
+int64_t paged_attn_workspace(const PagedAttnArgs& a, int max_new, int head_dim, int dtype);
+hipError_t paged_attn_launch(const PagedAttnArgs& a, int max_new, int head_dim, int dtype, hipStream_t s);

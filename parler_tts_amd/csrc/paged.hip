@@ -1,0 +1,461 @@
+// Rotary positions and the append of keys and values to a caller's paged cache, and the C entries of the paged operators.
+//
+// Rotation: the pair (a, b) of a head becomes (a cos t - b sin t, b cos t + a sin t); pairs are (i, i + r / 2) (half layout) or
+// (2 i, 2 i + 1) (interleaved) of the first r features, the features behind them are copied.  cos t / sin t come from the caller's
+// fp32 tables, built from 64-bit angles: an angle formed in 32 bits is off by half a unit of position * 2^-24, 4e-3 at position 131072.
+// Products and sum are rounded one by one (no fma contraction), so that a row has the same bits whichever kernel or layout turns it.
+#include "../../include/parler_tts_hip.h"
+#include "ptts_common.h"
+#include "gemm.h"
+#include "paged.h"
+#include <climits>
+#include <cmath>
+
+namespace {
+
+template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T e[N]; };
+
+template <typename T> __device__ inline float widen(T v);
+template <> __device__ inline float widen<uint16_t>(uint16_t v) { return bf16_bits_to_float(v); }
+template <> __device__ inline float widen<float>(float v) { return v; }
+template <typename T> __device__ inline T narrow(float v);
+template <> __device__ inline uint16_t narrow<uint16_t>(float v) { return float_to_bf16_bits(v); }     // half a bf16 step: the caller's type
+template <> __device__ inline float narrow<float>(float v) { return v; }
+
+// i / d for i < 65536, 1 <= d <= 65536: m = ceil(2^32 / d) (d = 1: m = 0, the quotient is i)
+struct SmallDiv { uint32_t m; };
+__device__ inline int small_div(int i, SmallDiv d) { return d.m ? (int)__umulhi((uint32_t)i, d.m) : i; }
+
+// One unit of work: N pairs of a rotated head (two runs of N elements), or 2 N elements that are copied.
+template <typename T, int N> struct Unit { Pack<T, N> a, b; };
+
+template <typename T, int N> __device__ inline void turn(Unit<T, N>& u, const float* cos_t, const float* sin_t, int interleaved) {
+#pragma clang fp contract(off)
+    const Pack<float, N> c = *reinterpret_cast<const Pack<float, N>*>(cos_t), s = *reinterpret_cast<const Pack<float, N>*>(sin_t);
+    float x[2 * N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) { x[i] = widen<T>(u.a.e[i]); x[N + i] = widen<T>(u.b.e[i]); }
+    float y[2 * N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int ia = interleaved ? 2 * i : i, ib = interleaved ? 2 * i + 1 : N + i;
+        y[ia] = x[ia] * c.e[i] - x[ib] * s.e[i];
+        y[ib] = x[ib] * c.e[i] + x[ia] * s.e[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) { u.a.e[i] = narrow<T>(y[i]); u.b.e[i] = narrow<T>(y[N + i]); }
+}
+
+struct UnitMap {            // where the units of one token lie
+    SmallDiv per_token, per_head;
+    int upt, uph, rotated;  // units per token and head; the first `rotated` units of a head turn
+    int tokens_per_block;
+};
+
+template <int N> __device__ inline void unit_offsets(const RotaryArgs& r, int rotated, int c, int* oa, int* ob) {
+    if (c >= rotated) { *oa = rotated * 2 * N + (c - rotated) * 2 * N; *ob = *oa + N; }
+    else if (r.interleaved) { *oa = c * 2 * N; *ob = *oa + N; }
+    else { *oa = c * N; *ob = r.dims / 2 + c * N; }
+}
+
+template <typename T, int N, bool IL>
+__global__ __launch_bounds__(256) void rotary_embed_kernel(RotaryEmbedArgs a, UnitMap m) {
+    const int t0 = blockIdx.x * m.tokens_per_block;
+    const int n = min(m.tokens_per_block, a.tokens - t0) * m.upt;
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int tl = small_div(i, m.per_token), r = i - tl * m.upt, h = small_div(r, m.per_head), c = r - h * m.uph;
+        const int64_t t = t0 + tl;
+        const int pos = a.pos[t];
+        const bool ok = (unsigned)pos < (unsigned)a.rot.positions;
+        int oa, ob;
+        unit_offsets<N>(a.rot, m.rotated, c, &oa, &ob);
+        const T* x = reinterpret_cast<const T*>(a.x) + t * a.xs[0] + h * a.xs[1];
+        T* o = reinterpret_cast<T*>(a.out) + t * a.os[0] + h * a.os[1];
+        Unit<T, N> u;
+        u.a = *reinterpret_cast<const Pack<T, N>*>(x + oa);
+        u.b = *reinterpret_cast<const Pack<T, N>*>(x + ob);
+        if (!ok) {
+            u = Unit<T, N>{};
+            if (r == 0) atomicOr(a.status, PAGED_BAD_POSITION);
+        } else if (c < m.rotated) {
+            const int64_t row = (int64_t)pos * (a.rot.dims / 2) + c * N;
+            turn<T, N>(u, a.rot.cos_t + row, a.rot.sin_t + row, IL);
+        }
+        *reinterpret_cast<Pack<T, N>*>(o + oa) = u.a;
+        *reinterpret_cast<Pack<T, N>*>(o + ob) = u.b;
+    }
+}
+
+// Sequence of a token and its first token; false: the token lies behind the last sequence (or in front of the first).
+__device__ inline bool find_sequence(const PagedBatchArgs& b, int t, int* seq, int* first, int* end) {
+    if (!b.starts) { *seq = t; *first = t; *end = t + 1; return true; }
+    int lo = 0, hi = b.n_seqs;                        // largest s with starts[s] <= t: never an empty sequence
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (b.starts[mid] <= t) lo = mid; else hi = mid;
+    }
+    *seq = lo; *first = b.starts[lo]; *end = b.starts[lo + 1];
+    return t >= *first && t < *end;
+}
+
+constexpr int APPEND_TOKENS = 64;      // most tokens of one workgroup
+
+// The rows of a block's tokens are looked up once (sequence, page, slot, position), then every thread moves units.
+template <typename T, typename TC, int N, bool IL>
+__global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, UnitMap m) {
+    __shared__ int page_of[APPEND_TOKENS], slot_of[APPEND_TOKENS], pos_of[APPEND_TOKENS];   // page -1: nothing to do, -2: refused
+    if (blockIdx.x == 0 && a.b.starts) check_starts(a.b.starts, a.b.n_seqs, a.b.tokens, a.status);
+    const int t0 = blockIdx.x * m.tokens_per_block, nt = min(m.tokens_per_block, a.b.tokens - t0);
+    if ((int)threadIdx.x < nt) {
+        const int t = t0 + threadIdx.x;
+        int s, first, end, page = -1, slot = 0, pos = 0;
+        if (find_sequence(a.b, t, &s, &first, &end)) {
+            const int past = a.b.past[s];
+            const int64_t at = (int64_t)past + (t - first);
+            int bad = 0;
+            if (first < 0 || end > a.b.tokens) bad = PAGED_BAD_STARTS;
+            else if (past < 0 || at >= ((int64_t)a.b.max_pages << a.b.page_shift)) bad = PAGED_BAD_LENGTH;
+            else {
+                page = a.b.table[s * a.b.table_stride + (at >> a.b.page_shift)];
+                slot = (int)at & ((1 << a.b.page_shift) - 1);
+                pos = a.pos ? a.pos[t] : (int)at;
+                if ((unsigned)page >= (unsigned)a.b.n_pages) bad = PAGED_BAD_PAGE;
+                else if (a.rot.cos_t && (unsigned)pos >= (unsigned)a.rot.positions) bad = PAGED_BAD_POSITION;
+            }
+            if (bad) { page = -2; atomicOr(a.status, bad); }
+        }
+        page_of[threadIdx.x] = page; slot_of[threadIdx.x] = slot; pos_of[threadIdx.x] = pos;
+    }
+    __syncthreads();
+    const int n = nt * m.upt;
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int tl = small_div(i, m.per_token), r = i - tl * m.upt, h = small_div(r, m.per_head), c = r - h * m.uph;
+        const int64_t t = t0 + tl;
+        const int page = page_of[tl];
+        const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.kv_heads;
+        if (page == -1 || (page < 0 && !is_q)) continue;
+        const int hk = is_v ? h - a.q_heads - a.kv_heads : h - a.q_heads;
+        int oa, ob;
+        unit_offsets<N>(a.rot, m.rotated, c, &oa, &ob);
+        const T* x = is_q ? reinterpret_cast<const T*>(a.q) + t * a.qs[0] + h * a.qs[1]
+                          : (is_v ? reinterpret_cast<const T*>(a.v) + t * a.vs[0] + hk * a.vs[1]
+                                  : reinterpret_cast<const T*>(a.k) + t * a.ks[0] + hk * a.ks[1]);
+        Unit<T, N> u;
+        u.a = *reinterpret_cast<const Pack<T, N>*>(x + oa);
+        u.b = *reinterpret_cast<const Pack<T, N>*>(x + ob);
+        if (page < 0) u = Unit<T, N>{};
+        if (is_q) {
+            if (c < m.rotated && page >= 0) {
+                const int64_t row = (int64_t)pos_of[tl] * (a.rot.dims / 2) + c * N;
+                turn<T, N>(u, a.rot.cos_t + row, a.rot.sin_t + row, IL);
+            }
+            T* o = reinterpret_cast<T*>(a.q_out) + t * a.qos[0] + h * a.qos[1];
+            *reinterpret_cast<Pack<T, N>*>(o + oa) = u.a;
+            *reinterpret_cast<Pack<T, N>*>(o + ob) = u.b;
+        } else {
+            if (c < m.rotated && !is_v) {
+                const int64_t row = (int64_t)pos_of[tl] * (a.rot.dims / 2) + c * N;
+                turn<T, N>(u, a.rot.cos_t + row, a.rot.sin_t + row, IL);
+            }
+            const int64_t* cs = is_v ? a.vc : a.kc;
+            TC* o = reinterpret_cast<TC*>(is_v ? a.v_cache : a.k_cache) + page * cs[0] + hk * cs[1] + slot_of[tl] * cs[2];
+            Pack<TC, N> ya, yb;
+#pragma unroll
+            for (int j = 0; j < N; ++j) { ya.e[j] = narrow<TC>(widen<T>(u.a.e[j])); yb.e[j] = narrow<TC>(widen<T>(u.b.e[j])); }
+            *reinterpret_cast<Pack<TC, N>*>(o + oa) = ya;
+            *reinterpret_cast<Pack<TC, N>*>(o + ob) = yb;
+        }
+    }
+}
+
+SmallDiv make_div(int d) { return SmallDiv{d == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + d - 1) / d)}; }
+
+UnitMap make_map(int heads, int head_dim, int rot_dims, int n, int tokens, int most_tokens) {
+    UnitMap m;
+    m.uph = head_dim / (2 * n);
+    m.upt = heads * m.uph;
+    m.rotated = rot_dims / (2 * n);
+    m.per_token = make_div(m.upt);
+    m.per_head = make_div(m.uph);
+    const int64_t total = (int64_t)tokens * m.upt;
+    const int want = total <= 256 * 256 ? 256 : 1024;
+    m.tokens_per_block = want / m.upt;
+    if (m.tokens_per_block < 1) m.tokens_per_block = 1;
+    if (m.tokens_per_block > most_tokens) m.tokens_per_block = most_tokens;
+    return m;
+}
+
+bool aligned(const void* p, const int64_t* strides, int ns, int64_t bytes, int64_t esz) {
+    if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
+    for (int i = 0; i < ns; ++i)
+        if (strides[i] * esz % bytes) return false;
+    return true;
+}
+
+}  // namespace
+
+hipError_t rotary_embed_launch(const RotaryEmbedArgs& a, int dtype, hipStream_t s) {
+    const int esz = dtype == PTTS_BF16 ? 2 : 4, full = 16 / esz;
+    const bool wide = a.rot.dims % (2 * full) == 0 && a.head_dim % (2 * full) == 0 && aligned(a.x, a.xs, 2, 16, esz) &&
+                      aligned(a.out, a.os, 2, 16, esz) && aligned(a.rot.cos_t, nullptr, 0, 16, 4) && aligned(a.rot.sin_t, nullptr, 0, 16, 4);
+    const UnitMap m = make_map(a.heads, a.head_dim, a.rot.dims, wide ? full : 1, a.tokens, 1 << 20);
+    const dim3 grid((a.tokens + m.tokens_per_block - 1) / m.tokens_per_block), block(256);
+#define LAUNCH(T, N)                                                                                        \
+    do {                                                                                                    \
+        if (a.rot.interleaved) hipLaunchKernelGGL((rotary_embed_kernel<T, N, true>), grid, block, 0, s, a, m); \
+        else hipLaunchKernelGGL((rotary_embed_kernel<T, N, false>), grid, block, 0, s, a, m);               \
+    } while (0)
+    if (dtype == PTTS_BF16) { if (wide) LAUNCH(uint16_t, 8); else LAUNCH(uint16_t, 1); }
+    else { if (wide) LAUNCH(float, 4); else LAUNCH(float, 1); }
+#undef LAUNCH
+    return hipGetLastError();
+}
+
+hipError_t kv_append_launch(const AppendArgs& a, int in_dtype, int cache_dtype, hipStream_t s) {
+    const int esz = in_dtype == PTTS_BF16 ? 2 : 4, full = 16 / esz;
+    const int csz = cache_dtype == PTTS_BF16 ? 2 : 4;
+    bool wide = a.rot.dims % (2 * full) == 0 && a.head_dim % (2 * full) == 0 && aligned(a.k, a.ks, 2, 16, esz) && aligned(a.v, a.vs, 2, 16, esz) &&
+                aligned(a.k_cache, a.kc, 3, full * csz, csz) && aligned(a.v_cache, a.vc, 3, full * csz, csz);
+    if (a.q_heads) wide = wide && aligned(a.q, a.qs, 2, 16, esz) && aligned(a.q_out, a.qos, 2, 16, esz);
+    if (a.rot.cos_t) wide = wide && aligned(a.rot.cos_t, nullptr, 0, 16, 4) && aligned(a.rot.sin_t, nullptr, 0, 16, 4);
+    const UnitMap m = make_map(a.q_heads + 2 * a.kv_heads, a.head_dim, a.rot.dims, wide ? full : 1, a.b.tokens, APPEND_TOKENS);
+    const dim3 grid((a.b.tokens + m.tokens_per_block - 1) / m.tokens_per_block), block(256);
+#define LAUNCH(T, TC, N)                                                                                      \
+    do {                                                                                                      \
+        if (a.rot.interleaved) hipLaunchKernelGGL((kv_append_kernel<T, TC, N, true>), grid, block, 0, s, a, m); \
+        else hipLaunchKernelGGL((kv_append_kernel<T, TC, N, false>), grid, block, 0, s, a, m);                \
+    } while (0)
+    if (in_dtype == PTTS_BF16) { if (wide) LAUNCH(uint16_t, uint16_t, 8); else LAUNCH(uint16_t, uint16_t, 1); }
+    else if (cache_dtype == PTTS_BF16) { if (wide) LAUNCH(float, uint16_t, 4); else LAUNCH(float, uint16_t, 1); }
+    else { if (wide) LAUNCH(float, float, 4); else LAUNCH(float, float, 1); }
+#undef LAUNCH
+    return hipGetLastError();
+}
+
+// ---- C entries ----------------------------------------------------------------------------------------------------------
+namespace {
+
+#define REFUSE(code, ...) return ptts_set_error(code, __VA_ARGS__)
+
+// rows of a written tensor may not share elements: the smaller stride holds the row inside it, the larger one all rows of the smaller
+bool overlaps_itself(const int64_t* st, const int64_t* n, int dims, int64_t inner) {
+    bool used[3] = {false, false, false};
+    int64_t span = inner;                      // elements from the first to behind the last of what has been nested so far
+    for (int k = 0; k < dims; ++k) {
+        int best = -1;
+        for (int i = 0; i < dims; ++i)
+            if (!used[i] && (best < 0 || st[i] < st[best])) best = i;
+        used[best] = true;
+        if (n[best] <= 1) continue;
+        if (st[best] < span) return true;
+        span += (n[best] - 1) * st[best];
+    }
+    return false;
+}
+
+bool fits(const int64_t* st, const int64_t* n, int dims) {     // offsets are formed in 64 bits; keep them far from the end
+    int64_t span = 0;
+    for (int i = 0; i < dims; ++i) {
+        if (st[i] < 0 || st[i] > ((int64_t)1 << 44)) return false;
+        span += st[i] * (n[i] > 0 ? n[i] - 1 : 0) / 4;
+        if (span > ((int64_t)1 << 56)) return false;
+    }
+    return true;
+}
+
+int check_rotary(const ptts_rotary* r, int head_dim) {
+    if (!r->cos_t || !r->sin_t) REFUSE(PTTS_E_INVALID, "rotary: null table");
+    if (r->positions <= 0) REFUSE(PTTS_E_INVALID, "rotary: %d positions", r->positions);
+    if (r->dims <= 0 || r->dims % 2 || r->dims > head_dim) REFUSE(PTTS_E_INVALID, "rotary: %d features of a head of %d", r->dims, head_dim);
+    return PTTS_OK;
+}
+
+int check_kv(const ptts_paged_kv* c) {
+    if (!c) REFUSE(PTTS_E_INVALID, "null cache");
+    if (c->dtype != PTTS_DTYPE_F32 && c->dtype != PTTS_DTYPE_BF16) REFUSE(PTTS_E_INVALID, "cache dtype must be 0 (f32) or 1 (bf16)");
+    if (!c->k || !c->v) REFUSE(PTTS_E_INVALID, "null cache tensor");
+    if (c->n_pages <= 0 || c->kv_heads <= 0) REFUSE(PTTS_E_INVALID, "cache of %d pages, %d heads", c->n_pages, c->kv_heads);
+    if (c->page_tokens < 16 || c->page_tokens > 4096 || (c->page_tokens & (c->page_tokens - 1)))
+        REFUSE(PTTS_E_UNSUPPORTED, "pages of %d tokens: a power of two from 16 to 4096 is served", c->page_tokens);
+    if (c->head_dim != 64 && c->head_dim != 128) REFUSE(PTTS_E_UNSUPPORTED, "head_dim %d: 64 and 128 are served", c->head_dim);
+    const int64_t n[3] = {c->n_pages, c->kv_heads, c->page_tokens};
+    if (!fits(c->k_strides, n, 3) || !fits(c->v_strides, n, 3)) REFUSE(PTTS_E_INVALID, "cache strides out of range");
+    if (overlaps_itself(c->k_strides, n, 3, c->head_dim) || overlaps_itself(c->v_strides, n, 3, c->head_dim))
+        REFUSE(PTTS_E_INVALID, "rows of the cache share elements");
+    const int esz = c->dtype == PTTS_DTYPE_BF16 ? 2 : 4;
+    if (!aligned(c->k, c->k_strides, 3, 16, esz) || !aligned(c->v, c->v_strides, 3, 16, esz))
+        REFUSE(PTTS_E_INVALID, "cache rows must start at multiples of 16 bytes");
+    return PTTS_OK;
+}
+
+int check_batch(const ptts_paged_batch* b) {
+    if (!b) REFUSE(PTTS_E_INVALID, "null batch");
+    if (b->n_seqs < 0 || b->tokens < 0 || b->max_pages < 0) REFUSE(PTTS_E_INVALID, "negative batch sizes");
+    if (b->n_seqs > 0 && (!b->past || (!b->table && b->max_pages > 0))) REFUSE(PTTS_E_INVALID, "null page table or lengths");
+    if (!b->starts && b->tokens != b->n_seqs) REFUSE(PTTS_E_INVALID, "%d tokens of %d sequences need starts", b->tokens, b->n_seqs);
+    if (b->table_stride < b->max_pages) REFUSE(PTTS_E_INVALID, "page table rows overlap");
+    if ((int64_t)b->table_stride > INT_MAX) REFUSE(PTTS_E_INVALID, "page table stride out of range");
+    return PTTS_OK;
+}
+
+int check_rows(const char* name, const void* p, const int64_t* st, int64_t tokens, int64_t heads, int64_t d, bool written) {
+    if (!p) REFUSE(PTTS_E_INVALID, "null %s", name);
+    const int64_t n[2] = {tokens, heads};
+    if (!fits(st, n, 2)) REFUSE(PTTS_E_INVALID, "%s: strides out of range", name);
+    if (written && overlaps_itself(st, n, 2, d)) REFUSE(PTTS_E_INVALID, "%s: rows share elements", name);
+    return PTTS_OK;
+}
+
+// byte range of a strided tensor of rows
+bool ranges_meet(const void* a, const int64_t* as, const void* b, const int64_t* bs, int64_t tokens, int64_t heads, int64_t d, int esz) {
+    const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
+    const uintptr_t ea = pa + (uintptr_t)(((tokens - 1) * as[0] + (heads - 1) * as[1] + d) * esz);
+    const uintptr_t eb = pb + (uintptr_t)(((tokens - 1) * bs[0] + (heads - 1) * bs[1] + d) * esz);
+    return pa < eb && pb < ea;
+}
+
+PagedBatchArgs batch_args(const ptts_paged_kv* c, const ptts_paged_batch* b) {
+    PagedBatchArgs r;
+    r.table = b->table; r.table_stride = b->table_stride; r.past = b->past; r.starts = b->starts;
+    r.max_pages = b->max_pages; r.n_pages = c->n_pages; r.n_seqs = b->n_seqs; r.tokens = b->tokens;
+    r.page_shift = __builtin_ctz((unsigned)c->page_tokens);
+    return r;
+}
+
+RotaryArgs rotary_args(const ptts_rotary* r) {
+    RotaryArgs a = {nullptr, nullptr, 0, 0, 0};
+    if (r) { a.cos_t = r->cos_t; a.sin_t = r->sin_t; a.positions = r->positions; a.dims = r->dims; a.interleaved = r->interleaved ? 1 : 0; }
+    return a;
+}
+
+#define TRY(expr)                       \
+    do {                                \
+        const int rc_ = (expr);         \
+        if (rc_ != PTTS_OK) return rc_; \
+    } while (0)
+
+int launched(const char* what, hipError_t e) {
+    if (e != hipSuccess) REFUSE(PTTS_E_HIP, "%s failed: %s", what, hipGetErrorString(e));
+    return PTTS_OK;
+}
+
+constexpr int MAX_UNITS = 32768;      // units of work of a token (SmallDiv)
+
+}  // namespace
+
+extern "C" {
+
+int ptts_rotary_embed(const ptts_rotary* rot, int32_t dtype, int32_t tokens, int32_t heads, int32_t head_dim, const void* x,
+                      int64_t x_token_stride, int64_t x_head_stride, const int32_t* positions, void* out, int64_t out_token_stride,
+                      int64_t out_head_stride, int32_t* status, void* stream) {
+    if (!rot || !status) REFUSE(PTTS_E_INVALID, "null argument");
+    if (dtype != PTTS_DTYPE_F32 && dtype != PTTS_DTYPE_BF16) REFUSE(PTTS_E_INVALID, "dtype must be 0 (f32) or 1 (bf16)");
+    if (tokens < 0 || heads <= 0 || head_dim <= 0 || head_dim % 2) REFUSE(PTTS_E_INVALID, "%d tokens of %d heads of %d", tokens, heads, head_dim);
+    if ((int64_t)heads * head_dim / 2 > MAX_UNITS) REFUSE(PTTS_E_UNSUPPORTED, "%d heads of %d: at most 65536 features a token", heads, head_dim);
+    TRY(check_rotary(rot, head_dim));
+    if (tokens == 0) return PTTS_OK;
+    if (!positions) REFUSE(PTTS_E_INVALID, "null positions");
+    RotaryEmbedArgs a;
+    a.x = x; a.out = out; a.xs[0] = x_token_stride; a.xs[1] = x_head_stride; a.os[0] = out_token_stride; a.os[1] = out_head_stride;
+    TRY(check_rows("x", x, a.xs, tokens, heads, head_dim, false));
+    TRY(check_rows("out", out, a.os, tokens, heads, head_dim, true));
+    const int esz = dtype == PTTS_DTYPE_BF16 ? 2 : 4;
+    if (!(x == out && a.xs[0] == a.os[0] && a.xs[1] == a.os[1]) && ranges_meet(x, a.xs, out, a.os, tokens, heads, head_dim, esz))
+        REFUSE(PTTS_E_INVALID, "x and out share memory in another layout than in place");
+    a.pos = positions; a.rot = rotary_args(rot); a.status = status; a.tokens = tokens; a.heads = heads; a.head_dim = head_dim;
+    return launched("ptts_rotary_embed", rotary_embed_launch(a, dtype, (hipStream_t)stream));
+}
+
+int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, int32_t dtype, const void* k, int64_t k_token_stride,
+                   int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, const ptts_rotary* rot,
+                   const int32_t* positions, int32_t q_heads, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
+                   int64_t q_out_token_stride, int64_t q_out_head_stride, int32_t* status, void* stream) {
+    TRY(check_kv(cache));
+    TRY(check_batch(batch));
+    if (!status) REFUSE(PTTS_E_INVALID, "null status");
+    if (dtype != PTTS_DTYPE_F32 && dtype != PTTS_DTYPE_BF16) REFUSE(PTTS_E_INVALID, "dtype must be 0 (f32) or 1 (bf16)");
+    if (dtype == PTTS_DTYPE_BF16 && cache->dtype != PTTS_DTYPE_BF16) REFUSE(PTTS_E_UNSUPPORTED, "bf16 rows into an f32 cache");
+    if (rot) TRY(check_rotary(rot, cache->head_dim));
+    if (q_heads < 0 || (q_heads == 0) != (q == nullptr) || (q_heads == 0) != (q_out == nullptr)) REFUSE(PTTS_E_INVALID, "q: %d heads", q_heads);
+    const int64_t T = batch->tokens, D = cache->head_dim;
+    if (((int64_t)q_heads + 2 * (int64_t)cache->kv_heads) * D / 2 > MAX_UNITS)
+        REFUSE(PTTS_E_UNSUPPORTED, "%d query and %d key heads of %d: at most 65536 features a token", q_heads, cache->kv_heads, cache->head_dim);
+    if (T == 0 || batch->n_seqs == 0) return PTTS_OK;
+    AppendArgs a;
+    a.q = q; a.k = k; a.v = v; a.q_out = q_out; a.k_cache = cache->k; a.v_cache = cache->v;
+    a.qs[0] = q_token_stride; a.qs[1] = q_head_stride; a.qos[0] = q_out_token_stride; a.qos[1] = q_out_head_stride;
+    a.ks[0] = k_token_stride; a.ks[1] = k_head_stride; a.vs[0] = v_token_stride; a.vs[1] = v_head_stride;
+    TRY(check_rows("k", k, a.ks, T, cache->kv_heads, D, false));
+    TRY(check_rows("v", v, a.vs, T, cache->kv_heads, D, false));
+    if (q_heads) {
+        const int esz = dtype == PTTS_DTYPE_BF16 ? 2 : 4;
+        TRY(check_rows("q", q, a.qs, T, q_heads, D, false));
+        TRY(check_rows("q_out", q_out, a.qos, T, q_heads, D, true));
+        if (!(q == q_out && a.qs[0] == a.qos[0] && a.qs[1] == a.qos[1]) && ranges_meet(q, a.qs, q_out, a.qos, T, q_heads, D, esz))
+            REFUSE(PTTS_E_INVALID, "q and q_out share memory in another layout than in place");
+    }
+    for (int i = 0; i < 3; ++i) { a.kc[i] = cache->k_strides[i]; a.vc[i] = cache->v_strides[i]; }
+    a.b = batch_args(cache, batch); a.rot = rotary_args(rot); a.pos = rot ? positions : nullptr; a.status = status;
+    a.q_heads = q_heads; a.kv_heads = cache->kv_heads; a.head_dim = cache->head_dim;
+    return launched("ptts_kv_append", kv_append_launch(a, dtype, cache->dtype, (hipStream_t)stream));
+}
+
+}  // extern "C"
+
+namespace {
+int attn_args(const ptts_paged_kv* cache, const ptts_paged_batch* batch, int32_t q_heads, int32_t max_new, PagedAttnArgs* a) {
+    TRY(check_kv(cache));
+    TRY(check_batch(batch));
+    if (q_heads <= 0 || q_heads % cache->kv_heads) REFUSE(PTTS_E_INVALID, "%d query heads over %d key heads", q_heads, cache->kv_heads);
+    if (q_heads > 65535) REFUSE(PTTS_E_UNSUPPORTED, "%d query heads", q_heads);
+    if (max_new < 0) REFUSE(PTTS_E_INVALID, "max_new %d", max_new);
+    if ((int64_t)batch->max_pages * cache->page_tokens > INT_MAX - 4096) REFUSE(PTTS_E_UNSUPPORTED, "a page table row reaches past 2^31 tokens");
+    if ((int64_t)batch->tokens * (q_heads / cache->kv_heads) > INT_MAX - 65536) REFUSE(PTTS_E_UNSUPPORTED, "too many query rows");
+    *a = PagedAttnArgs();
+    a->k = cache->k; a->v = cache->v;
+    for (int i = 0; i < 3; ++i) { a->kc[i] = cache->k_strides[i]; a->vc[i] = cache->v_strides[i]; }
+    const PagedBatchArgs b = batch_args(cache, batch);
+    a->table = b.table; a->table_stride = b.table_stride; a->past = b.past; a->starts = b.starts;
+    a->max_pages = b.max_pages; a->n_pages = b.n_pages; a->page_shift = b.page_shift; a->n_seqs = b.n_seqs; a->tokens = b.tokens;
+    a->q_heads = q_heads; a->kv_heads = cache->kv_heads; a->group = q_heads / cache->kv_heads;
+    return PTTS_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int64_t ptts_paged_attention_workspace(const ptts_paged_kv* cache, const ptts_paged_batch* batch, int32_t q_heads, int32_t max_new) {
+    PagedAttnArgs a;
+    TRY(attn_args(cache, batch, q_heads, max_new, &a));
+    if (a.tokens == 0 || a.n_seqs == 0) return 0;
+    return paged_attn_workspace(a, max_new, cache->head_dim, cache->dtype);
+}
+
+int ptts_paged_attention(const ptts_paged_kv* cache, const ptts_paged_batch* batch, int32_t q_heads, const void* q, int64_t q_token_stride,
+                         int64_t q_head_stride, void* out, int64_t out_token_stride, int64_t out_head_stride, float scale, int32_t causal,
+                         const uint8_t* key_mask, int64_t mask_stride, int32_t mask_width, int32_t max_new, void* workspace,
+                         int64_t workspace_bytes, int32_t* status, void* stream) {
+    PagedAttnArgs a;
+    TRY(attn_args(cache, batch, q_heads, max_new, &a));
+    if (!status) REFUSE(PTTS_E_INVALID, "null status");
+    if (!(scale > 0.f) || !std::isfinite(scale)) REFUSE(PTTS_E_INVALID, "softmax scale must be positive and finite");
+    if (key_mask && (mask_width < 0 || mask_stride < mask_width)) REFUSE(PTTS_E_INVALID, "key mask of %d columns", mask_width);
+    const int64_t T = batch->tokens, D = cache->head_dim;
+    if (T == 0 || batch->n_seqs == 0) return PTTS_OK;
+    a.q = q; a.out = out;
+    a.qs[0] = q_token_stride; a.qs[1] = q_head_stride; a.os[0] = out_token_stride; a.os[1] = out_head_stride;
+    TRY(check_rows("q", q, a.qs, T, q_heads, D, false));
+    TRY(check_rows("out", out, a.os, T, q_heads, D, true));
+    const int esz = cache->dtype == PTTS_DTYPE_BF16 ? 2 : 4;
+    if (!aligned(q, a.qs, 2, 16, esz) || !aligned(out, a.os, 2, 16, esz)) REFUSE(PTTS_E_INVALID, "rows of q and out must start at multiples of 16 bytes");
+    if (ranges_meet(q, a.qs, out, a.os, T, q_heads, D, esz)) REFUSE(PTTS_E_INVALID, "q and out share memory");
+    a.mask = key_mask && mask_width > 0 ? key_mask : nullptr; a.mask_stride = mask_stride; a.mask_width = a.mask ? mask_width : 0;
+    a.scale_log2 = scale * 1.4426950408889634f; a.causal = causal ? 1 : 0; a.status = status;
+    const int64_t need = paged_attn_workspace(a, max_new, cache->head_dim, cache->dtype);
+    if (need > 0 && (!workspace || workspace_bytes < need)) REFUSE(PTTS_E_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+    if ((uintptr_t)workspace % 16) REFUSE(PTTS_E_INVALID, "workspace must start at a multiple of 16 bytes");
+    a.part = (float*)workspace;
+    return launched("ptts_paged_attention", paged_attn_launch(a, max_new, cache->head_dim, cache->dtype, (hipStream_t)stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,332 @@
+"""Operators over a paged KV cache of the caller's: rotary positions, the append of new keys and values, the attention over them.
+
+The engine behind ``generate()`` keeps its cache to itself.  These are the same steps for a cache, a page table and a ragged batch that
+the caller owns (grouped heads, head dim 64 or 128, float32 or bfloat16), as calls on PyTorch tensors:
+
+    cache  = PagedKVCache(num_pages, page_tokens, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda")
+    rotary = RotaryTable(head_dim, max_positions)
+    q = kv_append(cache, k, v, table, past, starts, rotary=rotary, q=q)      # store k (turned) and v, turn q
+    o = paged_attention(q, cache, table, past, starts)
+
+``table`` [sequences, pages] int32 lists every sequence's pages, ``past`` [sequences] int32 how many of its tokens the cache held before
+this call, ``starts`` [sequences + 1] int32 where its new tokens begin in q / k / v (None: one new token each).  They are read on the
+device when the work runs, so a captured graph serves other lengths after an in-place update.  What they say wrongly is never followed
+out of a buffer: it sets ``cache.status`` / ``rotary.status``, which ``check()`` turns into an error, and the rows concerned come out as
+zeros (``kv_append``, ``rotary_embed``) or NaN (``paged_attention``).
+
+Work goes to the current stream of the tensors' device and nothing is synchronised.  No gradients: forward only.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Any, Dict, Optional
+
+import torch
+
+from . import _hip
+
+_DTYPES = {torch.float32: _hip.DTYPE_F32, torch.bfloat16: _hip.DTYPE_BF16}
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+class _OnDevice:
+    """makes `device` the current one for a launch if it is not; the current stream of it is `stream`"""
+
+    def __init__(self, device: torch.device):
+        self.other = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self) -> int:
+        if self.other is not None:
+            self.other.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.other is not None:
+            self.other.__exit__(*exc)
+
+
+def _read_status(status: torch.Tensor, who: str) -> None:
+    bits = int(status.item())
+    if bits:
+        status.zero_()
+        raise _hip.PttsError(-1, f"{who}: " + "; ".join(t for b, t in _hip.PAGED_STATUS.items() if bits & b))
+
+
+def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optional[Dict[str, Any]] = None):
+    """(angle per position of every pair, float64 [rotary_dim / 2]; factor on cos and sin) of rotary positions.
+
+    ``scaling`` stretches them to contexts longer than the model was trained on (factor s > 0):
+      None                                       f_i = theta^(-2 i / rotary_dim)
+      {"type": "linear", "factor": s}            f_i / s: positions interpolated
+      {"type": "ntk", "factor": s}               theta * s^(r / (r - 2)) in theta's place: the slowest pair interpolated, the fastest kept
+      {"type": "yarn", "factor": s, "original_positions": L [, "beta_fast": 32, "beta_slow": 1, "attention_factor": a]}
+          pairs that turn more than beta_fast times within L positions kept, those below beta_slow interpolated, linear in the number
+          of turns between; cos and sin times a = 0.1 ln s + 1 (Peng et al., "YaRN: Efficient Context Window Extension", 2023)
+    """
+    _need(isinstance(rotary_dim, int) and rotary_dim > 0 and rotary_dim % 2 == 0, f"rotary_dim {rotary_dim}: a positive even number")
+    _need(theta > 0 and math.isfinite(theta), f"theta {theta}")
+    given = dict(scaling or {"type": "none"})
+    kind = given.pop("type", None)
+    known = {"none": (), "linear": ("factor",), "ntk": ("factor",),
+             "yarn": ("factor", "original_positions", "beta_fast", "beta_slow", "attention_factor")}
+    _need(kind in known, f"rotary scaling type {kind!r}: one of {sorted(known)}")
+    _need(set(given) <= set(known[kind]), f"rotary scaling {kind!r} takes {known[kind]}, got {sorted(given)}")
+    _need(kind == "none" or "factor" in given, f"rotary scaling {kind!r} needs a factor")
+    s = float(given.get("factor", 1.0))
+    _need(s > 0 and math.isfinite(s), f"rotary scaling factor {s}")
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    if kind == "ntk":
+        _need(rotary_dim > 2, "ntk scaling needs more than one pair")
+        theta = theta * s ** (rotary_dim / (rotary_dim - 2))
+    freq, gain = theta ** (-2.0 * i / rotary_dim), 1.0
+    if kind == "linear":
+        freq = freq / s
+    elif kind == "yarn":
+        fast, slow = float(given.get("beta_fast", 32.0)), float(given.get("beta_slow", 1.0))
+        _need("original_positions" in given and given["original_positions"] > 0, "yarn scaling needs original_positions")
+        _need(fast > slow, "yarn scaling needs beta_fast > beta_slow")
+        keep = ((given["original_positions"] * freq / (2 * math.pi) - slow) / (fast - slow)).clamp(0.0, 1.0)
+        freq = keep * freq + (1.0 - keep) * freq / s
+        gain = given.get("attention_factor")
+        gain = 0.1 * math.log(s) + 1.0 if gain is None else float(gain)
+    return freq, gain
+
+
+class RotaryTable:
+    """cos and sin of every position's angles, float32 on the device from float64 angles; made once, kept with the model.
+
+    ``layout``: "half" turns the pairs (i, i + rotary_dim / 2), "interleaved" the pairs (2 i, 2 i + 1) of the first ``rotary_dim`` (default:
+    all) features of a head; the rest pass as they are."""
+
+    def __init__(self, head_dim: int, positions: int, *, theta: float = 10000.0, rotary_dim: Optional[int] = None, layout: str = "half",
+                 scaling: Optional[Dict[str, Any]] = None, device="cuda"):
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        _need(layout in ("half", "interleaved"), f"layout {layout!r}: 'half' or 'interleaved'")
+        _need(0 < positions < 2 ** 31, f"positions {positions}")
+        _need(head_dim > 0 and head_dim % 2 == 0 and rotary_dim <= head_dim, f"rotary_dim {rotary_dim} of a head of {head_dim}")
+        freq, gain = rotary_frequencies(rotary_dim, theta, scaling)
+        angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq.to(device)
+        self.cos, self.sin = (torch.cos(angle) * gain).float(), (torch.sin(angle) * gain).float()
+        self.head_dim, self.positions, self.rotary_dim, self.layout = head_dim, positions, rotary_dim, layout
+        self.device = self.cos.device
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._c = _hip.PttsRotary(self.cos.data_ptr(), self.sin.data_ptr(), positions, rotary_dim, 1 if layout == "interleaved" else 0)
+        self._ref = C.addressof(self._c)
+
+    def check(self) -> None:
+        """waits for the device; raises if a call since the last check met a position outside the table"""
+        _read_status(self.status, "rotary_embed")
+
+
+class PagedKVCache:
+    """One layer's keys and values in pages: ``k``, ``v`` [pages, kv_heads, page_tokens, head_dim]."""
+
+    def __init__(self, num_pages: int, page_tokens: int, kv_heads: int, head_dim: int, *, dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        shape = (num_pages, kv_heads, page_tokens, head_dim)
+        self._adopt(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+
+    @classmethod
+    def from_tensors(cls, k: torch.Tensor, v: torch.Tensor) -> "PagedKVCache":
+        """around tensors (or views: any strides of the first three dimensions) the caller already has"""
+        self = cls.__new__(cls)
+        self._adopt(k, v)
+        return self
+
+    def _adopt(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        _need(k.dim() == 4 and k.shape == v.shape, f"k {tuple(k.shape)} and v {tuple(v.shape)}: [pages, kv_heads, page_tokens, head_dim] each")
+        _need(k.dtype in _DTYPES and k.dtype == v.dtype, f"a cache of {k.dtype} / {v.dtype}: float32 or bfloat16")
+        _need(k.device.type == "cuda" and k.device == v.device, "the cache has to be on one ROCm device")
+        _need(k.stride(3) == 1 and v.stride(3) == 1, "the features of a cache row have to be contiguous")
+        pages, heads, tokens, dim = k.shape
+        _need(pages > 0 and heads > 0, f"a cache of {pages} pages and {heads} heads")
+        _need(16 <= tokens <= 4096 and tokens & (tokens - 1) == 0, f"pages of {tokens} tokens: a power of two from 16 to 4096 is served")
+        _need(dim in (64, 128), f"head_dim {dim}: 64 and 128 are served")
+        self.k, self.v = k, v
+        self.num_pages, self.kv_heads, self.page_tokens, self.head_dim = pages, heads, tokens, dim
+        self.dtype, self.device = k.dtype, k.device
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._c = _hip.PttsPagedKV(k.data_ptr(), v.data_ptr(), (C.c_int64 * 3)(*k.stride()[:3]), (C.c_int64 * 3)(*v.stride()[:3]),
+                                   _DTYPES[k.dtype], pages, heads, tokens, dim)
+        self._ref = C.addressof(self._c)
+        self._workspace: Dict[tuple, int] = {}      # bytes by sizes
+
+    def check(self) -> None:
+        """waits for the device; raises if a call since the last check met a page, length, position or start it could not follow"""
+        _read_status(self.status, "paged cache")
+
+
+def _rows(name: str, t: torch.Tensor, tokens: Optional[int], heads: Optional[int], dim: int, device: torch.device) -> None:
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or (tokens is not None and shape[0] != tokens) or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} {tuple(shape)}: [{'tokens' if tokens is None else tokens}, {'heads' if heads is None else heads}, {dim}] expected")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.stride(2) != 1:
+        raise ValueError(f"the features of a row of {name} have to be contiguous")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient; this operator has none (torch.no_grad(), or detach it)")
+
+
+def _ints(name: str, t: torch.Tensor, dims: int, device: torch.device) -> None:
+    if t.dtype != torch.int32 or t.dim() != dims or t.device != device or (t.numel() > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name} has to be a contiguous int32 tensor of {dims} dimension(s) on {device}")
+
+
+def _batch(cache: PagedKVCache, tokens: int, table: torch.Tensor, past: torch.Tensor, starts: Optional[torch.Tensor]):
+    device = cache.device
+    _ints("table", table, 2, device)
+    _ints("past", past, 1, device)
+    n = past.shape[0]
+    rows, width = table.shape
+    if rows != n:
+        raise ValueError(f"a page table of {rows} rows for {n} sequences")
+    at = None
+    if starts is not None:
+        _ints("starts", starts, 1, device)
+        if starts.shape[0] != n + 1:
+            raise ValueError(f"starts of {starts.shape[0]} entries for {n} sequences: one more than sequences")
+        at = starts.data_ptr()
+    elif tokens != n:
+        raise ValueError(f"{tokens} tokens of {n} sequences: starts says whose they are")
+    stride = table.stride(0) if rows > 1 else width
+    return _hip.PttsPagedBatch(table.data_ptr(), stride, past.data_ptr(), at, width, n, tokens)
+
+
+def rotary_embed(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x`` [tokens, heads, head_dim] (float32 or bfloat16) turned by ``positions`` [tokens] int32 -> ``out`` (may be ``x``).
+    A row whose position is outside the table becomes zero, and ``rotary.check()`` raises."""
+    tokens, heads = x.shape[0], x.shape[1] if x.dim() == 3 else None
+    _rows("x", x, None, None, rotary.head_dim, rotary.device)
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"x of {x.dtype}: float32 or bfloat16")
+    _ints("positions", positions, 1, rotary.device)
+    if positions.shape[0] != tokens:
+        raise ValueError(f"{positions.shape[0]} positions for {tokens} tokens")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        _rows("out", out, tokens, heads, rotary.head_dim, rotary.device)
+        if out.dtype != x.dtype:
+            raise ValueError(f"out of {out.dtype} for x of {x.dtype}")
+    if heads == 0 or tokens == 0:
+        return out
+    xs, os = x.stride(), out.stride()
+    with _OnDevice(rotary.device) as stream:
+        _hip.check(_hip.load_library().ptts_rotary_embed(
+            rotary._ref, _DTYPES[x.dtype], tokens, heads, rotary.head_dim, x.data_ptr(), xs[0], xs[1], positions.data_ptr(), out.data_ptr(),
+            os[0], os[1], rotary.status.data_ptr(), stream))
+    return out
+
+
+def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, past: torch.Tensor,
+              starts: Optional[torch.Tensor] = None, *, rotary: Optional[RotaryTable] = None, positions: Optional[torch.Tensor] = None,
+              q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Stores ``k``, ``v`` [tokens, kv_heads, head_dim]: token i of sequence s at slot ``past[s] + i``, k turned by ``rotary`` at that
+    position (or at ``positions`` [tokens] int32).  ``q`` [tokens, heads, head_dim] is turned in the same launch into ``q_out`` (may be ``q``),
+    which is returned.  float32 rows may be stored in a bfloat16 cache.  Rows behind the last sequence are left alone, in ``q_out`` too."""
+    device = cache.device
+    tokens = k.shape[0]
+    _rows("k", k, tokens, cache.kv_heads, cache.head_dim, device)
+    _rows("v", v, tokens, cache.kv_heads, cache.head_dim, device)
+    if k.dtype not in _DTYPES or v.dtype != k.dtype or (k.dtype != cache.dtype and k.dtype != torch.float32):
+        raise ValueError(f"k of {k.dtype} and v of {v.dtype} for a cache of {cache.dtype}")
+    batch = _batch(cache, tokens, table, past, starts)
+    rot = at = None
+    if rotary is not None:
+        if rotary.device != device or rotary.head_dim != cache.head_dim:
+            raise ValueError(f"a rotary table for heads of {rotary.head_dim} on {rotary.device}; the cache has {cache.head_dim} on {device}")
+        rot = rotary._ref
+    if positions is not None:
+        if rotary is None:
+            raise ValueError("positions without a rotary table")
+        _ints("positions", positions, 1, device)
+        if positions.shape[0] != tokens:
+            raise ValueError(f"{positions.shape[0]} positions for {tokens} tokens")
+        at = positions.data_ptr()
+    ks, vs = k.stride(), v.stride()
+    heads, qp, qop, qs, qos = 0, None, None, (0, 0), (0, 0)
+    if q is not None:
+        _rows("q", q, tokens, None, cache.head_dim, device)
+        heads = q.shape[1]
+        if q.dtype != k.dtype or heads == 0:
+            raise ValueError(f"q {tuple(q.shape)} of {q.dtype} beside k of {k.dtype}")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        else:
+            _rows("q_out", q_out, tokens, heads, cache.head_dim, device)
+            if q_out.dtype != q.dtype:
+                raise ValueError(f"q_out of {q_out.dtype} for q of {q.dtype}")
+        qp, qop, qs, qos = q.data_ptr(), q_out.data_ptr(), q.stride(), q_out.stride()
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    if tokens == 0:
+        return q_out
+    with _OnDevice(device) as stream:
+        _hip.check(_hip.load_library().ptts_kv_append(
+            cache._ref, C.addressof(batch), _DTYPES[k.dtype], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], rot, at,
+            heads, qp, qs[0], qs[1], qop, qos[0], qos[1], cache.status.data_ptr(), stream))
+    return q_out
+
+
+def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, past: torch.Tensor, starts: Optional[torch.Tensor] = None, *,
+                    scale: Optional[float] = None, causal: bool = True, key_mask: Optional[torch.Tensor] = None, max_new: int = 0,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale * q k^T) v over the cache -> [tokens, heads, head_dim], ``scale`` by default head_dim^-0.5.
+
+    causal: token i of sequence s sees the keys 0 .. past[s] + i (its own among them: append first); otherwise every token sees the keys
+    0 .. past[s] - 1 (states that were cached once, as a cross-attention reads them).  ``key_mask`` [sequences, columns] bool: a False
+    column is no key, whatever the cache holds there; keys behind its last column are seen.  A token without keys gets zeros.
+    ``q``'s heads are a multiple of the cache's, in groups: head h reads key head h // (heads / kv_heads).
+    ``max_new``: the longest sequence's number of new tokens if the caller knows it (it helps to pick the kernel; 0: unknown).
+    Rows behind the last sequence are left as they are in ``out``."""
+    device, dim = cache.device, cache.head_dim
+    tokens = q.shape[0]
+    _rows("q", q, None, None, dim, device)
+    heads = q.shape[1]
+    if q.dtype != cache.dtype:
+        raise ValueError(f"q of {q.dtype} over a cache of {cache.dtype}")
+    if heads == 0 or heads % cache.kv_heads:
+        raise ValueError(f"{heads} query heads over {cache.kv_heads} key heads")
+    batch = _batch(cache, tokens, table, past, starts)
+    mask, mask_stride, mask_width = None, 0, 0
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.dim() != 2 or key_mask.shape[0] != past.shape[0] or \
+                key_mask.device != device or (key_mask.shape[1] > 1 and key_mask.stride(1) != 1):
+            raise ValueError(f"key_mask has to be a bool tensor [{past.shape[0]}, columns] on {device}")
+        mask_width = key_mask.shape[1]
+        mask, mask_stride = key_mask.data_ptr() if mask_width else None, max(key_mask.stride(0), mask_width)
+        if key_mask.shape[0] > 1 and key_mask.stride(0) < mask_width:
+            key_mask = key_mask.contiguous()          # one row for every sequence, expanded
+            mask = key_mask.data_ptr()
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    else:
+        _rows("out", out, tokens, heads, dim, device)
+        if out.dtype != q.dtype:
+            raise ValueError(f"out of {out.dtype} for q of {q.dtype}")
+    if tokens == 0:
+        return out
+    lib = _hip.load_library()
+    bref = C.addressof(batch)
+    key = (tokens, batch.n_seqs, batch.max_pages, heads, max_new, starts is None)
+    need = cache._workspace.get(key)
+    if need is None:
+        need = lib.ptts_paged_attention_workspace(cache._ref, bref, heads, max_new)
+        if need < 0:
+            _hip.check(int(need))
+        if len(cache._workspace) > 4096:
+            cache._workspace.clear()
+        cache._workspace[key] = need
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    qs, os = q.stride(), out.stride()
+    with _OnDevice(device) as stream:
+        _hip.check(lib.ptts_paged_attention(
+            cache._ref, bref, heads, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], dim ** -0.5 if scale is None else scale,
+            1 if causal else 0, mask, mask_stride, mask_width, max_new, workspace.data_ptr() if need else None, need,
+            cache.status.data_ptr(), stream))
+    return out
