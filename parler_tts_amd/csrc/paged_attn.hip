@@ -1,9 +1,31 @@
 // Attention of new tokens over a paged KV cache: o_i = sum_j softmax_j(scale * q_i . k_j) v_j over the keys j a query may see.
+//
+// Both kernels make ONE pass over the keys with the running maximum and sum of the softmax, and both hold the scores TRANSPOSED:
+// S^T = K Q^T puts a query into a column, so that a lane owns one query and a few of its scores; the maximum is a register maximum
+// plus one or two lane swaps, the running state is one register per lane, and the probabilities are already the B operand of
+// O^T = V^T P^T when the keys of a matrix step are numbered as the accumulator left them (key 8 (j / 4) + 4 h + j % 4 in slot j of
+// half h: any numbering serves as long as V^T uses the same one).  V^T comes out of LDS by transposing reads (bf16) or plain
+// dword reads (f32: a lane reads its feature of the slot's key).
+//   * "rows" of a (sequence, key head) are its new tokens times the query heads of the group: a page is read once for all of them;
+//   * K and V travel to LDS by LDS-DMA, 16 bytes a lane, 16-byte chunks XOR-swizzled by the row so that neither the row-wise reads
+//     of K nor the transposing reads of V meet in a bank;
+//   * scores, maxima, sums and outputs are 32 bits; in bf16 the probabilities are rounded once (half a bf16 step of each, the type
+//     of V and of the result) to enter the matrix unit.
+//
+// A value that is not finite in a row that some queries may not see would reach them as 0 * inf in the matrix unit.  Nothing in the
+// loops guards against it: a query whose result is not finite is computed again, alone, over the keys it sees (row_alone).
 #include "ptts_common.h"
 #include "gemm.h"
 #include "paged.h"
 
 namespace {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+
+template <int N> __device__ inline void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ inline void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 template <typename P> __device__ inline void load16(const typename P::elem_t* p, float* f);
 template <> __device__ inline void load16<PBF16>(const uint16_t* p, float* f) {
@@ -20,94 +42,497 @@ template <> __device__ inline void load16<PF32>(const float* p, float* f) {
     f[0] = r[0]; f[1] = r[1]; f[2] = r[2]; f[3] = r[3];
 }
 
-// One wave per (token, query head), 64 keys a time: a lane takes one key's score, then the lanes are the features of the output.
+__device__ inline float swap_max32(float x) {      // maximum over lanes l and l ^ 32
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+    const unsigned r0 = r[0], r1 = r[1];
+    return fmaxf(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+#else
+    return x;
+#endif
+}
+__device__ inline float exp2_hw(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_exp2f(x);
+#else
+    return x;
+#endif
+}
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// ---- where a workgroup's rows lie ------------------------------------------------------------------------------------------
+struct Span {          // one sequence's new tokens
+    int seq, first, n, past;
+    bool bad;          // its length leads behind its row of the page table: every row becomes NaN
+};
+
+// The sequence of tile t of a launch whose tiles hold M rows: sequence s owns the tiles floor(starts[s] group / M) + s and on (at
+// least as many as its rows need, whatever lies in front of it), so no prefix sum over the batch is needed.  64-ary search, one wave.
+__device__ inline bool find_tile(const PagedAttnArgs& a, int t, int M, Span* sp, int* tile) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, len = a.n_seqs;
+    for (;;) {
+        const int step = (len + 63) >> 6, i = lo + lane * step;
+        bool le = false;
+        if (i < lo + len) le = (int64_t)(a.starts ? a.starts[i] : i) * a.group / M + i <= t;
+        const int c = __popcll(__ballot(le));
+        if (c == 0) return false;
+        const int end = lo + len;
+        lo += (c - 1) * step;
+        len = min(step, end - lo);
+        if (len <= 1) break;
+    }
+    lo = uniform(lo);
+    sp->seq = lo;
+    sp->first = a.starts ? uniform(a.starts[lo]) : lo;
+    const int end = a.starts ? uniform(a.starts[lo + 1]) : lo + 1;
+    sp->n = end - sp->first;
+    if (sp->first < 0 || end > a.tokens || sp->n <= 0) return false;
+    *tile = t - (int)((int64_t)sp->first * a.group / M + lo);
+    if ((int64_t)*tile * M >= (int64_t)sp->n * a.group) return false;
+    return true;
+}
+
+__device__ inline void read_past(const PagedAttnArgs& a, Span* sp) {
+    sp->past = uniform(a.past[sp->seq]);
+    const int64_t reach = (int64_t)a.max_pages << a.page_shift;
+    sp->bad = sp->past < 0 || (int64_t)sp->past + (a.causal ? sp->n : 0) > reach;
+    if (sp->bad) {
+        if (threadIdx.x == 0) atomicOr(a.status, PAGED_BAD_LENGTH);
+        sp->past = 0;
+    }
+}
+
+// ---- page ids of the keys ahead, one per lane ---------------------------------------------------------------------------------
+struct Pages {
+    const int* row;
+    int base, ids, n_pages;     // lane l holds the id of page base + l
+    bool bad;
+    __device__ inline void load(int first, int last) {       // pages first .. (at most 64), none behind `last`
+        base = first;
+        const int i = first + (int)(threadIdx.x & 63);
+        ids = row[min(i, last)];
+        const bool wrong = (unsigned)ids >= (unsigned)n_pages;
+        bad = bad || __any(wrong);
+        if (wrong) ids = 0;
+    }
+    __device__ inline int get(int page) const { return __builtin_amdgcn_readlane(ids, page - base); }
+};
+
+// ---- a tile of KT rows of K or V on its way to LDS: one wave moves ROWS of them -------------------------------------------------
+// chunk c (16 bytes) of row r stands at chunk c ^ (r & 7) of the row's LDS image.  Rows at or behind `end` are read from the last row
+// in front of it: what lies there is seen by nobody, and may be anything.
+template <typename P, int D, int ROWS>
+__device__ inline void dma_rows(const char* base, int64_t page_bytes, int64_t slot_bytes, const Pages& pg, int page_shift, int key0, int row0,
+                                int end, char* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef __attribute__((address_space(3))) void lds_void;
+    constexpr int RB = D * (int)sizeof(typename P::elem_t), RPI = 1024 / RB, CPR = RB / 16;
+    const int lane = threadIdx.x & 63, rl = lane / CPR, c = lane % CPR;
+    const int mask = (1 << page_shift) - 1;
+#pragma unroll
+    for (int i = 0; i < ROWS / RPI; ++i) {
+        const int r = row0 + i * RPI;                                   // first row of this instruction: its rows share a page
+        const int page = pg.get(min(key0 + r, end - 1) >> page_shift);
+        const int slot = min(key0 + r + rl, end - 1) & mask;
+        const char* src = base + page * page_bytes + slot * slot_bytes + ((c ^ ((r + rl) & 7)) << 4);
+        __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(src), (lds_void*)(lds + r * RB), 16, 0, 0);
+    }
+#endif
+}
+
+// keys that may be looked at at all, as bits: the key mask's bytes of the tile (lane i: key key0 + i), ones behind its last column
+__device__ inline uint64_t tile_mask(const PagedAttnArgs& a, int seq, int key0) {
+    if (!a.mask || key0 >= a.mask_width) return ~0ull;
+    const int j = key0 + (int)(threadIdx.x & 63);
+    bool live = true;
+    if (j < a.mask_width) live = a.mask[seq * a.mask_stride + j] != 0;
+    return __ballot(live);
+}
+
+// ---- one query over the keys [k0, k1) it sees, by one wave (see the head of the file) ------------------------------------------
 template <typename P, int D>
-__global__ __launch_bounds__(64) void paged_attn_simple_kernel(PagedAttnArgs a) {
+__device__ inline void row_alone(const PagedAttnArgs& a, int seq, int kvh, const typename P::elem_t* q, int k0, int k1, float* m_out, float* l_out,
+                                 float (&acc)[D / 64]) {
     typedef typename P::elem_t elem_t;
     constexpr int V = 16 / sizeof(elem_t), R = D / 64;
-    __shared__ float qs[D];
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    if (t == 0 && h == 0 && a.starts) check_starts(a.starts, a.n_seqs, a.tokens, a.status);
-    int s = t, first = t, end = t + 1;
-    if (a.starts) {
-        int lo = 0, hi = a.n_seqs;                    // largest s with starts[s] <= t
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.starts[mid] <= t) lo = mid; else hi = mid;
-        }
-        s = lo; first = a.starts[s]; end = a.starts[s + 1];
-        if (t < first || t >= end) return;            // behind the last sequence
-    }
-    const int past = a.past[s], reach = a.max_pages << a.page_shift;
-    bool bad = past < 0 || first < 0 || end > a.tokens;
-    const int64_t see = (int64_t)past + (a.causal ? t - first + 1 : 0);
-    int lim = see > reach ? 0 : (int)see;
-    if (bad || see > reach) { if (lane == 0) atomicOr(a.status, first < 0 || end > a.tokens ? PAGED_BAD_STARTS : PAGED_BAD_LENGTH); bad = true; lim = 0; }
-    const elem_t* qp = reinterpret_cast<const elem_t*>(a.q) + t * a.qs[0] + h * a.qs[1];
-    for (int d = lane; d < D; d += 64) qs[d] = from_elem<P>(qp[d]);
-    __syncthreads();
-    const int kvh = h / a.group;
+    const int lane = threadIdx.x & 63, mask = (1 << a.page_shift) - 1;
     const elem_t* kb = reinterpret_cast<const elem_t*>(a.k) + kvh * a.kc[1];
     const elem_t* vb = reinterpret_cast<const elem_t*>(a.v) + kvh * a.vc[1];
-    const int* table = a.table + s * a.table_stride;
-    float m = -INFINITY, l = 0.f, acc[R];
+    const int* table = a.table + seq * a.table_stride;
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) acc[r] = 0.f;
-    for (int j0 = 0; j0 < lim; j0 += 64) {
+    for (int j0 = k0; j0 < k1; j0 += 64) {
         const int j = j0 + lane;
         float sc = -INFINITY;
         int page = -1;
-        if (j < lim) {
+        if (j < k1 && (!a.mask || j >= a.mask_width || a.mask[seq * a.mask_stride + j])) {
             page = table[j >> a.page_shift];
-            const bool ok = (unsigned)page < (unsigned)a.n_pages;
-            if (!ok) { atomicOr(a.status, PAGED_BAD_PAGE); bad = true; }
-            const bool live = ok && (!a.mask || j >= a.mask_width || a.mask[s * a.mask_stride + j]);
-            if (live) {
-                const elem_t* kp = kb + page * a.kc[0] + (j & ((1 << a.page_shift) - 1)) * a.kc[2];
-                float d = 0.f;
-                for (int c = 0; c < D; c += V) {
-                    float f[V];
-                    load16<P>(kp + c, f);
+            if ((unsigned)page >= (unsigned)a.n_pages) page = 0;        // the caller of this has found it already
+            const elem_t* kp = kb + page * a.kc[0] + (j & mask) * a.kc[2];
+            float d = 0.f;
+            for (int c = 0; c < D; c += V) {
+                float x[V], y[V];
+                load16<P>(q + c, x);
+                load16<P>(kp + c, y);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) d = fmaf(qs[c + i], f[i], d);
-                }
-                sc = d * a.scale_log2;
-            } else page = -1;
+                for (int i = 0; i < V; ++i) d = fmaf(x[i], y[i], d);
+            }
+            sc = d * a.scale_log2;
         }
-        const float mn = fmaxf(m, wave_max(sc));
-        const float mu = mn == -INFINITY ? 0.f : mn;
-        const float p = page >= 0 ? exp2f(sc - mu) : 0.f, al = exp2f(m - mu);
+        const float mn = fmaxf(m, wave_max(sc)), mu = mn == -INFINITY ? 0.f : mn;
+        const float p = page >= 0 ? exp2_hw(sc - mu) : 0.f, al = exp2_hw(m - mu);
         l = l * al + wave_sum(p);
         m = mn;
 #pragma unroll
         for (int r = 0; r < R; ++r) acc[r] *= al;
-        for (int i = 0; i < 64 && j0 + i < lim; ++i) {
+        for (int i = 0; i < 64 && j0 + i < k1; ++i) {
             const int pg = __shfl(page, i);
             const float pi = __shfl(p, i);
             if (pg < 0) continue;
-            const elem_t* vp = vb + pg * a.vc[0] + ((j0 + i) & ((1 << a.page_shift) - 1)) * a.vc[2];
+            const elem_t* vp = vb + pg * a.vc[0] + ((j0 + i) & mask) * a.vc[2];
 #pragma unroll
             for (int r = 0; r < R; ++r) acc[r] = fmaf(pi, from_elem<P>(vp[r * 64 + lane]), acc[r]);
         }
     }
-    bad = __any(bad);
-    elem_t* op = reinterpret_cast<elem_t*>(a.out) + t * a.os[0] + h * a.os[1];
+    *m_out = m; *l_out = l;
+}
+
+// where the partial results of a split launch lie: outputs [split][token * q_heads + head][D], behind them (maximum, sum) pairs
+template <int D> __device__ inline float* part_out(const PagedAttnArgs& a, int split, int64_t row) {
+    return a.part + ((int64_t)split * a.tokens * a.q_heads + row) * D;
+}
+template <int D> __device__ inline float* part_ml(const PagedAttnArgs& a, int split, int64_t row) {
+    const int64_t rows = (int64_t)a.tokens * a.q_heads;
+    return a.part + (int64_t)a.splits * rows * D + (split * rows + row) * 2;
+}
+
+template <typename P, int D>
+__device__ inline void store_row_alone(const PagedAttnArgs& a, int seq, int kvh, int64_t token, int head, int split, int k0, int k1) {
+    typedef typename P::elem_t elem_t;
+    const int lane = threadIdx.x & 63;
+    float m, l, acc[D / 64];
+    row_alone<P, D>(a, seq, kvh, reinterpret_cast<const elem_t*>(a.q) + token * a.qs[0] + head * a.qs[1], k0, k1, &m, &l, acc);
+    const int64_t row = token * a.q_heads + head;
 #pragma unroll
-    for (int r = 0; r < R; ++r) op[r * 64 + lane] = to_elem<P>(bad ? NAN : (l == 0.f ? 0.f : acc[r] / l));
+    for (int r = 0; r < D / 64; ++r) {
+        if (a.splits > 1) part_out<D>(a, split, row)[r * 64 + lane] = acc[r];
+        else (reinterpret_cast<elem_t*>(a.out) + token * a.os[0] + head * a.os[1])[r * 64 + lane] = to_elem<P>(l == 0.f ? 0.f : acc[r] / l);
+    }
+    if (a.splits > 1 && lane == 0) { float* ml = part_ml<D>(a, split, row); ml[0] = m; ml[1] = l; }
+}
+
+// keys of split `split`: equal shares of whole tiles
+__device__ inline void split_range(const PagedAttnArgs& a, int split, int end, int KT, int* k0, int* k1) {
+    if (a.splits == 1) { *k0 = 0; *k1 = end; return; }
+    const int tiles = (end + KT - 1) / KT, share = (tiles + a.splits - 1) / a.splits;
+    *k0 = min(split * share * KT, end);
+    *k1 = min(*k0 + share * KT, end);
+}
+
+template <typename P> __device__ inline void store4(typename P::elem_t* p, float a, float b, float c, float d);
+template <> __device__ inline void store4<PBF16>(uint16_t* p, float a, float b, float c, float d) {
+    typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+    const bf16x4 v = {(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)d};
+    *reinterpret_cast<bf16x4*>(p) = v;
+}
+template <> __device__ inline void store4<PF32>(float* p, float a, float b, float c, float d) {
+    const f32x4 v = {a, b, c, d};
+    *reinterpret_cast<f32x4*>(p) = v;
+}
+
+// =================================================================================================================================
+// Chunks: a workgroup owns 128 rows (32 per wave), the keys pass in tiles of KT through two LDS buffers.
+// =================================================================================================================================
+template <typename P, int D> struct TileCfg {
+    static constexpr int M = 128, NW = 4;
+    static constexpr int RB = D * (int)sizeof(typename P::elem_t);
+    static constexpr int KT = RB <= 256 ? 64 : 32;
+    static constexpr int TILE = KT * RB;                       // bytes of K or V of a tile
+    static constexpr int LDS = 4 * TILE;                       // [2 buffers][K, V]
+    static constexpr int DMA = 2 * TILE / NW / 1024;           // LDS-DMA instructions per wave and tile
+};
+
+template <typename P, int D>
+__global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a) {
+    typedef typename P::elem_t elem_t;
+    typedef TileCfg<P, D> C;
+    constexpr int KT = C::KT, RB = C::RB, EPL = P::EPL, NKS = D / (2 * EPL), NKB = KT / 32, NDB = D / 32;
+    __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
+    const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l31 = lane & 31, h = lane >> 5;
+
+    if (blockIdx.x == 0 && a.starts) check_starts(a.starts, a.n_seqs, a.tokens, a.status);
+    // consecutive workgroups go to consecutive XCDs: with the key head innermost, an XCD's L2 holds few heads' pages
+    const int kvh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, split = rest % a.splits;
+    Span sp;
+    int tile;
+    if (!find_tile(a, rest / a.splits, C::M, &sp, &tile)) return;
+    read_past(a, &sp);
+    const int rows = sp.n * a.group;
+    tile = (rows + C::M - 1) / C::M - 1 - tile;                // the rows that see most first
+    const int r0 = tile * C::M, r_end = min(r0 + C::M, rows);
+    const int row = r0 + w * 32 + l31;                         // this lane's query
+    const bool live = row < r_end;
+    const int tok = live ? row / a.group : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
+    const int64_t token = sp.first + tok;
+    int lim = live && !sp.bad ? sp.past + (a.causal ? tok + 1 : 0) : 0;       // keys 0 .. lim - 1 are seen
+    const int tile_end = sp.bad ? 0 : sp.past + (a.causal ? (r_end - 1) / a.group + 1 : 0);
+    int k0, k1;
+    split_range(a, split, tile_end, KT, &k0, &k1);
+    const int wr0 = r0 + w * 32, wr1 = min(wr0 + 32, r_end);                  // rows of this wave: [wr0, wr1)
+    const int w_end = wr0 < wr1 && !sp.bad ? (a.causal ? sp.past + (wr1 - 1) / a.group + 1 : sp.past) : 0;   // keys any of them sees
+    const int w_all = wr0 < wr1 && !sp.bad ? (a.causal ? sp.past + wr0 / a.group + 1 : sp.past) : 0;         // keys all of them see
+
+    Pages pg;
+    pg.row = a.table + sp.seq * a.table_stride; pg.n_pages = a.n_pages; pg.bad = false; pg.base = 0; pg.ids = 0;
+    const int64_t kp = a.kc[0] * (int)sizeof(elem_t), ks = a.kc[2] * (int)sizeof(elem_t);
+    const int64_t vp = a.vc[0] * (int)sizeof(elem_t), vs = a.vc[2] * (int)sizeof(elem_t);
+    const char* kbase = reinterpret_cast<const char*>(a.k) + kvh * a.kc[1] * (int)sizeof(elem_t);
+    const char* vbase = reinterpret_cast<const char*>(a.v) + kvh * a.vc[1] * (int)sizeof(elem_t);
+    auto fetch = [&](int key0, int buf) {
+        const int last = (k1 - 1) >> a.page_shift;
+        if (((min(key0 + KT, k1) - 1) >> a.page_shift) >= pg.base + 64 || key0 == k0) pg.load(key0 >> a.page_shift, last);
+        char* lds = smem + buf * 2 * C::TILE;
+        dma_rows<P, D, KT / C::NW>(kbase, kp, ks, pg, a.page_shift, key0, w * (KT / C::NW), k1, lds);
+        dma_rows<P, D, KT / C::NW>(vbase, vp, vs, pg, a.page_shift, key0, w * (KT / C::NW), k1, lds + C::TILE);
+    };
+
+    // B operand of S^T = K Q^T: 16-byte chunk 2 s + h of the lane's query row at step s (and of the lane's key row for A)
+    u32x4 qf[NKS];
+    {
+        const elem_t* qp = reinterpret_cast<const elem_t*>(a.q) + token * a.qs[0] + head * a.qs[1];
+#pragma unroll
+        for (int s = 0; s < NKS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qp + (2 * s + h) * EPL);
+    }
+    f32x16 o[NDB];
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    float m = -INFINITY, l = 0.f;       // maximum of the query's scores (log2 units), sum of the weights of this half's keys
+
+    if (k0 < k1) fetch(k0, 0);
+    int buf = 0;
+    for (int key0 = k0; key0 < k1; key0 += KT, buf ^= 1) {
+        wait_vm<0>();
+        wait_lds();
+        __builtin_amdgcn_s_barrier();        // the tile has landed, and every wave has left the other buffer
+        if (key0 + KT < k1) fetch(key0 + KT, buf ^ 1);
+        if (key0 >= w_end) continue;         // nothing here for this wave's rows (it keeps moving its share of the tiles)
+        const char* kt = smem + buf * 2 * C::TILE;
+        const char* vt = kt + C::TILE;
+
+        f32x16 s[NKB];
+#pragma unroll
+        for (int b = 0; b < NKB; ++b) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+            const int kr = b * 32 + l31;
+#pragma unroll
+            for (int t = 0; t < NKS; ++t) {
+                const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + kr * RB + (((2 * t + h) ^ (kr & 7)) << 4));
+                if constexpr (P::IS_BF16) {
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[t]), s[b], 0, 0, 0);
+                } else {
+                    const f32x4 kx = __builtin_bit_cast(f32x4, kf), qx = __builtin_bit_cast(f32x4, qf[t]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(kx[j], qx[j], s[b], 0, 0, 0);
+                }
+            }
+        }
+        const uint64_t alive = tile_mask(a, sp.seq, key0);
+        if (key0 + KT > w_all || alive != ~0ull) {             // some key of the tile is not for some query
+            const int left = lim - key0;
+            const uint64_t see = (left >= 64 ? ~0ull : (left <= 0 ? 0ull : (1ull << left) - 1)) & alive;
+            const uint32_t half[2] = {(uint32_t)(see >> (4 * h)), (uint32_t)(see >> 32 >> (4 * h))};
+#pragma unroll
+            for (int b = 0; b < NKB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    s[b][r] = (half[b] >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[b][r] : -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int b = 0; b < NKB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+        mx = swap_max32(mx) * a.scale_log2;
+        // weights are kept relative to a maximum that may lag behind by 2^8 (their type holds that range as well as any): the sums
+        // are rescaled only when a query's maximum has risen further
+        if (__any(mx > m + 8.f)) {
+            const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.f : exp2_hw(m - mn);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < NDB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= al;
+        }
+        const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int b = 0; b < NKB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[b][r] = exp2_hw(fmaf(s[b][r], a.scale_log2, -mu));
+                l += s[b][r];
+            }
+        if constexpr (P::IS_BF16) {
+#if defined(__HIP_DEVICE_COMPILE__)
+            // transposing read: 16 lanes take a block of 4 keys x 16 features, lane i ends with feature i of the 4 keys
+            const int i16 = lane & 15, vrow = 4 * h + (i16 >> 2), vcol = 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+#pragma unroll
+            for (int kk = 0; kk < KT / 16; ++kk) {
+                bf16x8 pf;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) pf[j] = (__bf16)s[kk >> 1][8 * (kk & 1) + j];
+#pragma unroll
+                for (int d = 0; d < NDB; ++d) {
+                    const int ra = 16 * kk + vrow, rb = ra + 8, ch = (d * 32 + vcol) >> 3, sub = (vcol & 7) * 2;
+                    const s16x4 va = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vt + ra * RB + ((ch ^ (ra & 7)) << 4) + sub));
+                    const s16x4 vb = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vt + rb * RB + ((ch ^ (rb & 7)) << 4) + sub));
+                    const s16x8 vf = __builtin_shufflevector(va, vb, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf), pf, o[d], 0, 0, 0);
+                }
+            }
+#endif
+        } else {
+#pragma unroll
+            for (int b = 0; b < NKB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int vr = b * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
+#pragma unroll
+                    for (int d = 0; d < NDB; ++d) {
+                        const int f = d * 32 + l31;
+                        const float vx = *reinterpret_cast<const float*>(vt + vr * RB + (((f >> 2) ^ (vr & 7)) << 4) + (f & 3) * 4);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vx, s[b][r], o[d], 0, 0, 0);
+                    }
+                }
+        }
+    }
+    wait_vm<0>();
+    if (pg.bad && threadIdx.x == 0) atomicOr(a.status, PAGED_BAD_PAGE);
+    const bool bad = pg.bad || sp.bad;
+    l += __shfl_xor(l, 32);
+    float inv = l == 0.f ? 0.f : 1.f / l;
+    if (bad) { l = NAN; inv = NAN; }
+    // a result that is not finite: of this query's own making, or a key that it does not see
+    bool odd = false;
+    if (!bad) {
+        float z = l * 0.f;
+#pragma unroll
+        for (int d = 0; d < NDB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z = fmaf(o[d][r], 0.f, z);
+        odd = live && !(z == 0.f);
+    }
+    const uint64_t odds = __ballot(odd);
+    if (live) {
+        const int64_t orow = token * a.q_heads + head;
+#pragma unroll
+        for (int d = 0; d < NDB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int f = d * 32 + 2 * r + 4 * h;
+                if (a.splits > 1) store4<PF32>(part_out<D>(a, split, orow) + f, o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
+                else store4<P>(reinterpret_cast<elem_t*>(a.out) + token * a.os[0] + head * a.os[1] + f, o[d][r] * inv, o[d][r + 1] * inv,
+                               o[d][r + 2] * inv, o[d][r + 3] * inv);
+            }
+        if (a.splits > 1 && h == 0) { float* ml = part_ml<D>(a, split, orow); ml[0] = m; ml[1] = l; }
+    }
+    uint32_t again = (uint32_t)odds | (uint32_t)(odds >> 32);
+    while (again) {
+        const int i = __builtin_ctz(again);
+        again &= again - 1;
+        const int rr = wr0 + i, tk = rr / a.group;
+        store_row_alone<P, D>(a, sp.seq, kvh, sp.first + tk, kvh * a.group + rr - tk * a.group, split, k0,
+                              min(k1, sp.past + (a.causal ? tk + 1 : 0)));
+    }
+}
+
+// =================================================================================================================================
+// Joins the partial results of a split launch: one wave per (token, query head).
+// =================================================================================================================================
+template <typename P, int D>
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
+    typedef typename P::elem_t elem_t;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= (int64_t)a.tokens * a.q_heads) return;
+    const int64_t token = row / a.q_heads;
+    const int head = (int)(row - token * a.q_heads);
+    if (a.starts) {          // rows of no sequence (padding, bad starts) have no partial results
+        int lo = 0, hi = a.n_seqs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.starts[mid] <= token) lo = mid; else hi = mid;
+        }
+        if (a.starts[lo] < 0 || a.starts[lo + 1] > a.tokens || token < a.starts[lo] || token >= a.starts[lo + 1]) return;
+    }
+    float m = -INFINITY;
+    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, part_ml<D>(a, s, row)[0]);
+    m = wave_max(m);
+    const float mu = m == -INFINITY ? 0.f : m;
+    float l = 0.f, acc[D / 64];
+#pragma unroll
+    for (int r = 0; r < D / 64; ++r) acc[r] = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float* ml = part_ml<D>(a, s, row);
+        const float ls = ml[1];
+        if (ls == 0.f) continue;
+        const float f = exp2_hw(ml[0] - mu);
+        l = fmaf(ls, f, l);
+        const float* p = part_out<D>(a, s, row);
+#pragma unroll
+        for (int r = 0; r < D / 64; ++r) acc[r] = fmaf(p[r * 64 + lane], f, acc[r]);
+    }
+    elem_t* op = reinterpret_cast<elem_t*>(a.out) + token * a.os[0] + head * a.os[1];
+#pragma unroll
+    for (int r = 0; r < D / 64; ++r) op[r * 64 + lane] = to_elem<P>(l == 0.f ? 0.f : acc[r] / l);
+}
+
+struct Plan { int tiles, splits; };
+
+// Workgroups are few where rows are few: the keys are then shared out over `splits` workgroups.  Two workgroups fit a CU; a share has
+// at least 256 keys (its partial result costs a row of f32 outputs twice).
+Plan make_plan(const PagedAttnArgs& a, int max_new, int M) {
+    Plan p;
+    const int64_t ub = (int64_t)a.tokens * a.group / M + a.n_seqs;
+    p.tiles = (int)ub;
+    int64_t est = ub;
+    if (!a.starts || max_new > 0) est = (int64_t)a.n_seqs * (((a.starts ? max_new : 1) * (int64_t)a.group + M - 1) / M);
+    if (est > ub) est = ub;
+    const int64_t groups = est * a.kv_heads, keys = (int64_t)a.max_pages << a.page_shift;
+    int64_t s = 512 / (groups > 0 ? groups : 1);
+    if (s > keys / 256) s = keys / 256;
+    if (s > 64) s = 64;
+    p.splits = s < 1 ? 1 : (int)s;
+    return p;
 }
 
 }  // namespace
 
-int64_t paged_attn_workspace(const PagedAttnArgs&, int, int, int) { return 0; }
+int64_t paged_attn_workspace(const PagedAttnArgs& a, int max_new, int head_dim, int) {
+    const Plan p = make_plan(a, max_new, 128);
+    return p.splits == 1 ? 0 : (int64_t)p.splits * a.tokens * a.q_heads * (head_dim + 2) * (int64_t)sizeof(float);
+}
+
+template <typename P, int D>
+static hipError_t launch(PagedAttnArgs a, int max_new, hipStream_t s) {
+    const Plan p = make_plan(a, max_new, TileCfg<P, D>::M);
+    a.splits = p.splits;
+    if ((int64_t)p.tiles * p.splits * a.kv_heads > 0x7fffffff || (int64_t)a.tokens * a.q_heads > 0x7fffffff) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((paged_attn_tile_kernel<P, D>), dim3((unsigned)((int64_t)p.tiles * p.splits * a.kv_heads)), dim3(256), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.splits == 1) return e;
+    const int64_t rows = (int64_t)a.tokens * a.q_heads;
+    hipLaunchKernelGGL((paged_attn_join_kernel<P, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
 
 hipError_t paged_attn_launch(const PagedAttnArgs& a, int max_new, int head_dim, int dtype, hipStream_t s) {
-    dim3 grid(a.tokens, a.q_heads), block(64);
-    if (dtype == PTTS_BF16) {
-        if (head_dim == 64) hipLaunchKernelGGL((paged_attn_simple_kernel<PBF16, 64>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((paged_attn_simple_kernel<PBF16, 128>), grid, block, 0, s, a);
-    } else {
-        if (head_dim == 64) hipLaunchKernelGGL((paged_attn_simple_kernel<PF32, 64>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((paged_attn_simple_kernel<PF32, 128>), grid, block, 0, s, a);
-    }
-    return hipGetLastError();
+    if (dtype == PTTS_BF16) return head_dim == 64 ? launch<PBF16, 64>(a, max_new, s) : launch<PBF16, 128>(a, max_new, s);
+    return head_dim == 64 ? launch<PF32, 64>(a, max_new, s) : launch<PF32, 128>(a, max_new, s);
 }
