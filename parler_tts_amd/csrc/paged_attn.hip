@@ -17,6 +17,7 @@
 #include "ptts_common.h"
 #include "gemm.h"
 #include "paged.h"
+#include <type_traits>
 
 namespace {
 
@@ -51,12 +52,63 @@ __device__ inline float swap_max32(float x) {      // maximum over lanes l and l
     return x;
 #endif
 }
+__device__ inline float swap_max16(float x) {      // maximum over lanes l and l ^ 16
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+    const unsigned r0 = r[0], r1 = r[1];
+    return fmaxf(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+#else
+    return x;
+#endif
+}
 __device__ inline float exp2_hw(float x) {
 #if defined(__HIP_DEVICE_COMPILE__)
     return __builtin_amdgcn_exp2f(x);
 #else
     return x;
 #endif
+}
+// Transposing reads of V: 16 lanes take a block of 4 keys x 16 features (each lane 4 features of one key), lane i ends with feature i of
+// the 4 keys.  A and B are the two blocks of a matrix step.  Written out, because hipcc drains the LDS-DMA in flight in front of the
+// builtin; the wait stands in the same statement as the reads.
+template <int OFF_A, int OFF_B> __device__ inline void read_v4(unsigned a0, unsigned a1, unsigned a2, unsigned a3, s16x8 (&v)[4]) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    s16x4 r[8];
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+                 : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(OFF_A), "n"(OFF_B) : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __builtin_shufflevector(r[2 * i], r[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+#endif
+}
+// the same for two feature blocks a0, a1 of two steps
+template <int A, int B, int C, int D> __device__ inline void read_v2(unsigned a0, unsigned a1, s16x8 (&v)[4]) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    s16x4 r[8];
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%10\n\tds_read_b64_tr_b16 %1, %8 offset:%11\n\t"
+                 "ds_read_b64_tr_b16 %2, %9 offset:%10\n\tds_read_b64_tr_b16 %3, %9 offset:%11\n\t"
+                 "ds_read_b64_tr_b16 %4, %8 offset:%12\n\tds_read_b64_tr_b16 %5, %8 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %6, %9 offset:%12\n\tds_read_b64_tr_b16 %7, %9 offset:%13\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+                 : "v"(a0), "v"(a1), "n"(A), "n"(B), "n"(C), "n"(D) : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __builtin_shufflevector(r[2 * i], r[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+#endif
+}
+__device__ inline unsigned lds_address(const void* p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+#else
+    return 0;
+#endif
+}
+template <int I, int N, typename F> __device__ inline void unrolled(F&& f) {      // f(integral constant I), f(I + 1), ...
+    if constexpr (I < N) { f(std::integral_constant<int, I>()); unrolled<I + 1, N>(f); }
 }
 __device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
@@ -243,14 +295,15 @@ template <> __device__ inline void store4<PF32>(float* p, float a, float b, floa
 }
 
 // =================================================================================================================================
-// Chunks: a workgroup owns 128 rows (32 per wave), the keys pass in tiles of KT through two LDS buffers.
+// Chunks: a workgroup owns 128 rows (32 per wave), the keys pass in tiles of KT through a ring of LDS buffers.
 // =================================================================================================================================
 template <typename P, int D> struct TileCfg {
     static constexpr int M = 128, NW = 4;
     static constexpr int RB = D * (int)sizeof(typename P::elem_t);
     static constexpr int KT = RB <= 256 ? 64 : 32;
     static constexpr int TILE = KT * RB;                       // bytes of K or V of a tile
-    static constexpr int LDS = 4 * TILE;                       // [2 buffers][K, V]
+    static constexpr int NBUF = 65536 / (2 * TILE);            // ring of tiles: 64 KiB, two workgroups on a CU
+    static constexpr int LDS = NBUF * 2 * TILE;                // [buffer][K, V]
     static constexpr int DMA = 2 * TILE / NW / 1024;           // LDS-DMA instructions per wave and tile
 };
 
@@ -292,7 +345,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     const char* vbase = reinterpret_cast<const char*>(a.v) + kvh * a.vc[1] * (int)sizeof(elem_t);
     auto fetch = [&](int key0, int buf) {
         const int last = (k1 - 1) >> a.page_shift;
-        if (((min(key0 + KT, k1) - 1) >> a.page_shift) >= pg.base + 64 || key0 == k0) pg.load(key0 >> a.page_shift, last);
+        if (((min(key0 + KT, k1) - 1) >> a.page_shift) >= pg.base + 64) pg.load(key0 >> a.page_shift, last);
         char* lds = smem + buf * 2 * C::TILE;
         dma_rows<P, D, KT / C::NW>(kbase, kp, ks, pg, a.page_shift, key0, w * (KT / C::NW), k1, lds);
         dma_rows<P, D, KT / C::NW>(vbase, vp, vs, pg, a.page_shift, key0, w * (KT / C::NW), k1, lds + C::TILE);
@@ -312,13 +365,22 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
         for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
     float m = -INFINITY, l = 0.f;       // maximum of the query's scores (log2 units), sum of the weights of this half's keys
 
-    if (k0 < k1) fetch(k0, 0);
+    // the query rows arrive before the first tile is sent for: a wait for them inside the loop would be one for the tiles in flight too
+    if (k0 < k1) pg.load(k0 >> a.page_shift, (k1 - 1) >> a.page_shift);
+#pragma unroll
+    for (int t = 0; t < NKS; ++t) asm volatile("" : "+v"(qf[t]));
+#pragma unroll
+    for (int i = 0; i < C::NBUF - 1; ++i)
+        if (k0 + i * KT < k1) fetch(k0 + i * KT, i);
     int buf = 0;
-    for (int key0 = k0; key0 < k1; key0 += KT, buf ^= 1) {
-        wait_vm<0>();
+    for (int key0 = k0; key0 < k1; key0 += KT, buf = buf + 1 == C::NBUF ? 0 : buf + 1) {
+        const int ahead = min(C::NBUF - 2, (k1 - key0 - 1) / KT);           // younger tiles that stay in flight
+        if (C::NBUF > 3 && ahead >= 2) wait_vm<2 * C::DMA>();
+        else if (C::NBUF > 2 && ahead >= 1) wait_vm<C::DMA>();
+        else wait_vm<0>();
         wait_lds();
-        __builtin_amdgcn_s_barrier();        // the tile has landed, and every wave has left the other buffer
-        if (key0 + KT < k1) fetch(key0 + KT, buf ^ 1);
+        __builtin_amdgcn_s_barrier();        // the tile has landed, and every wave has left the buffer of the tile before it
+        if (key0 + (C::NBUF - 1) * KT < k1) fetch(key0 + (C::NBUF - 1) * KT, buf == 0 ? C::NBUF - 1 : buf - 1);
         if (key0 >= w_end) continue;         // nothing here for this wave's rows (it keeps moving its share of the tiles)
         const char* kt = smem + buf * 2 * C::TILE;
         const char* vt = kt + C::TILE;
@@ -379,23 +441,26 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
             }
         if constexpr (P::IS_BF16) {
 #if defined(__HIP_DEVICE_COMPILE__)
-            // transposing read: 16 lanes take a block of 4 keys x 16 features, lane i ends with feature i of the 4 keys
-            const int i16 = lane & 15, vrow = 4 * h + (i16 >> 2), vcol = 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
-            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            // key 16 kk + 4 h + 0 .. 3 in slots 0 .. 3, 8 further on in slots 4 .. 7; the chunk swizzle of a row depends on 4 h + i16 / 4 only
+            // and moves feature block d by 64 bytes for odd d, two blocks by 128
+            const int i16 = lane & 15, vrow = 4 * h + (i16 >> 2), c0 = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
+            const unsigned va = lds_address(vt) + vrow * RB + ((c0 ^ (vrow & 7)) << 4) + (i16 & 1) * 8, vb = va ^ 64;
+            unrolled<0, KT / 16>([&](auto KK) {
+                constexpr int kk = decltype(KK)::value;
+                if constexpr (NDB == 2 && (kk & 1)) return;           // done with the step in front
+                s16x8 vf[4];
+                if constexpr (NDB == 2) read_v2<16 * kk * RB, (16 * kk + 8) * RB, (16 * kk + 16) * RB, (16 * kk + 24) * RB>(va, vb, vf);
+                else read_v4<16 * kk * RB, (16 * kk + 8) * RB>(va, vb, va + 128, vb + 128, vf);
 #pragma unroll
-            for (int kk = 0; kk < KT / 16; ++kk) {
-                bf16x8 pf;
+                for (int u = 0; u < 4 / NDB; ++u) {
+                    bf16x8 pf;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) pf[j] = (__bf16)s[kk >> 1][8 * (kk & 1) + j];
+                    for (int j = 0; j < 8; ++j) pf[j] = (__bf16)s[(kk + u) >> 1][8 * ((kk + u) & 1) + j];
 #pragma unroll
-                for (int d = 0; d < NDB; ++d) {
-                    const int ra = 16 * kk + vrow, rb = ra + 8, ch = (d * 32 + vcol) >> 3, sub = (vcol & 7) * 2;
-                    const s16x4 va = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vt + ra * RB + ((ch ^ (ra & 7)) << 4) + sub));
-                    const s16x4 vb = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vt + rb * RB + ((ch ^ (rb & 7)) << 4) + sub));
-                    const s16x8 vf = __builtin_shufflevector(va, vb, 0, 1, 2, 3, 4, 5, 6, 7);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf), pf, o[d], 0, 0, 0);
+                    for (int d = 0; d < NDB; ++d)
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf[u * NDB + d]), pf, o[d], 0, 0, 0);
                 }
-            }
+            });
 #endif
         } else {
 #pragma unroll
@@ -453,13 +518,226 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
 }
 
 // =================================================================================================================================
-// Joins the partial results of a split launch: one wave per (token, query head).
+// Few rows (at most 16 per sequence and key head: single tokens, their groups, short drafts): bound by the stream of the cache.  A wave
+// owns every NW-th tile of 32 keys and two LDS buffers of its own, so that nothing in the loop waits for another wave; the waves'
+// states are joined once at the end.
 // =================================================================================================================================
+template <typename P, int D> struct StepCfg {
+    static constexpr int M = 16, KT = 32;
+    static constexpr int RB = D * (int)sizeof(typename P::elem_t);
+    static constexpr int TILE = KT * RB, STAGE = 2 * TILE;
+    static constexpr int NW = 65536 / (2 * STAGE);             // 4, 2, 2, 1 waves: 64 KiB of LDS, two workgroups on a CU
+    static constexpr int DMA = STAGE / 1024;
+    static_assert(NW * 16 * (D + 2) * 4 <= NW * 2 * STAGE, "the waves' states fit where their tiles were");
+};
+
 template <typename P, int D>
+__global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kernel(PagedAttnArgs a) {
+    typedef typename P::elem_t elem_t;
+    typedef StepCfg<P, D> C;
+    constexpr int KT = C::KT, RB = C::RB, EPL = P::EPL, NKS = D / (4 * EPL), NDB = D / 16, NW = C::NW;
+    __shared__ __attribute__((aligned(1024))) char smem[NW * 2 * C::STAGE];
+    const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
+
+    if (blockIdx.x == 0 && a.starts) check_starts(a.starts, a.n_seqs, a.tokens, a.status);
+    const int kvh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, split = rest % a.splits;
+    Span sp;
+    int tile;
+    if (!find_tile(a, rest / a.splits, C::M, &sp, &tile)) return;
+    read_past(a, &sp);
+    const int rows = sp.n * a.group, r0 = tile * C::M, r_end = min(r0 + C::M, rows);
+    const int row = r0 + l15;
+    const bool live = row < r_end;
+    const int tok = live ? row / a.group : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
+    const int64_t token = sp.first + tok;
+    const int lim = live && !sp.bad ? sp.past + (a.causal ? tok + 1 : 0) : 0;
+    const int tile_end = sp.bad ? 0 : sp.past + (a.causal ? (r_end - 1) / a.group + 1 : 0);
+    const int all = r_end - r0 == C::M && !sp.bad ? sp.past + (a.causal ? r0 / a.group + 1 : 0) : 0;      // keys every column sees
+    int k0, k1;
+    split_range(a, split, tile_end, KT, &k0, &k1);
+
+    Pages pg;
+    pg.row = a.table + sp.seq * a.table_stride; pg.n_pages = a.n_pages; pg.bad = false; pg.base = 0; pg.ids = 0;
+    const int64_t kp = a.kc[0] * (int)sizeof(elem_t), ks = a.kc[2] * (int)sizeof(elem_t);
+    const int64_t vp = a.vc[0] * (int)sizeof(elem_t), vs = a.vc[2] * (int)sizeof(elem_t);
+    const char* kbase = reinterpret_cast<const char*>(a.k) + kvh * a.kc[1] * (int)sizeof(elem_t);
+    const char* vbase = reinterpret_cast<const char*>(a.v) + kvh * a.vc[1] * (int)sizeof(elem_t);
+    char* ring = smem + w * 2 * C::STAGE;
+    const int first = k0 + w * KT;
+    auto fetch = [&](int key0, int buf) {
+        if (((min(key0 + KT, k1) - 1) >> a.page_shift) >= pg.base + 64) pg.load(key0 >> a.page_shift, (k1 - 1) >> a.page_shift);
+        char* lds = ring + buf * C::STAGE;
+        dma_rows<P, D, KT>(kbase, kp, ks, pg, a.page_shift, key0, 0, k1, lds);
+        dma_rows<P, D, KT>(vbase, vp, vs, pg, a.page_shift, key0, 0, k1, lds + C::TILE);
+    };
+
+    u32x4 qf[NKS];
+    {
+        const elem_t* qp = reinterpret_cast<const elem_t*>(a.q) + token * a.qs[0] + head * a.qs[1];
+#pragma unroll
+        for (int t = 0; t < NKS; ++t) qf[t] = *reinterpret_cast<const u32x4*>(qp + (4 * t + g) * EPL);
+    }
+    f32x4 o[NDB];
+#pragma unroll
+    for (int d = 0; d < NDB; ++d) o[d] = {0, 0, 0, 0};
+    float m = -INFINITY, l = 0.f;
+    if (first < k1) pg.load(first >> a.page_shift, (k1 - 1) >> a.page_shift);
+#pragma unroll
+    for (int t = 0; t < NKS; ++t) asm volatile("" : "+v"(qf[t]));
+
+    if (first < k1) fetch(first, 0);
+    int buf = 0;
+    for (int key0 = first; key0 < k1; key0 += NW * KT, buf ^= 1) {
+        wait_lds();                          // the other buffer's reads are over
+        if (key0 + NW * KT < k1) { fetch(key0 + NW * KT, buf ^ 1); wait_vm<C::DMA>(); }
+        else wait_vm<0>();
+        const char* kt = ring + buf * C::STAGE;
+        const char* vt = kt + C::TILE;
+        f32x4 s[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            s[b] = {0, 0, 0, 0};
+            const int kr = b * 16 + l15;
+#pragma unroll
+            for (int t = 0; t < NKS; ++t) {
+                const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + kr * RB + (((4 * t + g) ^ (kr & 7)) << 4));
+                if constexpr (P::IS_BF16) {
+                    s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[t]), s[b], 0, 0, 0);
+                } else {
+                    const f32x4 kx = __builtin_bit_cast(f32x4, kf), qx = __builtin_bit_cast(f32x4, qf[t]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[j], qx[j], s[b], 0, 0, 0);
+                }
+            }
+        }
+        const uint64_t alive = tile_mask(a, sp.seq, key0);
+        if (key0 + KT > all || (uint32_t)alive != ~0u) {
+            const int left = lim - key0;
+            const uint32_t see = (left >= 32 ? ~0u : (left <= 0 ? 0u : (1u << left) - 1)) & (uint32_t)alive;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[b][r] = (see >> (16 * b + 4 * g + r)) & 1 ? s[b][r] : -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        mx = swap_max32(swap_max16(mx)) * a.scale_log2;
+        if (__any(mx > m + 8.f)) {           // as in the tile kernel
+            const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.f : exp2_hw(m - mn);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < NDB; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[d][r] *= al;
+        }
+        const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[b][r] = exp2_hw(fmaf(s[b][r], a.scale_log2, -mu));
+                l += s[b][r];
+            }
+        if constexpr (P::IS_BF16) {
+#if defined(__HIP_DEVICE_COMPILE__)
+            // slots 0 .. 3 of group g: keys 4 g .. of the lower 16, slots 4 .. 7: of the upper 16
+            bf16x8 pf;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) pf[j] = (__bf16)s[j >> 2][j & 3];
+            const int vrow = 4 * g + (l15 >> 2);
+            const unsigned va = lds_address(vt) + vrow * RB + ((((l15 >> 1) & 1) ^ (vrow & 7)) << 4) + (l15 & 1) * 8;
+            unrolled<0, NDB / 4>([&](auto Q) {
+                constexpr int q4 = decltype(Q)::value;               // feature blocks 4 q4 .. (32 bytes each, swizzled within 128)
+                s16x8 vf[4];
+                read_v4<q4 * 128, q4 * 128 + 16 * RB>(va, va ^ 32, va ^ 64, va ^ 96, vf);
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                    o[4 * q4 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf[d]), pf, o[4 * q4 + d], 0, 0, 0);
+            });
+#endif
+        } else {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int vr = 16 * b + 4 * g + r;
+#pragma unroll
+                    for (int d = 0; d < NDB; ++d) {
+                        const int f = d * 16 + l15;
+                        const float vx = *reinterpret_cast<const float*>(vt + vr * RB + (((f >> 2) ^ (vr & 7)) << 4) + (f & 3) * 4);
+                        o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx, s[b][r], o[d], 0, 0, 0);
+                    }
+                }
+        }
+    }
+    wait_vm<0>();
+    if (pg.bad && lane == 0) atomicOr(a.status, PAGED_BAD_PAGE);
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (pg.bad || sp.bad) l = NAN;
+
+    // join the waves: outputs [NW][16][D] (16-byte pieces XOR-swizzled by the row) and maxima, sums [NW][16] in the place of the tiles
+    __syncthreads();
+    float* sm = reinterpret_cast<float*>(smem) + NW * 16 * D;
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+        *reinterpret_cast<f32x4*>(smem + ((w * 16 + l15) * D + (((d * 4 + g) ^ (l15 & 7)) << 2)) * 4) = o[d];
+    if (g == 0) { sm[w * 16 + l15] = m; sm[(NW + w) * 16 + l15] = l; }
+    __syncthreads();
+    constexpr int PPR = D / 4;               // pieces per row
+    for (int i = threadIdx.x; i < 16 * PPR; i += NW * 64) {
+        const int q = i / PPR, piece = i % PPR, rr = r0 + q;
+        const bool on = rr < r_end;
+        float top = sm[q], f[NW], sum = 0.f;
+#pragma unroll
+        for (int v = 1; v < NW; ++v) top = fmaxf(top, sm[v * 16 + q]);
+        const float mu = top == -INFINITY ? 0.f : top;
+        f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int v = 0; v < NW; ++v) {
+            f[v] = exp2_hw(sm[v * 16 + q] - mu);
+            sum = fmaf(sm[(NW + v) * 16 + q], f[v], sum);
+            const f32x4 x = *reinterpret_cast<const f32x4*>(smem + ((v * 16 + q) * D + ((piece ^ (q & 7)) << 2)) * 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] = fmaf(x[j], f[v], acc[j]);
+        }
+        const bool ruined = sum != sum && (pg.bad || sp.bad);
+        const float z = fmaf(acc[0], 0.f, fmaf(acc[1], 0.f, fmaf(acc[2], 0.f, fmaf(acc[3], 0.f, sum * 0.f))));
+        const int tk = on ? rr / a.group : 0, hd = kvh * a.group + (on ? rr - tk * a.group : 0);
+        const int64_t t64 = sp.first + tk;
+        if (on) {
+            if (a.splits > 1) {
+                const int64_t orow = t64 * a.q_heads + hd;
+                *reinterpret_cast<f32x4*>(part_out<D>(a, split, orow) + piece * 4) = acc;
+                if (piece == 0) { float* ml = part_ml<D>(a, split, orow); ml[0] = top; ml[1] = sum; }
+            } else {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                store4<P>(reinterpret_cast<elem_t*>(a.out) + t64 * a.os[0] + hd * a.os[1] + piece * 4, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+            }
+        }
+        // rows of this wave's pieces whose result is not finite (64 lanes hold 64 / PPR rows), again and alone
+        uint64_t odds = __ballot(on && !ruined && !(z == 0.f));
+        while (odds) {
+            const int src = __builtin_ctzll(odds), rw = (i - lane + src) / PPR;
+            const uint64_t same = PPR == 64 ? ~0ull : (((1ull << PPR) - 1) << (src / PPR * PPR));
+            odds &= ~same;
+            const int ar = r0 + uniform(rw), at = ar / a.group;
+            store_row_alone<P, D>(a, sp.seq, kvh, sp.first + at, kvh * a.group + ar - at * a.group, split, k0,
+                                  min(k1, sp.past + (a.causal ? at + 1 : 0)));
+        }
+    }
+}
+
+// =================================================================================================================================
+// Joins the partial results of a split launch: W waves per (token, query head).  The (maximum, sum) pairs of all splits (at most 64) sit
+// one per lane; 16-byte pieces of the partial outputs are then read by 64 / (D / 4) splits at a time and wave.
+// =================================================================================================================================
+template <typename P, int D, int W>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
     typedef typename P::elem_t elem_t;
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    constexpr int LPR = D / 4, SPW = 64 / LPR;          // lanes per row, splits per wave
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, piece = lane % LPR, sub = lane / LPR;
+    const int64_t row = (int64_t)blockIdx.x * (4 / W) + (W == 1 ? w : 0);
     if (row >= (int64_t)a.tokens * a.q_heads) return;
     const int64_t token = row / a.q_heads;
     const int head = (int)(row - token * a.q_heads);
@@ -471,38 +749,54 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
         }
         if (a.starts[lo] < 0 || a.starts[lo + 1] > a.tokens || token < a.starts[lo] || token >= a.starts[lo + 1]) return;
     }
-    float m = -INFINITY;
-    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, part_ml<D>(a, s, row)[0]);
-    m = wave_max(m);
-    const float mu = m == -INFINITY ? 0.f : m;
-    float l = 0.f, acc[D / 64];
+    float m = -INFINITY, l = 0.f;
+    if (lane < a.splits) { const float2 ml = *reinterpret_cast<const float2*>(part_ml<D>(a, lane, row)); m = ml.x; l = ml.y; }
+    const float top = wave_max(m), f = l == 0.f ? 0.f : exp2_hw(m - (top == -INFINITY ? 0.f : top));
+    const float sum = wave_sum(l * f);
+    f32x4 acc = {0, 0, 0, 0};
+    for (int s0 = W == 1 ? 0 : w * SPW; s0 < a.splits; s0 += W * SPW) {
+        const int s = s0 + sub;
+        const float fs = __shfl(f, s & 63);
+        if (s < a.splits && fs != 0.f) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(part_out<D>(a, s, row) + piece * 4);
 #pragma unroll
-    for (int r = 0; r < D / 64; ++r) acc[r] = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float* ml = part_ml<D>(a, s, row);
-        const float ls = ml[1];
-        if (ls == 0.f) continue;
-        const float f = exp2_hw(ml[0] - mu);
-        l = fmaf(ls, f, l);
-        const float* p = part_out<D>(a, s, row);
-#pragma unroll
-        for (int r = 0; r < D / 64; ++r) acc[r] = fmaf(p[r * 64 + lane], f, acc[r]);
+            for (int i = 0; i < 4; ++i) acc[i] = fmaf(x[i], fs, acc[i]);
+        }
     }
-    elem_t* op = reinterpret_cast<elem_t*>(a.out) + token * a.os[0] + head * a.os[1];
 #pragma unroll
-    for (int r = 0; r < D / 64; ++r) op[r * 64 + lane] = to_elem<P>(l == 0.f ? 0.f : acc[r] / l);
+    for (int i = 0; i < 4; ++i) {
+        if (SPW >= 4) acc[i] += __shfl_xor(acc[i], 16);
+        acc[i] += __shfl_xor(acc[i], 32);
+    }
+    if constexpr (W > 1) {
+        __shared__ f32x4 other[W][LPR];
+        if (sub == 0) other[w][piece] = acc;
+        __syncthreads();
+        if (w != 0) return;
+#pragma unroll
+        for (int i = 1; i < W; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] += other[i][piece][j];
+    }
+    if (sub == 0) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        store4<P>(reinterpret_cast<elem_t*>(a.out) + token * a.os[0] + head * a.os[1] + piece * 4, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    }
 }
 
-struct Plan { int tiles, splits; };
+struct Plan { bool step; int tiles, splits; };
 
+// max_new tokens a sequence at most (0: not known) make at most max_new * group rows per key head: up to 16 take the step kernel.
 // Workgroups are few where rows are few: the keys are then shared out over `splits` workgroups.  Two workgroups fit a CU; a share has
 // at least 256 keys (its partial result costs a row of f32 outputs twice).
-Plan make_plan(const PagedAttnArgs& a, int max_new, int M) {
+Plan make_plan(const PagedAttnArgs& a, int max_new) {
     Plan p;
+    const int64_t most = (a.starts ? max_new : 1) * (int64_t)a.group;       // 0: not known
+    p.step = most > 0 && most <= 16;
+    const int M = p.step ? 16 : 128;
     const int64_t ub = (int64_t)a.tokens * a.group / M + a.n_seqs;
     p.tiles = (int)ub;
-    int64_t est = ub;
-    if (!a.starts || max_new > 0) est = (int64_t)a.n_seqs * (((a.starts ? max_new : 1) * (int64_t)a.group + M - 1) / M);
+    int64_t est = most > 0 ? (int64_t)a.n_seqs * ((most + M - 1) / M) : ub;
     if (est > ub) est = ub;
     const int64_t groups = est * a.kv_heads, keys = (int64_t)a.max_pages << a.page_shift;
     int64_t s = 512 / (groups > 0 ? groups : 1);
@@ -512,24 +806,26 @@ Plan make_plan(const PagedAttnArgs& a, int max_new, int M) {
     return p;
 }
 
+template <typename P, int D>
+hipError_t launch(PagedAttnArgs a, int max_new, hipStream_t s) {
+    const Plan p = make_plan(a, max_new);
+    a.splits = p.splits;
+    const int64_t rows = (int64_t)a.tokens * a.q_heads, groups = (int64_t)p.tiles * p.splits * a.kv_heads;
+    if (groups > 0x7fffffff || rows > 0x7fffffff) return hipErrorInvalidValue;
+    if (p.step) hipLaunchKernelGGL((paged_attn_step_kernel<P, D>), dim3((unsigned)groups), dim3(StepCfg<P, D>::NW * 64), 0, s, a);
+    else hipLaunchKernelGGL((paged_attn_tile_kernel<P, D>), dim3((unsigned)groups), dim3(256), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.splits == 1) return e;
+    if (p.splits > 8) hipLaunchKernelGGL((paged_attn_join_kernel<P, D, 4>), dim3((unsigned)rows), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((paged_attn_join_kernel<P, D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
 }  // namespace
 
 int64_t paged_attn_workspace(const PagedAttnArgs& a, int max_new, int head_dim, int) {
-    const Plan p = make_plan(a, max_new, 128);
+    const Plan p = make_plan(a, max_new);
     return p.splits == 1 ? 0 : (int64_t)p.splits * a.tokens * a.q_heads * (head_dim + 2) * (int64_t)sizeof(float);
-}
-
-template <typename P, int D>
-static hipError_t launch(PagedAttnArgs a, int max_new, hipStream_t s) {
-    const Plan p = make_plan(a, max_new, TileCfg<P, D>::M);
-    a.splits = p.splits;
-    if ((int64_t)p.tiles * p.splits * a.kv_heads > 0x7fffffff || (int64_t)a.tokens * a.q_heads > 0x7fffffff) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((paged_attn_tile_kernel<P, D>), dim3((unsigned)((int64_t)p.tiles * p.splits * a.kv_heads)), dim3(256), 0, s, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.splits == 1) return e;
-    const int64_t rows = (int64_t)a.tokens * a.q_heads;
-    hipLaunchKernelGGL((paged_attn_join_kernel<P, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
-    return hipGetLastError();
 }
 
 hipError_t paged_attn_launch(const PagedAttnArgs& a, int max_new, int head_dim, int dtype, hipStream_t s) {
