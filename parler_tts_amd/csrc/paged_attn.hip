@@ -118,41 +118,49 @@ struct Span {          // one sequence's new tokens
     bool bad;          // its length leads behind its row of the page table: every row becomes NaN
 };
 
-// The sequence of tile t of a launch whose tiles hold M rows: sequence s owns the tiles floor(starts[s] group / M) + s and on (at
-// least as many as its rows need, whatever lies in front of it), so no prefix sum over the batch is needed.  64-ary search, one wave.
+// The sequence and its tile that tile t of a launch is, where tiles hold M rows: a prefix sum over the sequences' tiles, 64 sequences at
+// a time, by every wave for itself (lengths and cache lengths come in one round trip).  Tiles of no sequence are the launch's last ones:
+// with holes between the sequences (a numbering that needs no sum) the dispatcher put all work of equal chunks on half of the CUs.
 __device__ inline bool find_tile(const PagedAttnArgs& a, int t, int M, Span* sp, int* tile) {
-    const int lane = threadIdx.x & 63;
-    int lo = 0, len = a.n_seqs;
-    for (;;) {
-        const int step = (len + 63) >> 6, i = lo + lane * step;
-        bool le = false;
-        if (i < lo + len) le = (int64_t)(a.starts ? a.starts[i] : i) * a.group / M + i <= t;
-        const int c = __popcll(__ballot(le));
-        if (c == 0) return false;
-        const int end = lo + len;
-        lo += (c - 1) * step;
-        len = min(step, end - lo);
-        if (len <= 1) break;
+    if (!a.starts) {
+        const int per = (a.group + M - 1) / M, s = t / per;
+        sp->seq = sp->first = s;
+        sp->n = 1;
+        sp->past = uniform(a.past[s]);
+        *tile = t - s * per;
+    } else {
+        const int lane = threadIdx.x & 63;
+        int rest = t, i0 = 0, sel, first = 0, n = 0, past = 0, sum;
+        for (;; i0 += 64) {
+            if (i0 >= a.n_seqs) return false;
+            const int i = min(i0 + lane, a.n_seqs - 1);
+            first = a.starts[i];
+            const int end = a.starts[i + 1];
+            past = a.past[i];
+            n = i0 + lane < a.n_seqs && first >= 0 && end <= a.tokens ? max(end - first, 0) : 0;       // starts that are wrong own no rows
+            const int own = (n * a.group + M - 1) / M;
+            sum = own;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) { const int x = __shfl_up(sum, d); sum += lane >= d ? x : 0; }
+            sel = __popcll(__ballot(sum <= rest));
+            if (sel < 64) { sum -= own; break; }
+            rest -= __builtin_amdgcn_readlane(sum, 63);
+        }
+        sel = uniform(sel);
+        sp->seq = i0 + sel;
+        sp->first = __builtin_amdgcn_readlane(first, sel);
+        sp->n = __builtin_amdgcn_readlane(n, sel);
+        sp->past = __builtin_amdgcn_readlane(past, sel);
+        *tile = rest - __builtin_amdgcn_readlane(sum, sel);
+        if (sp->n == 0) return false;
     }
-    lo = uniform(lo);
-    sp->seq = lo;
-    sp->first = a.starts ? uniform(a.starts[lo]) : lo;
-    const int end = a.starts ? uniform(a.starts[lo + 1]) : lo + 1;
-    sp->n = end - sp->first;
-    if (sp->first < 0 || end > a.tokens || sp->n <= 0) return false;
-    *tile = t - (int)((int64_t)sp->first * a.group / M + lo);
-    if ((int64_t)*tile * M >= (int64_t)sp->n * a.group) return false;
-    return true;
-}
-
-__device__ inline void read_past(const PagedAttnArgs& a, Span* sp) {
-    sp->past = uniform(a.past[sp->seq]);
     const int64_t reach = (int64_t)a.max_pages << a.page_shift;
     sp->bad = sp->past < 0 || (int64_t)sp->past + (a.causal ? sp->n : 0) > reach;
     if (sp->bad) {
         if (threadIdx.x == 0) atomicOr(a.status, PAGED_BAD_LENGTH);
         sp->past = 0;
     }
+    return true;
 }
 
 // ---- page ids of the keys ahead, one per lane ---------------------------------------------------------------------------------
@@ -321,7 +329,6 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     Span sp;
     int tile;
     if (!find_tile(a, rest / a.splits, C::M, &sp, &tile)) return;
-    read_past(a, &sp);
     const int rows = sp.n * a.group;
     tile = (rows + C::M - 1) / C::M - 1 - tile;                // the rows that see most first
     const int r0 = tile * C::M, r_end = min(r0 + C::M, rows);
@@ -544,7 +551,6 @@ __global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kern
     Span sp;
     int tile;
     if (!find_tile(a, rest / a.splits, C::M, &sp, &tile)) return;
-    read_past(a, &sp);
     const int rows = sp.n * a.group, r0 = tile * C::M, r_end = min(r0 + C::M, rows);
     const int row = r0 + l15;
     const bool live = row < r_end;
@@ -794,7 +800,7 @@ Plan make_plan(const PagedAttnArgs& a, int max_new) {
     const int64_t most = (a.starts ? max_new : 1) * (int64_t)a.group;       // 0: not known
     p.step = most > 0 && most <= 16;
     const int M = p.step ? 16 : 128;
-    const int64_t ub = (int64_t)a.tokens * a.group / M + a.n_seqs;
+    const int64_t ub = a.starts ? (int64_t)a.tokens * a.group / M + a.n_seqs : (int64_t)a.n_seqs * ((a.group + M - 1) / M);
     p.tiles = (int)ub;
     int64_t est = most > 0 ? (int64_t)a.n_seqs * ((most + M - 1) / M) : ub;
     if (est > ub) est = ub;
