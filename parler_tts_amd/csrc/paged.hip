@@ -283,6 +283,8 @@ int check_kv(const ptts_paged_kv* c) {
     if (overlaps_itself(c->k_strides, n, 3, c->head_dim) || overlaps_itself(c->v_strides, n, 3, c->head_dim))
         REFUSE(PTTS_E_INVALID, "rows of the cache share elements");
     const int esz = c->dtype == PTTS_DTYPE_BF16 ? 2 : 4;
+    if (c->k_strides[2] * esz >= ((int64_t)1 << 27) || c->v_strides[2] * esz >= ((int64_t)1 << 27))
+        REFUSE(PTTS_E_UNSUPPORTED, "slots of a page 128 MiB or more apart");
     if (!aligned(c->k, c->k_strides, 3, 16, esz) || !aligned(c->v, c->v_strides, 3, 16, esz))
         REFUSE(PTTS_E_INVALID, "cache rows must start at multiples of 16 bytes");
     return PTTS_OK;

@@ -25,11 +25,11 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(8))) short s16x8;
 
-template <int N> __device__ inline void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
-__device__ inline void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-template <typename P> __device__ inline void load16(const typename P::elem_t* p, float* f);
-template <> __device__ inline void load16<PBF16>(const uint16_t* p, float* f) {
+template <typename P> __device__ __forceinline__ void load16(const typename P::elem_t* p, float* f);
+template <> __device__ __forceinline__ void load16<PBF16>(const uint16_t* p, float* f) {
     const u32x4 r = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -38,12 +38,12 @@ template <> __device__ inline void load16<PBF16>(const uint16_t* p, float* f) {
         f[2 * i + 1] = __builtin_bit_cast(float, w & 0xffff0000u);
     }
 }
-template <> __device__ inline void load16<PF32>(const float* p, float* f) {
+template <> __device__ __forceinline__ void load16<PF32>(const float* p, float* f) {
     const f32x4 r = *reinterpret_cast<const f32x4*>(p);
     f[0] = r[0]; f[1] = r[1]; f[2] = r[2]; f[3] = r[3];
 }
 
-__device__ inline float swap_max32(float x) {      // maximum over lanes l and l ^ 32
+__device__ __forceinline__ float swap_max32(float x) {      // maximum over lanes l and l ^ 32
 #if defined(__HIP_DEVICE_COMPILE__)
     const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
     const unsigned r0 = r[0], r1 = r[1];
@@ -52,7 +52,7 @@ __device__ inline float swap_max32(float x) {      // maximum over lanes l and l
     return x;
 #endif
 }
-__device__ inline float swap_max16(float x) {      // maximum over lanes l and l ^ 16
+__device__ __forceinline__ float swap_max16(float x) {      // maximum over lanes l and l ^ 16
 #if defined(__HIP_DEVICE_COMPILE__)
     const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
     const unsigned r0 = r[0], r1 = r[1];
@@ -61,106 +61,194 @@ __device__ inline float swap_max16(float x) {      // maximum over lanes l and l
     return x;
 #endif
 }
-__device__ inline float exp2_hw(float x) {
+__device__ __forceinline__ float exp2_hw(float x) {
 #if defined(__HIP_DEVICE_COMPILE__)
     return __builtin_amdgcn_exp2f(x);
 #else
     return x;
 #endif
 }
-// Transposing reads of V: 16 lanes take a block of 4 keys x 16 features (each lane 4 features of one key), lane i ends with feature i of
-// the 4 keys.  A and B are the two blocks of a matrix step.  Written out, because hipcc drains the LDS-DMA in flight in front of the
-// builtin; the wait stands in the same statement as the reads.
-template <int OFF_A, int OFF_B> __device__ inline void read_v4(unsigned a0, unsigned a1, unsigned a2, unsigned a3, s16x8 (&v)[4]) {
+// Transposing read of V: 16 lanes take a block of 4 keys x 16 features (each lane 4 features of one key), lane i ends with feature i of
+// the 4 keys.  The two halves of a matrix step's operand.
+__device__ __forceinline__ bf16x8 read_v(unsigned lo, unsigned hi) {
+    s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
 #if defined(__HIP_DEVICE_COMPILE__)
-    s16x4 r[8];
-    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
-                 "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
-                 "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
-                 "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
-                 "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
-                 : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(OFF_A), "n"(OFF_B) : "memory");
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __builtin_shufflevector(r[2 * i], r[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)lo);
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)hi);
+    v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+#endif
+    return __builtin_bit_cast(bf16x8, v);
+}
+__device__ __forceinline__ u32x4 read_lds(unsigned p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+    return *(lds_u32x4*)(uintptr_t)p;
+#else
+    return {0, 0, 0, 0};
 #endif
 }
-// the same for two feature blocks a0, a1 of two steps
-template <int A, int B, int C, int D> __device__ inline void read_v2(unsigned a0, unsigned a1, s16x8 (&v)[4]) {
+__device__ __forceinline__ float read_lds_f32(unsigned p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    s16x4 r[8];
-    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%10\n\tds_read_b64_tr_b16 %1, %8 offset:%11\n\t"
-                 "ds_read_b64_tr_b16 %2, %9 offset:%10\n\tds_read_b64_tr_b16 %3, %9 offset:%11\n\t"
-                 "ds_read_b64_tr_b16 %4, %8 offset:%12\n\tds_read_b64_tr_b16 %5, %8 offset:%13\n\t"
-                 "ds_read_b64_tr_b16 %6, %9 offset:%12\n\tds_read_b64_tr_b16 %7, %9 offset:%13\n\t"
-                 "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
-                 : "v"(a0), "v"(a1), "n"(A), "n"(B), "n"(C), "n"(D) : "memory");
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __builtin_shufflevector(r[2 * i], r[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+    typedef __attribute__((address_space(3))) const float lds_f32;
+    return *(lds_f32*)(uintptr_t)p;
+#else
+    return 0.f;
 #endif
 }
-__device__ inline unsigned lds_address(const void* p) {
+__device__ __forceinline__ unsigned lds_address(const void* p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 #else
     return 0;
 #endif
 }
-template <int I, int N, typename F> __device__ inline void unrolled(F&& f) {      // f(integral constant I), f(I + 1), ...
-    if constexpr (I < N) { f(std::integral_constant<int, I>()); unrolled<I + 1, N>(f); }
+// Chunk c (16 bytes) of row r stands at chunk c ^ swizzle(r) of the row's LDS image.  16 lanes that read one chunk of 16 rows (K), and 32
+// lanes that read 4 x 64 or 8 x 32 bytes of neighbouring rows (V), then meet in no bank: 64 banks hold 16 chunks, and the low bits of the
+// row move the high bits of the chunk (bf16) or, for f32 (V: 4 rows 4 apart, 64 bytes each), bits 2 and 3 do.
+template <int RB, bool BF16> __device__ __forceinline__ unsigned swizzle(unsigned r) {
+    if (RB == 128) return ((r >> 1 & 1) << 2) | ((r >> 2 & 1) << 1) | (r >> 3 & 1);
+    return BF16 ? ((r & 3) << 2) | ((r >> 2 & 1) << 1) | (r >> 3 & 1) : r & 15;
 }
-__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+template <int I, int N, typename F> __device__ __forceinline__ void each(F&& f) {      // f(0), f(1), ... with the number as a type
+    if constexpr (I < N) { f(std::integral_constant<int, I>()); each<I + 1, N>(f); }
+}
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// ---- where a workgroup's rows lie ------------------------------------------------------------------------------------------
-struct Span {          // one sequence's new tokens
-    int seq, first, n, past;
-    bool bad;          // its length leads behind its row of the page table: every row becomes NaN
+// ---- which rows and keys a workgroup takes -------------------------------------------------------------------------------------
+// A launch's items are (tile of M rows of a sequence, share of its keys, key head).  Their numbers come from the lengths on the device:
+// every wave sums the sequences' tiles up for itself, 64 sequences at a time, all lengths in one round trip.  Items are numbered without
+// holes (with holes between the sequences the dispatcher put all work of equal chunks on half of the CUs).
+// Keys are shared out only where that evens the load: SLOTS workgroups run at a time, and a tile whose keys exceed what one of them would
+// get of everything (by the factor LAG) is cut into shares of that size, at least MIN_SHARE keys each (a share costs its rows' f32 partial
+// results, written and read once more).
+constexpr int SLOTS = 512, MIN_SHARE = 256, MAX_SPLITS = 256;
+constexpr float TILE_LAG = 2.f, STEP_LAG = 2.f;
+
+struct Item {
+    int seq, first, n, past;    // the sequence, its first token, its new tokens, its cached ones
+    int tile, split, splits;    // of the sequence's tiles; share of the keys; shares of this tile
+    int end, k0, k1;            // keys any of the tile's rows sees; this item's keys
+    bool bad;                   // the length leads behind the row of the page table: every row becomes NaN
 };
 
-// The sequence and its tile that tile t of a launch is, where tiles hold M rows: a prefix sum over the sequences' tiles, 64 sequences at
-// a time, by every wave for itself (lengths and cache lengths come in one round trip).  Tiles of no sequence are the launch's last ones:
-// with holes between the sequences (a numbering that needs no sum) the dispatcher put all work of equal chunks on half of the CUs.
-__device__ inline bool find_tile(const PagedAttnArgs& a, int t, int M, Span* sp, int* tile) {
-    if (!a.starts) {
-        const int per = (a.group + M - 1) / M, s = t / per;
-        sp->seq = sp->first = s;
-        sp->n = 1;
-        sp->past = uniform(a.past[s]);
-        *tile = t - s * per;
-    } else {
-        const int lane = threadIdx.x & 63;
-        int rest = t, i0 = 0, sel, first = 0, n = 0, past = 0, sum;
-        for (;; i0 += 64) {
-            if (i0 >= a.n_seqs) return false;
-            const int i = min(i0 + lane, a.n_seqs - 1);
+template <int M, int KT> struct Schedule {
+    int first, n, past;         // this lane's sequence of the current 64
+    int base;                   // its number - lane
+    int share;                  // tiles of KT keys of a share (of all keys: not cut)
+    int items;                  // (tile, share) pairs of the batch
+
+    __device__ __forceinline__ void load(const PagedAttnArgs& a, int i0) {
+        const int lane = threadIdx.x & 63, i = min(i0 + lane, a.n_seqs - 1);
+        base = i0;
+        if (a.starts) {
             first = a.starts[i];
             const int end = a.starts[i + 1];
-            past = a.past[i];
-            n = i0 + lane < a.n_seqs && first >= 0 && end <= a.tokens ? max(end - first, 0) : 0;       // starts that are wrong own no rows
-            const int own = (n * a.group + M - 1) / M;
-            sum = own;
+            n = first >= 0 && end <= a.tokens ? max(end - first, 0) : 0;      // starts that are wrong own no rows
+        } else { first = i; n = 1; }
+        past = a.past[i];
+        if (i0 + lane >= a.n_seqs) n = 0;
+    }
+    __device__ __forceinline__ bool bad_length(const PagedAttnArgs& a, int np, int pp) const {
+        return pp < 0 || (int64_t)pp + (a.causal ? np : 0) > ((int64_t)a.max_pages << a.page_shift);
+    }
+    __device__ __forceinline__ int row_tiles(const PagedAttnArgs& a) const { return (n * a.group + M - 1) / M; }
+    __device__ __forceinline__ int key_tiles(const PagedAttnArgs& a) const {
+        return bad_length(a, n, past) ? 1 : (past + (a.causal ? n : 0) + KT - 1) / KT;
+    }
+    __device__ __forceinline__ int own(const PagedAttnArgs& a) const {
+        const int kt = key_tiles(a);
+        return row_tiles(a) * (kt <= share ? 1 : (kt + share - 1) / share);
+    }
+    // share for the whole batch, the number of items
+    __device__ __forceinline__ void plan(const PagedAttnArgs& a, float lag) {
+        share = 0x3fffffff;
+        load(a, 0);
+        if (a.splits > 1) {
+            float work = 0.f;
+            int most = 0;
+            for (int i0 = 0;;) {
+                const int rt = row_tiles(a), kt = key_tiles(a);
+                work += (float)rt * (float)(a.causal ? max(kt - n / (2 * KT), 1) : kt);
+                most = max(most, rt > 0 ? kt : 0);
+                i0 += 64;
+                if (i0 >= a.n_seqs) break;
+                load(a, i0);
+            }
+            const float mean = wave_sum(work) * (float)a.kv_heads / SLOTS;
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) most = max(most, __shfl_xor(most, d));
+            if ((float)most > lag * mean) share = max(max((int)ceilf(mean), MIN_SHARE / KT), (most + a.splits - 1) / a.splits);
+            if (a.n_seqs > 64) load(a, 0);
+        }
+        share = uniform(share);
+        count(a);
+    }
+    __device__ __forceinline__ void count(const PagedAttnArgs& a) {
+        int sum = 0;
+        for (int i0 = 0;;) {
+            sum += own(a);
+            i0 += 64;
+            if (i0 >= a.n_seqs) break;
+            load(a, i0);
+        }
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+        items = uniform(sum);
+    }
+    // item t < items
+    __device__ __forceinline__ void find(const PagedAttnArgs& a, int t, Item* it) {
+        const int lane = threadIdx.x & 63;
+        int sel, sum, ours;
+        if (base != 0) load(a, 0);
+        for (;;) {
+            ours = own(a);
+            sum = ours;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) { const int x = __shfl_up(sum, d); sum += lane >= d ? x : 0; }
-            sel = __popcll(__ballot(sum <= rest));
-            if (sel < 64) { sum -= own; break; }
-            rest -= __builtin_amdgcn_readlane(sum, 63);
+            sel = __popcll(__ballot(sum <= t));
+            if (sel < 64 || base + 64 >= a.n_seqs) break;
+            t -= __builtin_amdgcn_readlane(sum, 63);
+            load(a, base + 64);
         }
-        sel = uniform(sel);
-        sp->seq = i0 + sel;
-        sp->first = __builtin_amdgcn_readlane(first, sel);
-        sp->n = __builtin_amdgcn_readlane(n, sel);
-        sp->past = __builtin_amdgcn_readlane(past, sel);
-        *tile = rest - __builtin_amdgcn_readlane(sum, sel);
-        if (sp->n == 0) return false;
+        sel = uniform(min(sel, 63));
+        it->seq = base + sel;
+        it->first = __builtin_amdgcn_readlane(first, sel);
+        it->n = __builtin_amdgcn_readlane(n, sel);
+        it->past = __builtin_amdgcn_readlane(past, sel);
+        t -= __builtin_amdgcn_readlane(sum - ours, sel);
+        const int tiles = (it->n * a.group + M - 1) / M, cuts = __builtin_amdgcn_readlane(ours, sel) / max(tiles, 1);
+        it->tile = cuts > 1 ? t / cuts : t;
+        it->split = t - it->tile * cuts;
+        it->tile = tiles - 1 - it->tile;               // the rows that see most first
+        it->bad = bad_length(a, it->n, it->past);
+        if (it->bad) it->past = 0;
+        it->end = it->bad ? 0 : it->past;
+        if (a.causal && !it->bad) it->end += (min((it->tile + 1) * M, it->n * a.group) - 1) / a.group + 1;
+        const int kt = (it->end + KT - 1) / KT;
+        it->splits = kt <= share ? 1 : (kt + share - 1) / share;
+        it->k0 = it->k1 = 0;
+        if (it->splits == 1) it->k1 = it->split == 0 ? it->end : 0;
+        else if (it->split < it->splits) { it->k0 = it->split * share * KT; it->k1 = min(it->k0 + share * KT, it->end); }
     }
-    const int64_t reach = (int64_t)a.max_pages << a.page_shift;
-    sp->bad = sp->past < 0 || (int64_t)sp->past + (a.causal ? sp->n : 0) > reach;
-    if (sp->bad) {
-        if (threadIdx.x == 0) atomicOr(a.status, PAGED_BAD_LENGTH);
-        sp->past = 0;
-    }
-    return true;
+};
+
+// The arguments once more, for what stands behind a main loop: read there, instead of kept in scalar registers through it.
+__device__ __forceinline__ PagedAttnArgs arguments_again() {
+    PagedAttnArgs z = {};
+#if defined(__HIP_DEVICE_COMPILE__)
+    uintptr_t p = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    typedef const __attribute__((address_space(4))) PagedAttnArgs kernarg;
+    __builtin_memcpy(&z, (kernarg*)p, sizeof(z));
+#endif
+    return z;
+}
+
+template <typename S> __device__ __forceinline__ void begin(const PagedAttnArgs& a, S& sched, float lag) {
+    if (blockIdx.x == 0 && a.starts) check_starts(a.starts, a.n_seqs, a.tokens, a.status);
+    sched.plan(a, lag);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.splits > 1) a.part[0] = __builtin_bit_cast(float, sched.share);
 }
 
 // ---- page ids of the keys ahead, one per lane ---------------------------------------------------------------------------------
@@ -168,7 +256,7 @@ struct Pages {
     const int* row;
     int base, ids, n_pages;     // lane l holds the id of page base + l
     bool bad;
-    __device__ inline void load(int first, int last) {       // pages first .. (at most 64), none behind `last`
+    __device__ __forceinline__ void load(int first, int last) {       // pages first .. (at most 64), none behind `last`
         base = first;
         const int i = first + (int)(threadIdx.x & 63);
         ids = row[min(i, last)];
@@ -176,33 +264,58 @@ struct Pages {
         bad = bad || __any(wrong);
         if (wrong) ids = 0;
     }
-    __device__ inline int get(int page) const { return __builtin_amdgcn_readlane(ids, page - base); }
+    __device__ __forceinline__ int get(int page) const { return __builtin_amdgcn_readlane(ids, page - base); }
 };
 
-// ---- a tile of KT rows of K or V on its way to LDS: one wave moves ROWS of them -------------------------------------------------
-// chunk c (16 bytes) of row r stands at chunk c ^ (r & 7) of the row's LDS image.  Rows at or behind `end` are read from the last row
-// in front of it: what lies there is seen by nobody, and may be anything.
-template <typename P, int D, int ROWS>
-__device__ inline void dma_rows(const char* base, int64_t page_bytes, int64_t slot_bytes, const Pages& pg, int page_shift, int key0, int row0,
-                                int end, char* lds) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    typedef __attribute__((address_space(3))) void lds_void;
-    constexpr int RB = D * (int)sizeof(typename P::elem_t), RPI = 1024 / RB, CPR = RB / 16;
-    const int lane = threadIdx.x & 63, rl = lane / CPR, c = lane % CPR;
-    const int mask = (1 << page_shift) - 1;
-#pragma unroll
-    for (int i = 0; i < ROWS / RPI; ++i) {
-        const int r = row0 + i * RPI;                                   // first row of this instruction: its rows share a page
-        const int page = pg.get(min(key0 + r, end - 1) >> page_shift);
-        const int slot = min(key0 + r + rl, end - 1) & mask;
-        const char* src = base + page * page_bytes + slot * slot_bytes + ((c ^ ((r + rl) & 7)) << 4);
-        __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(src), (lds_void*)(lds + r * RB), 16, 0, 0);
+// ---- ROWS rows of K or V on their way to LDS, by one wave ------------------------------------------------------------------------
+// Rows at or behind `end` are read from the last row in front of it: what lies there is seen by nobody, and may be anything.  A wave
+// instruction moves RPI rows, which share a page (pages hold 16 tokens or more); its address is a scalar base and a 32-bit lane offset
+// (slot strides are below 2^27 bytes).  The LDS-DMA is written out: behind its builtin hipcc drains every transfer in flight in front of
+// the next transposing read, wherever that reads.  It has no register results; the kernels wait for it by counted vmcnt.
+template <typename P, int D> struct Rows {
+    static constexpr int RB = D * (int)sizeof(typename P::elem_t), RPI = 1024 / RB, CPR = RB / 16;
+    const char* base;
+    int64_t page_bytes;
+    int slot_bytes;
+    __device__ __forceinline__ Rows(const void* cache, const int64_t* strides, int kvh) {
+        constexpr int E = sizeof(typename P::elem_t);
+        base = reinterpret_cast<const char*>(cache) + kvh * strides[1] * E;
+        page_bytes = strides[0] * E;
+        slot_bytes = (int)(strides[2] * E);
     }
+    template <int ROWS> __device__ __forceinline__ void fetch(const Pages& pg, int page_shift, int key0, int row0, int end, unsigned lds) const {
+        const int lane = threadIdx.x & 63, rl = lane / CPR, c = lane % CPR, mask = (1 << page_shift) - 1;
+#pragma unroll
+        for (int i = 0; i < ROWS / RPI; ++i) {
+            const int r = row0 + i * RPI;
+            const unsigned chunk = (c ^ swizzle<RB, P::IS_BF16>((r + rl) & 15)) << 4;
+            if (key0 + r + RPI <= end) {
+                send(base + pg.get((key0 + r) >> page_shift) * page_bytes + (int64_t)((key0 + r) & mask) * slot_bytes, rl * slot_bytes + chunk, lds + r * RB);
+            } else {                                            // some of the rows, or all, are behind the end
+                const int last = min(key0 + r, end - 1);
+                send(base + pg.get(last >> page_shift) * page_bytes + (int64_t)(last & mask) * slot_bytes,
+                     (min(key0 + r + rl, end - 1) - last) * slot_bytes + chunk, lds + r * RB);
+            }
+        }
+    }
+    static __device__ __forceinline__ void send(const char* src, unsigned off, unsigned lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(src) : "memory");
 #endif
-}
+    }
+    // 16 rows that are all there (key a multiple of 16: they share a page), one instruction a time
+    __device__ __forceinline__ const char* slice(const Pages& pg, int page_shift, int key) const {
+        return base + pg.get(key >> page_shift) * page_bytes + (int64_t)(key & ((1 << page_shift) - 1)) * slot_bytes;
+    }
+    template <int I> __device__ __forceinline__ void fetch_one(const char*& src, unsigned lds, unsigned lane) const {
+        const unsigned rl = lane / CPR, c = lane % CPR;
+        send(src, rl * (unsigned)slot_bytes + ((c ^ swizzle<RB, P::IS_BF16>(I * RPI + rl)) << 4), lds + I * RPI * RB);
+        src += RPI * slot_bytes;
+    }
+};
 
 // keys that may be looked at at all, as bits: the key mask's bytes of the tile (lane i: key key0 + i), ones behind its last column
-__device__ inline uint64_t tile_mask(const PagedAttnArgs& a, int seq, int key0) {
+__device__ __forceinline__ uint64_t tile_mask(const PagedAttnArgs& a, int seq, int key0) {
     if (!a.mask || key0 >= a.mask_width) return ~0ull;
     const int j = key0 + (int)(threadIdx.x & 63);
     bool live = true;
@@ -212,7 +325,7 @@ __device__ inline uint64_t tile_mask(const PagedAttnArgs& a, int seq, int key0) 
 
 // ---- one query over the keys [k0, k1) it sees, by one wave (see the head of the file) ------------------------------------------
 template <typename P, int D>
-__device__ inline void row_alone(const PagedAttnArgs& a, int seq, int kvh, const typename P::elem_t* q, int k0, int k1, float* m_out, float* l_out,
+__device__ __forceinline__ void row_alone(const PagedAttnArgs& a, int seq, int kvh, const typename P::elem_t* q, int k0, int k1, float* m_out, float* l_out,
                                  float (&acc)[D / 64]) {
     typedef typename P::elem_t elem_t;
     constexpr int V = 16 / sizeof(elem_t), R = D / 64;
@@ -259,51 +372,312 @@ __device__ inline void row_alone(const PagedAttnArgs& a, int seq, int kvh, const
     *m_out = m; *l_out = l;
 }
 
-// where the partial results of a split launch lie: outputs [split][token * q_heads + head][D], behind them (maximum, sum) pairs
-template <int D> __device__ inline float* part_out(const PagedAttnArgs& a, int split, int64_t row) {
-    return a.part + ((int64_t)split * a.tokens * a.q_heads + row) * D;
+// where the partial results of cut tiles lie: the share (for the join), outputs [split][token * q_heads + head][D], (maximum, sum) pairs
+constexpr int PART_HEAD = 4;
+template <int D> __device__ __forceinline__ float* part_out(const PagedAttnArgs& a, int split, int64_t row) {
+    return a.part + PART_HEAD + ((int64_t)split * a.tokens * a.q_heads + row) * D;
 }
-template <int D> __device__ inline float* part_ml(const PagedAttnArgs& a, int split, int64_t row) {
+template <int D> __device__ __forceinline__ float* part_ml(const PagedAttnArgs& a, int split, int64_t row) {
     const int64_t rows = (int64_t)a.tokens * a.q_heads;
-    return a.part + (int64_t)a.splits * rows * D + (split * rows + row) * 2;
+    return a.part + PART_HEAD + (int64_t)a.splits * rows * D + (split * rows + row) * 2;
 }
 
 template <typename P, int D>
-__device__ inline void store_row_alone(const PagedAttnArgs& a, int seq, int kvh, int64_t token, int head, int split, int k0, int k1) {
+__device__ __forceinline__ void store_row_alone(const PagedAttnArgs& a, const Item& it, int kvh, int row) {
     typedef typename P::elem_t elem_t;
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, tok = row / a.group, head = kvh * a.group + row - tok * a.group;
+    const int64_t token = it.first + tok;
     float m, l, acc[D / 64];
-    row_alone<P, D>(a, seq, kvh, reinterpret_cast<const elem_t*>(a.q) + token * a.qs[0] + head * a.qs[1], k0, k1, &m, &l, acc);
-    const int64_t row = token * a.q_heads + head;
+    row_alone<P, D>(a, it.seq, kvh, reinterpret_cast<const elem_t*>(a.q) + token * a.qs[0] + head * a.qs[1], it.k0,
+                    min(it.k1, it.past + (a.causal ? tok + 1 : 0)), &m, &l, acc);
+    const int64_t orow = token * a.q_heads + head;
 #pragma unroll
     for (int r = 0; r < D / 64; ++r) {
-        if (a.splits > 1) part_out<D>(a, split, row)[r * 64 + lane] = acc[r];
+        if (it.splits > 1) part_out<D>(a, it.split, orow)[r * 64 + lane] = acc[r];
         else (reinterpret_cast<elem_t*>(a.out) + token * a.os[0] + head * a.os[1])[r * 64 + lane] = to_elem<P>(l == 0.f ? 0.f : acc[r] / l);
     }
-    if (a.splits > 1 && lane == 0) { float* ml = part_ml<D>(a, split, row); ml[0] = m; ml[1] = l; }
+    if (it.splits > 1 && lane == 0) { float* ml = part_ml<D>(a, it.split, orow); ml[0] = m; ml[1] = l; }
 }
 
-// keys of split `split`: equal shares of whole tiles
-__device__ inline void split_range(const PagedAttnArgs& a, int split, int end, int KT, int* k0, int* k1) {
-    if (a.splits == 1) { *k0 = 0; *k1 = end; return; }
-    const int tiles = (end + KT - 1) / KT, share = (tiles + a.splits - 1) / a.splits;
-    *k0 = min(split * share * KT, end);
-    *k1 = min(*k0 + share * KT, end);
-}
-
-template <typename P> __device__ inline void store4(typename P::elem_t* p, float a, float b, float c, float d);
-template <> __device__ inline void store4<PBF16>(uint16_t* p, float a, float b, float c, float d) {
+template <typename P> __device__ __forceinline__ void store4(typename P::elem_t* p, float a, float b, float c, float d);
+template <> __device__ __forceinline__ void store4<PBF16>(uint16_t* p, float a, float b, float c, float d) {
     typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
     const bf16x4 v = {(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)d};
     *reinterpret_cast<bf16x4*>(p) = v;
 }
-template <> __device__ inline void store4<PF32>(float* p, float a, float b, float c, float d) {
+template <> __device__ __forceinline__ void store4<PF32>(float* p, float a, float b, float c, float d) {
     const f32x4 v = {a, b, c, d};
     *reinterpret_cast<f32x4*>(p) = v;
 }
 
 // =================================================================================================================================
-// Chunks: a workgroup owns 128 rows (32 per wave), the keys pass in tiles of KT through a ring of LDS buffers.
+// Chunks in bf16: a workgroup owns 128 rows (32 per wave), the keys pass in tiles of 64.
+// One wave alone keeps the matrix unit busy: the products of the NEXT tile's scores go out between the exponentials of this one, the
+// products with V between the additions of its weights and the maximum of the next scores.  (With a tile's steps one after the other, two
+// waves per SIMD spent 2300 cycles on 1024 of matrix work at D = 128; they overlap their phases only by chance.)  K runs one tile ahead of
+// V, so each has a ring of its own: iteration i sends for K(i + NB) and V(i + NB - 1) into the buffers that iteration i - 1 left, one
+// instruction between two products.  Iterations with less in front of the end are written out apart: they wait for all in flight.
+// =================================================================================================================================
+template <int D> struct ChunkCfg {
+    static constexpr int M = 128, NW = 4, KT = 64, RB = D * 2;
+    static constexpr int TILE = KT * RB;
+    static constexpr int NB = 65536 / (2 * TILE);              // 64 KiB of LDS: two workgroups on a CU
+    static constexpr int LDS = 2 * NB * TILE;                  // [K ring][V ring]
+    static constexpr int DMA = TILE / NW / 1024;               // LDS-DMA instructions per wave and tile of K or of V
+};
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void paged_attn_chunk_kernel(PagedAttnArgs a) {
+    typedef PBF16 P;
+    typedef uint16_t elem_t;
+    typedef ChunkCfg<D> C;
+    constexpr int KT = C::KT, RB = C::RB, NB = C::NB, NKS = D / 16, NDB = D / 32, NQ = 2 * NKS, NP = 4 * NDB;
+    __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
+    const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l31 = lane & 31, h = lane >> 5;
+
+    Schedule<C::M, KT> sched;
+    begin(a, sched, TILE_LAG);
+    const int item = blockIdx.x;
+    if (item >= sched.items * a.kv_heads) return;
+    // consecutive workgroups go to consecutive XCDs: with the key head innermost, an XCD's L2 holds few heads' pages
+    const int kvh = item % a.kv_heads;
+    Item it;
+    sched.find(a, item / a.kv_heads, &it);
+    if (it.split >= it.splits) return;
+    const int k0 = it.k0, k1 = it.k1, r0 = it.tile * C::M, r_end = min(r0 + C::M, it.n * a.group);
+    int row = r0 + w * 32 + l31;                               // this lane's query
+    int lim;                                                   // keys 0 .. lim - 1 are seen
+    const int wr0 = r0 + w * 32, wr1 = min(wr0 + 32, r_end);                            // rows of this wave: [wr0, wr1)
+    const bool some = wr0 < wr1 && !it.bad;
+    const int w_end = some ? it.past + (a.causal ? (wr1 - 1) / a.group + 1 : 0) : 0;    // keys any of them sees
+    const int w_all = some ? it.past + (a.causal ? wr0 / a.group + 1 : 0) : 0;          // keys all of them see
+
+    Pages pg;
+    pg.row = a.table + it.seq * a.table_stride; pg.n_pages = a.n_pages; pg.bad = false; pg.base = 0; pg.ids = 0;
+    const Rows<P, D> krows(a.k, a.kc, kvh), vrows(a.v, a.vc, kvh);
+    const unsigned kring = lds_address(smem), vring = kring + NB * C::TILE;
+    const int last_page = (k1 - 1) >> a.page_shift;
+    // K of the tile at key0, V of the tile in front of it
+    auto fetch_k = [&](int key0, int buf) { krows.template fetch<KT / C::NW>(pg, a.page_shift, key0, w * (KT / C::NW), k1, kring + buf * C::TILE); };
+    auto fetch_v = [&](int key0, int buf) { vrows.template fetch<KT / C::NW>(pg, a.page_shift, key0, w * (KT / C::NW), k1, vring + buf * C::TILE); };
+    auto pages_for = [&](int vkey, int kkey) {
+        if (((min(kkey + KT, k1) - 1) >> a.page_shift) >= pg.base + 64) pg.load(min(vkey, k1 - 1) >> a.page_shift, last_page);
+    };
+    // lane parts of the LDS addresses: row l31 of K (chunk 2 t + h at step t), the two blocks of read_v
+    const unsigned ka = l31 * RB + ((h ^ swizzle<RB, true>(l31 & 15)) << 4);
+    const int i16 = lane & 15, vr = 4 * h + (i16 >> 2), vc = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
+    const unsigned va = vr * RB + ((vc ^ swizzle<RB, true>(vr)) << 4) + (i16 & 1) * 8;
+    const unsigned vb = (vr + 8) * RB + ((vc ^ swizzle<RB, true>(vr + 8)) << 4) + (i16 & 1) * 8;
+
+    bf16x8 qf[NKS];
+    {
+        const bool live = row < r_end;
+        const int tok = live ? row / a.group : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
+        lim = live && !it.bad ? it.past + (a.causal ? tok + 1 : 0) : 0;
+        const elem_t* qp = reinterpret_cast<const elem_t*>(a.q) + (int64_t)(it.first + tok) * a.qs[0] + head * a.qs[1];
+#pragma unroll
+        for (int t = 0; t < NKS; ++t) qf[t] = *reinterpret_cast<const bf16x8*>(qp + (2 * t + h) * 8);
+    }
+    f32x16 o[NDB], sa[2], sb[2];      // the scores of a tile and of the next take turns
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    float m = -INFINITY, l = 0.f;       // maximum of the query's scores (log2 units), sum of the weights of this half's keys
+
+    if (k0 < k1) pg.load(k0 >> a.page_shift, last_page);
+    // the query rows arrive before the first tile is sent for: a wait for them further on would be one for the tiles in flight too
+#pragma unroll
+    for (int t = 0; t < NKS; ++t) asm volatile("" : "+v"(qf[t]));
+    if (k0 < k1) {
+        fetch_k(k0, 0);
+#pragma unroll
+        for (int j = 1; j < NB; ++j) {                         // rows behind the end are its last row: as many transfers for a short range
+            pages_for(k0 + (j - 1) * KT, k0 + j * KT);
+            fetch_k(k0 + j * KT, j);
+            fetch_v(k0 + (j - 1) * KT, j - 1);
+        }
+        wait_vm<(NB - 1) * 2 * C::DMA>();
+        __builtin_amdgcn_s_barrier();
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sa[b][r] = 0.f;
+#pragma unroll
+            for (int t = 0; t < NKS; ++t)
+                sa[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, read_lds(kring + b * 32 * RB + (ka ^ (t << 5)))), qf[t], sa[b], 0, 0, 0);
+        }
+    }
+    float mx = -INFINITY;               // maximum of a tile's scores, unmasked
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sa[b][r]);
+    int buf = 0;                        // of V(i), and of the K(i) that is in `s`
+    // one tile; FULL: the tiles it sends for lie in front of the end
+    auto iteration = [&](int key0, f32x16 (&s)[2], f32x16 (&sn)[2], auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        const int knext = buf + 1 == NB ? 0 : buf + 1, free_v = buf == 0 ? NB - 1 : buf - 1;
+        if constexpr (FULL) wait_vm<(NB - 2) * 2 * C::DMA>();
+        else wait_vm<0>();
+        wait_lds();
+        __builtin_amdgcn_s_barrier();        // K(i + 1) and V(i) have landed, every wave has left K(i) and V(i - 1)
+        const unsigned kt = kring + knext * C::TILE, vt = vring + buf * C::TILE;
+        const unsigned ksend = kring + buf * C::TILE + w * (KT / C::NW) * RB, vsend = vring + free_v * C::TILE + w * (KT / C::NW) * RB;
+        pages_for(key0 + (NB - 1) * KT, key0 + NB * KT);
+        const char *ksrc = nullptr, *vsrc = nullptr;
+        if constexpr (FULL) {
+            ksrc = krows.slice(pg, a.page_shift, key0 + NB * KT + w * (KT / C::NW));
+            vsrc = vrows.slice(pg, a.page_shift, key0 + (NB - 1) * KT + w * (KT / C::NW));
+        } else {
+            if (key0 + NB * KT < k1) fetch_k(key0 + NB * KT, buf);
+            if (key0 + (NB - 1) * KT < k1) fetch_v(key0 + (NB - 1) * KT, free_v);
+        }
+        buf = knext;
+        unsigned dma_lane = lane;
+        asm volatile("" : "+v"(dma_lane));   // the lane offsets of the transfers are computed anew (8 registers)
+        if (key0 >= w_end) {                 // nothing here for this wave's rows (it keeps moving its share of the tiles)
+            if constexpr (FULL) {
+                each<0, C::DMA>([&](auto I) { krows.template fetch_one<decltype(I)::value>(ksrc, ksend, dma_lane); });
+                each<0, C::DMA>([&](auto I) { vrows.template fetch_one<decltype(I)::value>(vsrc, vsend, dma_lane); });
+            }
+            return;
+        }
+        // operand fragments from LDS, AHEAD steps ahead: K of the next tile (steps 0 .. NQ - 1), then V of this one.  (The step is xor-ed into
+        // the whole address, not into its lane part: that would be 16 registers kept.)
+        constexpr int RING = D == 64 ? 8 : 6, AHEAD = RING - 1;
+        bf16x8 fr[RING];
+        const unsigned kat = kt + ka, vat = vt + va, vbt = vt + vb;
+        auto fragment = [&](int u) {
+            if (u < NQ) fr[u % RING] = __builtin_bit_cast(bf16x8, read_lds((kat ^ (u % NKS << 5)) + (u / NKS) * 32 * RB));
+            else {
+                const int v = u - NQ;
+                fr[u % RING] = read_v((vat ^ (v % NDB << 6)) + 16 * (v / NDB) * RB, (vbt ^ (v % NDB << 6)) + 16 * (v / NDB) * RB);
+            }
+        };
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) fragment(u);
+        const uint64_t alive = tile_mask(a, it.seq, key0);
+        if (key0 + KT > w_all || alive != ~0ull) {             // some key of the tile is not for some query
+            const int left = lim - key0;
+            const uint64_t see = (left >= 64 ? ~0ull : (left <= 0 ? 0ull : (1ull << left) - 1)) & alive;
+            const uint32_t half[2] = {(uint32_t)(see >> (4 * h)), (uint32_t)(see >> 32 >> (4 * h))};
+            mx = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[b][r] = (half[b] >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[b][r] : -INFINITY;
+                    mx = fmaxf(mx, s[b][r]);
+                }
+        }
+        mx = swap_max32(mx) * a.scale_log2;
+        // weights are kept relative to a maximum that may lag behind by 2^8 (their type holds that range as well as any): the sums
+        // are rescaled only when a query's maximum has risen further
+        if (__any(mx > m + 8.f)) {
+            const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.f : exp2_hw(m - mn);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < NDB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= al;
+        }
+        const float mu = m == -INFINITY ? 0.f : m;
+
+        // scores of the next tile (behind the last: of whatever the buffer holds, unused) beside the weights of this one
+        bf16x8 pf[4];
+        constexpr int SQ = 32 / NQ, SP = 32 / NP, EVERY = NQ / (2 * C::DMA);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sn[0][r] = sn[1][r] = 0.f;
+        __builtin_amdgcn_sched_barrier(0);
+        each<0, NQ>([&](auto U) {
+            constexpr int u = decltype(U)::value;
+            if (u + AHEAD < NQ + NP) fragment(u + AHEAD);
+            sn[u / NKS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[u % RING], qf[u % NKS], sn[u / NKS], 0, 0, 0);
+            if constexpr (FULL && u % EVERY == 0) {
+                constexpr int i = u / EVERY;
+                if constexpr (i < C::DMA) krows.template fetch_one<i>(ksrc, ksend, dma_lane);
+                else vrows.template fetch_one<i - C::DMA>(vsrc, vsend, dma_lane);
+            }
+#pragma unroll
+            for (int j = 0; j < SQ; ++j) {
+                const int e = u * SQ + j;
+                s[e >> 4][e & 15] = exp2_hw(fmaf(s[e >> 4][e & 15], a.scale_log2, -mu));
+            }
+#pragma unroll
+            for (int j = 0; j < SQ; ++j) {
+                const int e = u * SQ + j;
+                l += s[e >> 4][e & 15];
+                pf[e >> 3][e & 7] = (__bf16)s[e >> 4][e & 15];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        mx = sn[0][0];
+        each<0, NP>([&](auto V) {
+            constexpr int v = decltype(V)::value;
+            if (v + AHEAD < NP) fragment(NQ + v + AHEAD);
+            o[v % NDB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[(NQ + v) % RING], pf[v / NDB], o[v % NDB], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < SP; ++j) mx = fmaxf(mx, sn[(v * SP + j) >> 4][(v * SP + j) & 15]);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    int key0 = k0;
+    for (; key0 + (NB + 2) * KT <= k1; key0 += 2 * KT) {
+        iteration(key0, sa, sb, std::true_type());
+        iteration(key0 + KT, sb, sa, std::true_type());
+    }
+    for (; key0 < k1; key0 += KT) {
+        iteration(key0, sa, sb, std::false_type());
+        sa[0] = sb[0];
+        sa[1] = sb[1];
+    }
+    wait_vm<0>();
+    const PagedAttnArgs z = arguments_again();
+    asm volatile("" : "+v"(row));            // recomputed here, not kept through the loop
+    const bool live = row < r_end;
+    const int tok = live ? row / z.group : 0, head = kvh * z.group + (live ? row - tok * z.group : 0);
+    const int64_t token = it.first + tok;
+    if ((pg.bad || it.bad) && threadIdx.x == 0) atomicOr(z.status, (pg.bad ? PAGED_BAD_PAGE : 0) | (it.bad ? PAGED_BAD_LENGTH : 0));
+    const bool bad = pg.bad || it.bad;
+    l += __shfl_xor(l, 32);
+    float inv = l == 0.f ? 0.f : 1.f / l;
+    if (bad) { l = NAN; inv = NAN; }
+    // a result that is not finite: of this query's own making, or a key that it does not see
+    bool odd = false;
+    if (!bad) {
+        float z = l * 0.f;
+#pragma unroll
+        for (int d = 0; d < NDB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z = fmaf(o[d][r], 0.f, z);
+        odd = live && !(z == 0.f);
+    }
+    const uint64_t odds = __ballot(odd);
+    if (live) {
+        const int64_t orow = token * z.q_heads + head;
+#pragma unroll
+        for (int d = 0; d < NDB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int f = d * 32 + 2 * r + 4 * h;
+                if (it.splits > 1) store4<PF32>(part_out<D>(z, it.split, orow) + f, o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
+                else store4<P>(reinterpret_cast<elem_t*>(z.out) + token * z.os[0] + head * z.os[1] + f, o[d][r] * inv, o[d][r + 1] * inv,
+                               o[d][r + 2] * inv, o[d][r + 3] * inv);
+            }
+        if (it.splits > 1 && h == 0) { float* ml = part_ml<D>(z, it.split, orow); ml[0] = m; ml[1] = l; }
+    }
+    uint32_t again = (uint32_t)odds | (uint32_t)(odds >> 32);
+    while (again) {
+        const int i = __builtin_ctz(again);
+        again &= again - 1;
+        store_row_alone<P, D>(z, it, kvh, wr0 + i);
+    }
+}
+
+// =================================================================================================================================
+// Chunks in f32: a workgroup owns 128 rows (32 per wave), the keys pass in tiles of KT through a ring of LDS buffers.
 // =================================================================================================================================
 template <typename P, int D> struct TileCfg {
     static constexpr int M = 128, NW = 4;
@@ -323,40 +697,41 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
     const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l31 = lane & 31, h = lane >> 5;
 
-    if (blockIdx.x == 0 && a.starts) check_starts(a.starts, a.n_seqs, a.tokens, a.status);
+    Schedule<C::M, KT> sched;
+    begin(a, sched, TILE_LAG);
+    const int item = blockIdx.x;
+    if (item >= sched.items * a.kv_heads) return;
     // consecutive workgroups go to consecutive XCDs: with the key head innermost, an XCD's L2 holds few heads' pages
-    const int kvh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, split = rest % a.splits;
-    Span sp;
-    int tile;
-    if (!find_tile(a, rest / a.splits, C::M, &sp, &tile)) return;
-    const int rows = sp.n * a.group;
-    tile = (rows + C::M - 1) / C::M - 1 - tile;                // the rows that see most first
-    const int r0 = tile * C::M, r_end = min(r0 + C::M, rows);
+    const int kvh = item % a.kv_heads;
+    Item it;
+    sched.find(a, item / a.kv_heads, &it);
+    if (it.split >= it.splits) return;
+    const int k0 = it.k0, k1 = it.k1, r0 = it.tile * C::M, r_end = min(r0 + C::M, it.n * a.group);
     const int row = r0 + w * 32 + l31;                         // this lane's query
     const bool live = row < r_end;
     const int tok = live ? row / a.group : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
-    const int64_t token = sp.first + tok;
-    int lim = live && !sp.bad ? sp.past + (a.causal ? tok + 1 : 0) : 0;       // keys 0 .. lim - 1 are seen
-    const int tile_end = sp.bad ? 0 : sp.past + (a.causal ? (r_end - 1) / a.group + 1 : 0);
-    int k0, k1;
-    split_range(a, split, tile_end, KT, &k0, &k1);
-    const int wr0 = r0 + w * 32, wr1 = min(wr0 + 32, r_end);                  // rows of this wave: [wr0, wr1)
-    const int w_end = wr0 < wr1 && !sp.bad ? (a.causal ? sp.past + (wr1 - 1) / a.group + 1 : sp.past) : 0;   // keys any of them sees
-    const int w_all = wr0 < wr1 && !sp.bad ? (a.causal ? sp.past + wr0 / a.group + 1 : sp.past) : 0;         // keys all of them see
+    const int64_t token = it.first + tok;
+    const int lim = live && !it.bad ? it.past + (a.causal ? tok + 1 : 0) : 0;           // keys 0 .. lim - 1 are seen
+    const int wr0 = r0 + w * 32, wr1 = min(wr0 + 32, r_end);                            // rows of this wave: [wr0, wr1)
+    const bool some = wr0 < wr1 && !it.bad;
+    const int w_end = some ? it.past + (a.causal ? (wr1 - 1) / a.group + 1 : 0) : 0;    // keys any of them sees
+    const int w_all = some ? it.past + (a.causal ? wr0 / a.group + 1 : 0) : 0;          // keys all of them see
 
     Pages pg;
-    pg.row = a.table + sp.seq * a.table_stride; pg.n_pages = a.n_pages; pg.bad = false; pg.base = 0; pg.ids = 0;
-    const int64_t kp = a.kc[0] * (int)sizeof(elem_t), ks = a.kc[2] * (int)sizeof(elem_t);
-    const int64_t vp = a.vc[0] * (int)sizeof(elem_t), vs = a.vc[2] * (int)sizeof(elem_t);
-    const char* kbase = reinterpret_cast<const char*>(a.k) + kvh * a.kc[1] * (int)sizeof(elem_t);
-    const char* vbase = reinterpret_cast<const char*>(a.v) + kvh * a.vc[1] * (int)sizeof(elem_t);
+    pg.row = a.table + it.seq * a.table_stride; pg.n_pages = a.n_pages; pg.bad = false; pg.base = 0; pg.ids = 0;
+    const Rows<P, D> krows(a.k, a.kc, kvh), vrows(a.v, a.vc, kvh);
+    const unsigned lds = lds_address(smem);
     auto fetch = [&](int key0, int buf) {
-        const int last = (k1 - 1) >> a.page_shift;
-        if (((min(key0 + KT, k1) - 1) >> a.page_shift) >= pg.base + 64) pg.load(key0 >> a.page_shift, last);
-        char* lds = smem + buf * 2 * C::TILE;
-        dma_rows<P, D, KT / C::NW>(kbase, kp, ks, pg, a.page_shift, key0, w * (KT / C::NW), k1, lds);
-        dma_rows<P, D, KT / C::NW>(vbase, vp, vs, pg, a.page_shift, key0, w * (KT / C::NW), k1, lds + C::TILE);
+        if (((min(key0 + KT, k1) - 1) >> a.page_shift) >= pg.base + 64) pg.load(key0 >> a.page_shift, (k1 - 1) >> a.page_shift);
+        const unsigned to = lds + buf * 2 * C::TILE;
+        krows.template fetch<KT / C::NW>(pg, a.page_shift, key0, w * (KT / C::NW), k1, to);
+        vrows.template fetch<KT / C::NW>(pg, a.page_shift, key0, w * (KT / C::NW), k1, to + C::TILE);
     };
+    // lane parts of the LDS addresses: row l31 of K (chunk 2 t + h at step t); for V the blocks of read_v (bf16) or row 4 h (f32)
+    const unsigned ka = l31 * RB + ((h ^ swizzle<RB, P::IS_BF16>(l31 & 15)) << 4);
+    const int i16 = lane & 15, vr = 4 * h + (i16 >> 2), vc = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
+    const unsigned va = vr * RB + ((vc ^ swizzle<RB, P::IS_BF16>(vr)) << 4) + (i16 & 1) * 8;
+    const unsigned vb = (vr + 8) * RB + ((vc ^ swizzle<RB, P::IS_BF16>(vr + 8)) << 4) + (i16 & 1) * 8;
 
     // B operand of S^T = K Q^T: 16-byte chunk 2 s + h of the lane's query row at step s (and of the lane's key row for A)
     u32x4 qf[NKS];
@@ -389,28 +764,43 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
         __builtin_amdgcn_s_barrier();        // the tile has landed, and every wave has left the buffer of the tile before it
         if (key0 + (C::NBUF - 1) * KT < k1) fetch(key0 + (C::NBUF - 1) * KT, buf == 0 ? C::NBUF - 1 : buf - 1);
         if (key0 >= w_end) continue;         // nothing here for this wave's rows (it keeps moving its share of the tiles)
-        const char* kt = smem + buf * 2 * C::TILE;
-        const char* vt = kt + C::TILE;
-
+        const unsigned kt = lds + buf * 2 * C::TILE, vt = kt + C::TILE;
+        // reads of a key block are sent ahead of the products of the block in front (left to itself, hipcc reads, waits and multiplies in turn)
         f32x16 s[NKB];
+        u32x4 kf[2][NKS];
+#pragma unroll
+        for (int t = 0; t < NKS; ++t) kf[0][t] = read_lds(kt + (ka ^ (t << 5)));
 #pragma unroll
         for (int b = 0; b < NKB; ++b) {
+            if (b + 1 < NKB) {
+#pragma unroll
+                for (int t = 0; t < NKS; ++t) kf[(b + 1) & 1][t] = read_lds(kt + (b + 1) * 32 * RB + (ka ^ (t << 5)));
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
-            const int kr = b * 32 + l31;
 #pragma unroll
             for (int t = 0; t < NKS; ++t) {
-                const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + kr * RB + (((2 * t + h) ^ (kr & 7)) << 4));
                 if constexpr (P::IS_BF16) {
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[t]), s[b], 0, 0, 0);
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf[b & 1][t]), __builtin_bit_cast(bf16x8, qf[t]), s[b], 0, 0, 0);
                 } else {
-                    const f32x4 kx = __builtin_bit_cast(f32x4, kf), qx = __builtin_bit_cast(f32x4, qf[t]);
+                    const f32x4 kx = __builtin_bit_cast(f32x4, kf[b & 1][t]), qx = __builtin_bit_cast(f32x4, qf[t]);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(kx[j], qx[j], s[b], 0, 0, 0);
                 }
             }
         }
-        const uint64_t alive = tile_mask(a, sp.seq, key0);
+        // V of the first steps travels while the softmax runs
+        constexpr int VSTEPS = KT / 16, VAHEAD = NDB == 2 ? VSTEPS : VSTEPS / 2;
+        bf16x8 vf[P::IS_BF16 ? VSTEPS : 1][NDB];
+        if constexpr (P::IS_BF16) {
+#pragma unroll
+            for (int kk = 0; kk < VAHEAD; ++kk)
+#pragma unroll
+                for (int d = 0; d < NDB; ++d) vf[kk][d] = read_v(vt + 16 * kk * RB + (va ^ (d << 6)), vt + 16 * kk * RB + (vb ^ (d << 6)));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const uint64_t alive = tile_mask(a, it.seq, key0);
         if (key0 + KT > w_all || alive != ~0ull) {             // some key of the tile is not for some query
             const int left = lim - key0;
             const uint64_t see = (left >= 64 ? ~0ull : (left <= 0 ? 0ull : (1ull << left) - 1)) & alive;
@@ -447,46 +837,37 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
                 l += s[b][r];
             }
         if constexpr (P::IS_BF16) {
-#if defined(__HIP_DEVICE_COMPILE__)
-            // key 16 kk + 4 h + 0 .. 3 in slots 0 .. 3, 8 further on in slots 4 .. 7; the chunk swizzle of a row depends on 4 h + i16 / 4 only
-            // and moves feature block d by 64 bytes for odd d, two blocks by 128
-            const int i16 = lane & 15, vrow = 4 * h + (i16 >> 2), c0 = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
-            const unsigned va = lds_address(vt) + vrow * RB + ((c0 ^ (vrow & 7)) << 4) + (i16 & 1) * 8, vb = va ^ 64;
-            unrolled<0, KT / 16>([&](auto KK) {
-                constexpr int kk = decltype(KK)::value;
-                if constexpr (NDB == 2 && (kk & 1)) return;           // done with the step in front
-                s16x8 vf[4];
-                if constexpr (NDB == 2) read_v2<16 * kk * RB, (16 * kk + 8) * RB, (16 * kk + 16) * RB, (16 * kk + 24) * RB>(va, vb, vf);
-                else read_v4<16 * kk * RB, (16 * kk + 8) * RB>(va, vb, va + 128, vb + 128, vf);
+            // key 16 kk + 4 h + 0 .. 3 in slots 0 .. 3, 8 further on in slots 4 .. 7
 #pragma unroll
-                for (int u = 0; u < 4 / NDB; ++u) {
-                    bf16x8 pf;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) pf[j] = (__bf16)s[(kk + u) >> 1][8 * ((kk + u) & 1) + j];
+            for (int kk = 0; kk < KT / 16; ++kk) {
+                if (kk + VAHEAD < VSTEPS) {
 #pragma unroll
                     for (int d = 0; d < NDB; ++d)
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf[u * NDB + d]), pf, o[d], 0, 0, 0);
+                        vf[kk + VAHEAD][d] = read_v(vt + 16 * (kk + VAHEAD) * RB + (va ^ (d << 6)), vt + 16 * (kk + VAHEAD) * RB + (vb ^ (d << 6)));
                 }
-            });
-#endif
+                bf16x8 pf;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) pf[j] = (__bf16)s[kk >> 1][8 * (kk & 1) + j];
+#pragma unroll
+                for (int d = 0; d < NDB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[kk][d], pf, o[d], 0, 0, 0);
+            }
         } else {
 #pragma unroll
             for (int b = 0; b < NKB; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int vr = b * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
+                    const int row = b * 32 + 8 * (r >> 2) + (r & 3);               // and 4 h
+                    const unsigned at = vt + (row + 4 * h) * RB + (l31 & 3) * 4;
+                    const unsigned sw = swizzle<RB, P::IS_BF16>((row + 4 * h) & 15);
 #pragma unroll
-                    for (int d = 0; d < NDB; ++d) {
-                        const int f = d * 32 + l31;
-                        const float vx = *reinterpret_cast<const float*>(vt + vr * RB + (((f >> 2) ^ (vr & 7)) << 4) + (f & 3) * 4);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vx, s[b][r], o[d], 0, 0, 0);
-                    }
+                    for (int d = 0; d < NDB; ++d)
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(read_lds_f32(at + (((d * 8 + (l31 >> 2)) ^ sw) << 4)), s[b][r], o[d], 0, 0, 0);
                 }
         }
     }
     wait_vm<0>();
-    if (pg.bad && threadIdx.x == 0) atomicOr(a.status, PAGED_BAD_PAGE);
-    const bool bad = pg.bad || sp.bad;
+    if ((pg.bad || it.bad) && threadIdx.x == 0) atomicOr(a.status, (pg.bad ? PAGED_BAD_PAGE : 0) | (it.bad ? PAGED_BAD_LENGTH : 0));
+    const bool bad = pg.bad || it.bad;
     l += __shfl_xor(l, 32);
     float inv = l == 0.f ? 0.f : 1.f / l;
     if (bad) { l = NAN; inv = NAN; }
@@ -508,19 +889,17 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 const int f = d * 32 + 2 * r + 4 * h;
-                if (a.splits > 1) store4<PF32>(part_out<D>(a, split, orow) + f, o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
+                if (it.splits > 1) store4<PF32>(part_out<D>(a, it.split, orow) + f, o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
                 else store4<P>(reinterpret_cast<elem_t*>(a.out) + token * a.os[0] + head * a.os[1] + f, o[d][r] * inv, o[d][r + 1] * inv,
                                o[d][r + 2] * inv, o[d][r + 3] * inv);
             }
-        if (a.splits > 1 && h == 0) { float* ml = part_ml<D>(a, split, orow); ml[0] = m; ml[1] = l; }
+        if (it.splits > 1 && h == 0) { float* ml = part_ml<D>(a, it.split, orow); ml[0] = m; ml[1] = l; }
     }
     uint32_t again = (uint32_t)odds | (uint32_t)(odds >> 32);
     while (again) {
         const int i = __builtin_ctz(again);
         again &= again - 1;
-        const int rr = wr0 + i, tk = rr / a.group;
-        store_row_alone<P, D>(a, sp.seq, kvh, sp.first + tk, kvh * a.group + rr - tk * a.group, split, k0,
-                              min(k1, sp.past + (a.causal ? tk + 1 : 0)));
+        store_row_alone<P, D>(a, it, kvh, wr0 + i);
     }
 }
 
@@ -546,36 +925,36 @@ __global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kern
     __shared__ __attribute__((aligned(1024))) char smem[NW * 2 * C::STAGE];
     const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
 
-    if (blockIdx.x == 0 && a.starts) check_starts(a.starts, a.n_seqs, a.tokens, a.status);
-    const int kvh = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, split = rest % a.splits;
-    Span sp;
-    int tile;
-    if (!find_tile(a, rest / a.splits, C::M, &sp, &tile)) return;
-    const int rows = sp.n * a.group, r0 = tile * C::M, r_end = min(r0 + C::M, rows);
+    Schedule<C::M, KT> sched;
+    begin(a, sched, STEP_LAG);
+    const int item = blockIdx.x;
+    if (item >= sched.items * a.kv_heads) return;
+    const int kvh = item % a.kv_heads;
+    Item it;
+    sched.find(a, item / a.kv_heads, &it);
+    if (it.split >= it.splits) return;
+    const int k0 = it.k0, k1 = it.k1, r0 = it.tile * C::M, r_end = min(r0 + C::M, it.n * a.group);
     const int row = r0 + l15;
     const bool live = row < r_end;
     const int tok = live ? row / a.group : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
-    const int64_t token = sp.first + tok;
-    const int lim = live && !sp.bad ? sp.past + (a.causal ? tok + 1 : 0) : 0;
-    const int tile_end = sp.bad ? 0 : sp.past + (a.causal ? (r_end - 1) / a.group + 1 : 0);
-    const int all = r_end - r0 == C::M && !sp.bad ? sp.past + (a.causal ? r0 / a.group + 1 : 0) : 0;      // keys every column sees
-    int k0, k1;
-    split_range(a, split, tile_end, KT, &k0, &k1);
+    const int64_t token = it.first + tok;
+    const int lim = live && !it.bad ? it.past + (a.causal ? tok + 1 : 0) : 0;
+    const int all = r_end - r0 == C::M && !it.bad ? it.past + (a.causal ? r0 / a.group + 1 : 0) : 0;      // keys every column sees
 
     Pages pg;
-    pg.row = a.table + sp.seq * a.table_stride; pg.n_pages = a.n_pages; pg.bad = false; pg.base = 0; pg.ids = 0;
-    const int64_t kp = a.kc[0] * (int)sizeof(elem_t), ks = a.kc[2] * (int)sizeof(elem_t);
-    const int64_t vp = a.vc[0] * (int)sizeof(elem_t), vs = a.vc[2] * (int)sizeof(elem_t);
-    const char* kbase = reinterpret_cast<const char*>(a.k) + kvh * a.kc[1] * (int)sizeof(elem_t);
-    const char* vbase = reinterpret_cast<const char*>(a.v) + kvh * a.vc[1] * (int)sizeof(elem_t);
-    char* ring = smem + w * 2 * C::STAGE;
+    pg.row = a.table + it.seq * a.table_stride; pg.n_pages = a.n_pages; pg.bad = false; pg.base = 0; pg.ids = 0;
+    const Rows<P, D> krows(a.k, a.kc, kvh), vrows(a.v, a.vc, kvh);
+    const unsigned ring = lds_address(smem) + w * 2 * C::STAGE;
     const int first = k0 + w * KT;
     auto fetch = [&](int key0, int buf) {
         if (((min(key0 + KT, k1) - 1) >> a.page_shift) >= pg.base + 64) pg.load(key0 >> a.page_shift, (k1 - 1) >> a.page_shift);
-        char* lds = ring + buf * C::STAGE;
-        dma_rows<P, D, KT>(kbase, kp, ks, pg, a.page_shift, key0, 0, k1, lds);
-        dma_rows<P, D, KT>(vbase, vp, vs, pg, a.page_shift, key0, 0, k1, lds + C::TILE);
+        const unsigned to = ring + buf * C::STAGE;
+        krows.template fetch<KT>(pg, a.page_shift, key0, 0, k1, to);
+        vrows.template fetch<KT>(pg, a.page_shift, key0, 0, k1, to + C::TILE);
     };
+    const unsigned ka = l15 * RB + ((g ^ swizzle<RB, P::IS_BF16>(l15)) << 4);
+    const int vr = 4 * g + (l15 >> 2), vc = (l15 >> 1) & 1;
+    const unsigned va = vr * RB + ((vc ^ swizzle<RB, P::IS_BF16>(vr)) << 4) + (l15 & 1) * 8;       // and 16 rows further on
 
     u32x4 qf[NKS];
     {
@@ -597,16 +976,14 @@ __global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kern
         wait_lds();                          // the other buffer's reads are over
         if (key0 + NW * KT < k1) { fetch(key0 + NW * KT, buf ^ 1); wait_vm<C::DMA>(); }
         else wait_vm<0>();
-        const char* kt = ring + buf * C::STAGE;
-        const char* vt = kt + C::TILE;
+        const unsigned kt = ring + buf * C::STAGE, vt = kt + C::TILE;
         f32x4 s[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             s[b] = {0, 0, 0, 0};
-            const int kr = b * 16 + l15;
 #pragma unroll
             for (int t = 0; t < NKS; ++t) {
-                const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + kr * RB + (((4 * t + g) ^ (kr & 7)) << 4));
+                const u32x4 kf = read_lds(kt + b * 16 * RB + (ka ^ (t << 6)));
                 if constexpr (P::IS_BF16) {
                     s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[t]), s[b], 0, 0, 0);
                 } else {
@@ -616,7 +993,7 @@ __global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kern
                 }
             }
         }
-        const uint64_t alive = tile_mask(a, sp.seq, key0);
+        const uint64_t alive = tile_mask(a, it.seq, key0);
         if (key0 + KT > all || (uint32_t)alive != ~0u) {
             const int left = lim - key0;
             const uint32_t see = (left >= 32 ? ~0u : (left <= 0 ? 0u : (1u << left) - 1)) & (uint32_t)alive;
@@ -645,42 +1022,31 @@ __global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kern
                 l += s[b][r];
             }
         if constexpr (P::IS_BF16) {
-#if defined(__HIP_DEVICE_COMPILE__)
             // slots 0 .. 3 of group g: keys 4 g .. of the lower 16, slots 4 .. 7: of the upper 16
             bf16x8 pf;
 #pragma unroll
             for (int j = 0; j < 8; ++j) pf[j] = (__bf16)s[j >> 2][j & 3];
-            const int vrow = 4 * g + (l15 >> 2);
-            const unsigned va = lds_address(vt) + vrow * RB + ((((l15 >> 1) & 1) ^ (vrow & 7)) << 4) + (l15 & 1) * 8;
-            unrolled<0, NDB / 4>([&](auto Q) {
-                constexpr int q4 = decltype(Q)::value;               // feature blocks 4 q4 .. (32 bytes each, swizzled within 128)
-                s16x8 vf[4];
-                read_v4<q4 * 128, q4 * 128 + 16 * RB>(va, va ^ 32, va ^ 64, va ^ 96, vf);
 #pragma unroll
-                for (int d = 0; d < 4; ++d)
-                    o[4 * q4 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf[d]), pf, o[4 * q4 + d], 0, 0, 0);
-            });
-#endif
+            for (int d = 0; d < NDB; ++d)
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(read_v(vt + (va ^ (d << 5)), vt + 16 * RB + (va ^ (d << 5))), pf, o[d], 0, 0, 0);
         } else {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int vr = 16 * b + 4 * g + r;
+                    const int row = 16 * b + 4 * g + r;
+                    const unsigned at = vt + row * RB + (l15 & 3) * 4, sw = swizzle<RB, P::IS_BF16>(row & 15);
 #pragma unroll
-                    for (int d = 0; d < NDB; ++d) {
-                        const int f = d * 16 + l15;
-                        const float vx = *reinterpret_cast<const float*>(vt + vr * RB + (((f >> 2) ^ (vr & 7)) << 4) + (f & 3) * 4);
-                        o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx, s[b][r], o[d], 0, 0, 0);
-                    }
+                    for (int d = 0; d < NDB; ++d)
+                        o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(read_lds_f32(at + (((d * 4 + (l15 >> 2)) ^ sw) << 4)), s[b][r], o[d], 0, 0, 0);
                 }
         }
     }
     wait_vm<0>();
-    if (pg.bad && lane == 0) atomicOr(a.status, PAGED_BAD_PAGE);
+    if ((pg.bad || it.bad) && lane == 0) atomicOr(a.status, (pg.bad ? PAGED_BAD_PAGE : 0) | (it.bad ? PAGED_BAD_LENGTH : 0));
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (pg.bad || sp.bad) l = NAN;
+    if (pg.bad || it.bad) l = NAN;
 
     // join the waves: outputs [NW][16][D] (16-byte pieces XOR-swizzled by the row) and maxima, sums [NW][16] in the place of the tiles
     __syncthreads();
@@ -707,15 +1073,15 @@ __global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kern
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[j] = fmaf(x[j], f[v], acc[j]);
         }
-        const bool ruined = sum != sum && (pg.bad || sp.bad);
+        const bool ruined = sum != sum && (pg.bad || it.bad);
         const float z = fmaf(acc[0], 0.f, fmaf(acc[1], 0.f, fmaf(acc[2], 0.f, fmaf(acc[3], 0.f, sum * 0.f))));
         const int tk = on ? rr / a.group : 0, hd = kvh * a.group + (on ? rr - tk * a.group : 0);
-        const int64_t t64 = sp.first + tk;
+        const int64_t t64 = it.first + tk;
         if (on) {
-            if (a.splits > 1) {
+            if (it.splits > 1) {
                 const int64_t orow = t64 * a.q_heads + hd;
-                *reinterpret_cast<f32x4*>(part_out<D>(a, split, orow) + piece * 4) = acc;
-                if (piece == 0) { float* ml = part_ml<D>(a, split, orow); ml[0] = top; ml[1] = sum; }
+                *reinterpret_cast<f32x4*>(part_out<D>(a, it.split, orow) + piece * 4) = acc;
+                if (piece == 0) { float* ml = part_ml<D>(a, it.split, orow); ml[0] = top; ml[1] = sum; }
             } else {
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
                 store4<P>(reinterpret_cast<elem_t*>(a.out) + t64 * a.os[0] + hd * a.os[1] + piece * 4, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
@@ -727,64 +1093,82 @@ __global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kern
             const int src = __builtin_ctzll(odds), rw = (i - lane + src) / PPR;
             const uint64_t same = PPR == 64 ? ~0ull : (((1ull << PPR) - 1) << (src / PPR * PPR));
             odds &= ~same;
-            const int ar = r0 + uniform(rw), at = ar / a.group;
-            store_row_alone<P, D>(a, sp.seq, kvh, sp.first + at, kvh * a.group + ar - at * a.group, split, k0,
-                                  min(k1, sp.past + (a.causal ? at + 1 : 0)));
+            store_row_alone<P, D>(a, it, kvh, r0 + uniform(rw));
         }
     }
 }
 
 // =================================================================================================================================
-// Joins the partial results of a split launch: W waves per (token, query head).  The (maximum, sum) pairs of all splits (at most 64) sit
-// one per lane; 16-byte pieces of the partial outputs are then read by 64 / (D / 4) splits at a time and wave.
+// Joins the partial results of cut tiles.  A workgroup takes RPB rows of a tile: 256 / (D / 4) of them, one 16-byte piece of a row per
+// thread, or (few rows, many shares) a single one, the shares dealt out over its threads.
 // =================================================================================================================================
-template <typename P, int D, int W>
+template <typename P, int D, int M, int KT, int RPB>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
     typedef typename P::elem_t elem_t;
-    constexpr int LPR = D / 4, SPW = 64 / LPR;          // lanes per row, splits per wave
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, piece = lane % LPR, sub = lane / LPR;
-    const int64_t row = (int64_t)blockIdx.x * (4 / W) + (W == 1 ? w : 0);
-    if (row >= (int64_t)a.tokens * a.q_heads) return;
-    const int64_t token = row / a.q_heads;
-    const int head = (int)(row - token * a.q_heads);
-    if (a.starts) {          // rows of no sequence (padding, bad starts) have no partial results
-        int lo = 0, hi = a.n_seqs;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.starts[mid] <= token) lo = mid; else hi = mid;
-        }
-        if (a.starts[lo] < 0 || a.starts[lo + 1] > a.tokens || token < a.starts[lo] || token >= a.starts[lo + 1]) return;
-    }
-    float m = -INFINITY, l = 0.f;
-    if (lane < a.splits) { const float2 ml = *reinterpret_cast<const float2*>(part_ml<D>(a, lane, row)); m = ml.x; l = ml.y; }
-    const float top = wave_max(m), f = l == 0.f ? 0.f : exp2_hw(m - (top == -INFINITY ? 0.f : top));
-    const float sum = wave_sum(l * f);
+    constexpr int LPR = D / 4, SP = 256 / (RPB * LPR), PARTS = M / RPB;
+    static_assert(SP * RPB * LPR == 256, "one piece per thread");
+    __shared__ float weight[RPB == 1 ? MAX_SPLITS : 1], red[8];
+    __shared__ f32x4 pieces[RPB == 1 ? 256 : 1];
+    const int share = __builtin_bit_cast(int, a.part[0]);
+    Schedule<M, KT> sched;
+    sched.share = 0x3fffffff;
+    sched.load(a, 0);
+    sched.count(a);
+    const int t = blockIdx.x / PARTS;
+    if (t >= sched.items * a.kv_heads) return;
+    const int kvh = t % a.kv_heads;
+    Item it;
+    sched.find(a, t / a.kv_heads, &it);
+    const int kt = (it.end + KT - 1) / KT, splits = min(kt <= share ? 1 : (kt + share - 1) / share, a.splits);
+    if (splits == 1) return;                 // written already
+    const int tid = threadIdx.x, piece = tid % LPR, sub = tid / LPR % SP;
+    const int row = it.tile * M + (blockIdx.x % PARTS) * RPB + (RPB == 1 ? 0 : tid / LPR);
+    const bool live = row < it.n * a.group;
+    if (RPB == 1 && !live) return;
+    const int tok = live ? row / a.group : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
+    const int64_t token = it.first + tok, orow = token * a.q_heads + head;
     f32x4 acc = {0, 0, 0, 0};
-    for (int s0 = W == 1 ? 0 : w * SPW; s0 < a.splits; s0 += W * SPW) {
-        const int s = s0 + sub;
-        const float fs = __shfl(f, s & 63);
-        if (s < a.splits && fs != 0.f) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(part_out<D>(a, s, row) + piece * 4);
+    float sum = 0.f;
+    if constexpr (RPB > 1) {
+        float top = -INFINITY;
+        for (int s = 0; s < splits; ++s) top = fmaxf(top, part_ml<D>(a, s, orow)[0]);
+        const float mu = top == -INFINITY ? 0.f : top;
+        for (int s = 0; s < splits; ++s) {
+            const float* ml = part_ml<D>(a, s, orow);
+            const float f = ml[1] == 0.f ? 0.f : exp2_hw(ml[0] - mu);
+            sum = fmaf(ml[1], f, sum);
+            const f32x4 x = *reinterpret_cast<const f32x4*>(part_out<D>(a, s, orow) + piece * 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = fmaf(x[i], fs, acc[i]);
+            for (int i = 0; i < 4; ++i) acc[i] = f == 0.f ? acc[i] : fmaf(x[i], f, acc[i]);
         }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (SPW >= 4) acc[i] += __shfl_xor(acc[i], 16);
-        acc[i] += __shfl_xor(acc[i], 32);
-    }
-    if constexpr (W > 1) {
-        __shared__ f32x4 other[W][LPR];
-        if (sub == 0) other[w][piece] = acc;
+    } else {
+        float m = -INFINITY, l = 0.f;
+        if (tid < splits) { const float* ml = part_ml<D>(a, tid, orow); m = ml[0]; l = ml[1]; }
+        float top = wave_max(m);
+        if ((tid & 63) == 0) red[tid >> 6] = top;
         __syncthreads();
-        if (w != 0) return;
+        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        const float f = l == 0.f ? 0.f : exp2_hw(m - (top == -INFINITY ? 0.f : top));
+        weight[tid] = f;
+        const float part = wave_sum(l * f);
+        if ((tid & 63) == 0) red[4 + (tid >> 6)] = part;
+        __syncthreads();
+        sum = (red[4] + red[5]) + (red[6] + red[7]);
+#pragma unroll 4
+        for (int s = sub; s < splits; s += SP) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(part_out<D>(a, s, orow) + piece * 4);
+            const float fs = weight[s];
 #pragma unroll
-        for (int i = 1; i < W; ++i)
+            for (int i = 0; i < 4; ++i) acc[i] = fs == 0.f ? acc[i] : fmaf(x[i], fs, acc[i]);
+        }
+        pieces[tid] = acc;
+        __syncthreads();
+        if (sub != 0) return;
+        for (int s = 1; s < SP; ++s)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] += other[i][piece][j];
+            for (int i = 0; i < 4; ++i) acc[i] += pieces[s * LPR + piece][i];
     }
-    if (sub == 0) {
+    if (live) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         store4<P>(reinterpret_cast<elem_t*>(a.out) + token * a.os[0] + head * a.os[1] + piece * 4, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
     }
@@ -793,9 +1177,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
 struct Plan { bool step; int tiles, splits; };
 
 // max_new tokens a sequence at most (0: not known) make at most max_new * group rows per key head: up to 16 take the step kernel.
-// Workgroups are few where rows are few: the keys are then shared out over `splits` workgroups.  Two workgroups fit a CU; a share has
-// at least 256 keys (its partial result costs a row of f32 outputs twice).
-Plan make_plan(const PagedAttnArgs& a, int max_new) {
+Plan make_plan(const PagedAttnArgs& a, int max_new, int head_dim) {
     Plan p;
     const int64_t most = (a.starts ? max_new : 1) * (int64_t)a.group;       // 0: not known
     p.step = most > 0 && most <= 16;
@@ -804,34 +1186,42 @@ Plan make_plan(const PagedAttnArgs& a, int max_new) {
     p.tiles = (int)ub;
     int64_t est = most > 0 ? (int64_t)a.n_seqs * ((most + M - 1) / M) : ub;
     if (est > ub) est = ub;
-    const int64_t groups = est * a.kv_heads, keys = (int64_t)a.max_pages << a.page_shift;
-    int64_t s = 512 / (groups > 0 ? groups : 1);
-    if (s > keys / 256) s = keys / 256;
-    if (s > 64) s = 64;
-    p.splits = s < 1 ? 1 : (int)s;
+    // most shares of a tile: none where the keys a workgroup could be left with alone take less time than joining; 128 MiB of partial results
+    const int64_t keys = (int64_t)a.max_pages << a.page_shift, row_bytes = (int64_t)a.tokens * a.q_heads * (head_dim + 2) * 4;
+    const bool full = est * a.kv_heads >= SLOTS;
+    int64_t s = keys / MIN_SHARE;
+    if (keys <= (p.step ? (full ? 4096 : 1024) : (full ? 1024 : 512))) s = 1;
+    if (s > MAX_SPLITS) s = MAX_SPLITS;
+    if (s > ((int64_t)128 << 20) / row_bytes) s = ((int64_t)128 << 20) / row_bytes;
+    p.splits = s < 2 ? 1 : (int)s;
     return p;
 }
 
 template <typename P, int D>
 hipError_t launch(PagedAttnArgs a, int max_new, hipStream_t s) {
-    const Plan p = make_plan(a, max_new);
+    const Plan p = make_plan(a, max_new, D);
     a.splits = p.splits;
-    const int64_t rows = (int64_t)a.tokens * a.q_heads, groups = (int64_t)p.tiles * p.splits * a.kv_heads;
-    if (groups > 0x7fffffff || rows > 0x7fffffff) return hipErrorInvalidValue;
-    if (p.step) hipLaunchKernelGGL((paged_attn_step_kernel<P, D>), dim3((unsigned)groups), dim3(StepCfg<P, D>::NW * 64), 0, s, a);
-    else hipLaunchKernelGGL((paged_attn_tile_kernel<P, D>), dim3((unsigned)groups), dim3(256), 0, s, a);
+    // cutting adds at most 2 SLOTS items: a share is no less than a slot's part of a work that counts at least half of every tile's keys
+    // (64 more for the roundings of that sum)
+    const int64_t groups = (int64_t)p.tiles * a.kv_heads;
+    const int64_t cut = groups * p.splits < groups + 2 * SLOTS + 64 ? groups * p.splits : groups + 2 * SLOTS + 64;
+    if (cut > 0x7fffffff / 16) return hipErrorInvalidValue;
+    if (p.step) hipLaunchKernelGGL((paged_attn_step_kernel<P, D>), dim3((unsigned)cut), dim3(StepCfg<P, D>::NW * 64), 0, s, a);
+    else if constexpr (P::IS_BF16) hipLaunchKernelGGL(paged_attn_chunk_kernel<D>, dim3((unsigned)cut), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((paged_attn_tile_kernel<P, D>), dim3((unsigned)cut), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    if (p.splits > 8) hipLaunchKernelGGL((paged_attn_join_kernel<P, D, 4>), dim3((unsigned)rows), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((paged_attn_join_kernel<P, D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+    constexpr int RPB = 1024 / D;
+    if (p.step) hipLaunchKernelGGL((paged_attn_join_kernel<P, D, 16, 32, 1>), dim3((unsigned)groups * 16), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((paged_attn_join_kernel<P, D, 128, TileCfg<P, D>::KT, RPB>), dim3((unsigned)groups * (128 / RPB)), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t paged_attn_workspace(const PagedAttnArgs& a, int max_new, int head_dim, int) {
-    const Plan p = make_plan(a, max_new);
-    return p.splits == 1 ? 0 : (int64_t)p.splits * a.tokens * a.q_heads * (head_dim + 2) * (int64_t)sizeof(float);
+    const Plan p = make_plan(a, max_new, head_dim);
+    return p.splits == 1 ? 0 : (PART_HEAD + (int64_t)p.splits * a.tokens * a.q_heads * (head_dim + 2)) * (int64_t)sizeof(float);
 }
 
 hipError_t paged_attn_launch(const PagedAttnArgs& a, int max_new, int head_dim, int dtype, hipStream_t s) {
