@@ -51,6 +51,18 @@ struct AppendArgs {
     int q_heads, kv_heads, head_dim;         // q_heads 0: no q
 };
 
+// x / d for 0 <= x < 2^31: the high half of 2 x times m = ceil(2^(31 + s) / d), s = ceil(log2 d), shifted by s
+struct IntDiv { uint32_t m, s; };
+inline IntDiv make_int_div(uint32_t d) {
+    IntDiv r = {0, 0};
+    while (((uint64_t)1 << r.s) < d) ++r.s;
+    r.m = (uint32_t)((((uint64_t)1 << (31 + r.s)) + d - 1) / d);
+    return r;
+}
+#if defined(__HIPCC__)
+__device__ __forceinline__ int int_div(int x, IntDiv d) { return (int)(__umulhi(2u * (uint32_t)x, d.m) >> d.s); }
+#endif
+
 struct PagedAttnArgs {
     const void *q, *k, *v;
     void* out;
@@ -65,6 +77,7 @@ struct PagedAttnArgs {
     float scale_log2;        // softmax scale * log2(e)
     int max_pages, n_pages, page_shift, n_seqs, tokens, mask_width, causal;
     int q_heads, kv_heads, group, splits;
+    IntDiv by_group, by_kv_heads;
 };
 
 hipError_t rotary_embed_launch(const RotaryEmbedArgs& a, int dtype, hipStream_t s);

@@ -110,6 +110,23 @@ template <int RB, bool BF16> __device__ __forceinline__ unsigned swizzle(unsigne
     if (RB == 128) return ((r >> 1 & 1) << 2) | ((r >> 2 & 1) << 1) | (r >> 3 & 1);
     return BF16 ? ((r & 3) << 2) | ((r >> 2 & 1) << 1) | (r >> 3 & 1) : r & 15;
 }
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int x) {      // x plus the moved x, where there is one
+    return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ unsigned wave_max_u32(unsigned x) {
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, true));
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, true));
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, true));
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, true));
+    const unsigned a = max((unsigned)__builtin_amdgcn_readlane((int)x, 0), (unsigned)__builtin_amdgcn_readlane((int)x, 16));
+    const unsigned b = max((unsigned)__builtin_amdgcn_readlane((int)x, 32), (unsigned)__builtin_amdgcn_readlane((int)x, 48));
+    return max(a, b);
+}
+__device__ __forceinline__ int scan_add(int x) {        // sum over the lanes up to this one
+    x = dpp_add<0x111, 0xf>(x); x = dpp_add<0x112, 0xf>(x); x = dpp_add<0x114, 0xf>(x); x = dpp_add<0x118, 0xf>(x);
+    x = dpp_add<0x142, 0xa>(x);                         // lane 15 of a row of 16 into the next row
+    return dpp_add<0x143, 0xc>(x);                      // lane 31 into the upper half
+}
 template <int I, int N, typename F> __device__ __forceinline__ void each(F&& f) {      // f(0), f(1), ... with the number as a type
     if constexpr (I < N) { f(std::integral_constant<int, I>()); each<I + 1, N>(f); }
 }
@@ -132,15 +149,18 @@ struct Item {
     bool bad;                   // the length leads behind the row of the page table: every row becomes NaN
 };
 
-template <int M, int KT> struct Schedule {
-    int first, n, past;         // this lane's sequence of the current 64
-    int base;                   // its number - lane
+// SORTED: of every 64 sequences the longest first, so that what starts last is short.
+template <int M, int KT, bool SORTED> struct Schedule {
+    int seq, first, n, past;    // this lane's sequence of the current 64
+    int base;                   // number of the first of these
+    int sum, own;               // (tile, share) pairs of the lane's sequence, and of all up to it
     int share;                  // tiles of KT keys of a share (of all keys: not cut)
-    int items;                  // (tile, share) pairs of the batch
+    int items;                  // pairs of the batch
 
     __device__ __forceinline__ void load(const PagedAttnArgs& a, int i0) {
         const int lane = threadIdx.x & 63, i = min(i0 + lane, a.n_seqs - 1);
         base = i0;
+        seq = i;
         if (a.starts) {
             first = a.starts[i];
             const int end = a.starts[i + 1];
@@ -149,16 +169,32 @@ template <int M, int KT> struct Schedule {
         past = a.past[i];
         if (i0 + lane >= a.n_seqs) n = 0;
     }
-    __device__ __forceinline__ bool bad_length(const PagedAttnArgs& a, int np, int pp) const {
+    static __device__ __forceinline__ bool bad_length(const PagedAttnArgs& a, int np, int pp) {
         return pp < 0 || (int64_t)pp + (a.causal ? np : 0) > ((int64_t)a.max_pages << a.page_shift);
     }
     __device__ __forceinline__ int row_tiles(const PagedAttnArgs& a) const { return (n * a.group + M - 1) / M; }
     __device__ __forceinline__ int key_tiles(const PagedAttnArgs& a) const {
         return bad_length(a, n, past) ? 1 : (past + (a.causal ? n : 0) + KT - 1) / KT;
     }
-    __device__ __forceinline__ int own(const PagedAttnArgs& a) const {
-        const int kt = key_tiles(a);
-        return row_tiles(a) * (kt <= share ? 1 : (kt + share - 1) / share);
+    __device__ __forceinline__ int shares(int kt) const { return kt <= share ? 1 : (kt + share - 1) / share; }
+    __device__ __forceinline__ void count(const PagedAttnArgs& a) {
+        own = row_tiles(a);
+        if (a.splits > 1) own *= shares(key_tiles(a));
+        sum = scan_add(own);
+    }
+    __device__ __forceinline__ void sort(const PagedAttnArgs& a) {
+        const int lane = threadIdx.x & 63, here = min(a.n_seqs - base, 64), key = n > 0 ? key_tiles(a) : 0;
+        if (here <= 1) return;
+        int rank = 0;
+        for (int j = 0; j < here; ++j) {
+            const int other = __builtin_amdgcn_readlane(key, j);
+            rank += other > key || (other == key && j < lane) ? 1 : 0;
+        }
+        if (lane >= here) rank = lane;
+        seq = __builtin_amdgcn_ds_permute(rank << 2, seq);
+        first = __builtin_amdgcn_ds_permute(rank << 2, first);
+        n = __builtin_amdgcn_ds_permute(rank << 2, n);
+        past = __builtin_amdgcn_ds_permute(rank << 2, past);
     }
     // share for the whole batch, the number of items
     __device__ __forceinline__ void plan(const PagedAttnArgs& a, float lag) {
@@ -176,60 +212,59 @@ template <int M, int KT> struct Schedule {
                 load(a, i0);
             }
             const float mean = wave_sum(work) * (float)a.kv_heads / SLOTS;
-#pragma unroll
-            for (int d = 32; d > 0; d >>= 1) most = max(most, __shfl_xor(most, d));
+            most = (int)wave_max_u32((unsigned)most);
             if ((float)most > lag * mean) share = max(max((int)ceilf(mean), MIN_SHARE / KT), (most + a.splits - 1) / a.splits);
+            share = uniform(share);
             if (a.n_seqs > 64) load(a, 0);
         }
-        share = uniform(share);
-        count(a);
+        number(a);
     }
-    __device__ __forceinline__ void count(const PagedAttnArgs& a) {
-        int sum = 0;
+    __device__ __forceinline__ void number(const PagedAttnArgs& a) {
+        items = 0;
         for (int i0 = 0;;) {
-            sum += own(a);
+            if (SORTED) sort(a);
+            count(a);
+            items += __builtin_amdgcn_readlane(sum, 63);
             i0 += 64;
             if (i0 >= a.n_seqs) break;
             load(a, i0);
         }
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-        items = uniform(sum);
     }
     // item t < items
     __device__ __forceinline__ void find(const PagedAttnArgs& a, int t, Item* it) {
-        const int lane = threadIdx.x & 63;
-        int sel, sum, ours;
-        if (base != 0) load(a, 0);
-        for (;;) {
-            ours = own(a);
-            sum = ours;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) { const int x = __shfl_up(sum, d); sum += lane >= d ? x : 0; }
-            sel = __popcll(__ballot(sum <= t));
-            if (sel < 64 || base + 64 >= a.n_seqs) break;
-            t -= __builtin_amdgcn_readlane(sum, 63);
-            load(a, base + 64);
+        if (a.n_seqs > 64) {
+            load(a, 0);
+            for (;;) {
+                if (SORTED) sort(a);
+                count(a);
+                const int here = __builtin_amdgcn_readlane(sum, 63);
+                if (t < here || base + 64 >= a.n_seqs) break;
+                t -= here;
+                load(a, base + 64);
+            }
         }
-        sel = uniform(min(sel, 63));
-        it->seq = base + sel;
+        const int sel = uniform(min((int)__popcll(__ballot(sum <= t)), 63));
+        it->seq = __builtin_amdgcn_readlane(seq, sel);
         it->first = __builtin_amdgcn_readlane(first, sel);
         it->n = __builtin_amdgcn_readlane(n, sel);
         it->past = __builtin_amdgcn_readlane(past, sel);
-        t -= __builtin_amdgcn_readlane(sum - ours, sel);
-        const int tiles = (it->n * a.group + M - 1) / M, cuts = __builtin_amdgcn_readlane(ours, sel) / max(tiles, 1);
-        it->tile = cuts > 1 ? t / cuts : t;
-        it->split = t - it->tile * cuts;
-        it->tile = tiles - 1 - it->tile;               // the rows that see most first
+        t -= __builtin_amdgcn_readlane(sum - own, sel);
+        const int tiles = (it->n * a.group + M - 1) / M;
         it->bad = bad_length(a, it->n, it->past);
         if (it->bad) it->past = 0;
+        it->split = 0;
+        if (a.splits > 1) {
+            const int cuts = it->bad ? 1 : shares((it->past + (a.causal ? it->n : 0) + KT - 1) / KT);
+            if (cuts > 1) { const int q = t / cuts; it->split = t - q * cuts; t = q; }
+        }
+        it->tile = tiles - 1 - t;                      // the rows that see most first
         it->end = it->bad ? 0 : it->past;
-        if (a.causal && !it->bad) it->end += (min((it->tile + 1) * M, it->n * a.group) - 1) / a.group + 1;
+        if (a.causal && !it->bad) it->end += int_div(min((it->tile + 1) * M, it->n * a.group) - 1, a.by_group) + 1;
         const int kt = (it->end + KT - 1) / KT;
-        it->splits = kt <= share ? 1 : (kt + share - 1) / share;
-        it->k0 = it->k1 = 0;
-        if (it->splits == 1) it->k1 = it->split == 0 ? it->end : 0;
-        else if (it->split < it->splits) { it->k0 = it->split * share * KT; it->k1 = min(it->k0 + share * KT, it->end); }
+        it->splits = a.splits > 1 ? shares(kt) : 1;
+        it->k0 = 0;
+        it->k1 = it->end;
+        if (it->splits > 1) { it->k0 = min(it->split * share * KT, it->end); it->k1 = min(it->k0 + share * KT, it->end); }
     }
 };
 
@@ -385,7 +420,7 @@ template <int D> __device__ __forceinline__ float* part_ml(const PagedAttnArgs& 
 template <typename P, int D>
 __device__ __forceinline__ void store_row_alone(const PagedAttnArgs& a, const Item& it, int kvh, int row) {
     typedef typename P::elem_t elem_t;
-    const int lane = threadIdx.x & 63, tok = row / a.group, head = kvh * a.group + row - tok * a.group;
+    const int lane = threadIdx.x & 63, tok = int_div(row, a.by_group), head = kvh * a.group + row - tok * a.group;
     const int64_t token = it.first + tok;
     float m, l, acc[D / 64];
     row_alone<P, D>(a, it.seq, kvh, reinterpret_cast<const elem_t*>(a.q) + token * a.qs[0] + head * a.qs[1], it.k0,
@@ -435,22 +470,22 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk_kernel(PagedAttnArgs 
     __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
     const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l31 = lane & 31, h = lane >> 5;
 
-    Schedule<C::M, KT> sched;
+    Schedule<C::M, KT, true> sched;
     begin(a, sched, TILE_LAG);
     const int item = blockIdx.x;
     if (item >= sched.items * a.kv_heads) return;
     // consecutive workgroups go to consecutive XCDs: with the key head innermost, an XCD's L2 holds few heads' pages
-    const int kvh = item % a.kv_heads;
+    const int at = int_div(item, a.by_kv_heads), kvh = item - at * a.kv_heads;
     Item it;
-    sched.find(a, item / a.kv_heads, &it);
+    sched.find(a, at, &it);
     if (it.split >= it.splits) return;
     const int k0 = it.k0, k1 = it.k1, r0 = it.tile * C::M, r_end = min(r0 + C::M, it.n * a.group);
     int row = r0 + w * 32 + l31;                               // this lane's query
     int lim;                                                   // keys 0 .. lim - 1 are seen
     const int wr0 = r0 + w * 32, wr1 = min(wr0 + 32, r_end);                            // rows of this wave: [wr0, wr1)
     const bool some = wr0 < wr1 && !it.bad;
-    const int w_end = some ? it.past + (a.causal ? (wr1 - 1) / a.group + 1 : 0) : 0;    // keys any of them sees
-    const int w_all = some ? it.past + (a.causal ? wr0 / a.group + 1 : 0) : 0;          // keys all of them see
+    const int w_end = some ? it.past + (a.causal ? int_div(wr1 - 1, a.by_group) + 1 : 0) : 0;    // keys any of them sees
+    const int w_all = some ? it.past + (a.causal ? int_div(wr0, a.by_group) + 1 : 0) : 0;          // keys all of them see
 
     Pages pg;
     pg.row = a.table + it.seq * a.table_stride; pg.n_pages = a.n_pages; pg.bad = false; pg.base = 0; pg.ids = 0;
@@ -472,7 +507,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk_kernel(PagedAttnArgs 
     bf16x8 qf[NKS];
     {
         const bool live = row < r_end;
-        const int tok = live ? row / a.group : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
+        const int tok = live ? int_div(row, a.by_group) : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
         lim = live && !it.bad ? it.past + (a.causal ? tok + 1 : 0) : 0;
         const elem_t* qp = reinterpret_cast<const elem_t*>(a.q) + (int64_t)(it.first + tok) * a.qs[0] + head * a.qs[1];
 #pragma unroll
@@ -637,7 +672,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk_kernel(PagedAttnArgs 
     const PagedAttnArgs z = arguments_again();
     asm volatile("" : "+v"(row));            // recomputed here, not kept through the loop
     const bool live = row < r_end;
-    const int tok = live ? row / z.group : 0, head = kvh * z.group + (live ? row - tok * z.group : 0);
+    const int tok = live ? int_div(row, z.by_group) : 0, head = kvh * z.group + (live ? row - tok * z.group : 0);
     const int64_t token = it.first + tok;
     if ((pg.bad || it.bad) && threadIdx.x == 0) atomicOr(z.status, (pg.bad ? PAGED_BAD_PAGE : 0) | (it.bad ? PAGED_BAD_LENGTH : 0));
     const bool bad = pg.bad || it.bad;
@@ -697,25 +732,25 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
     const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l31 = lane & 31, h = lane >> 5;
 
-    Schedule<C::M, KT> sched;
+    Schedule<C::M, KT, true> sched;
     begin(a, sched, TILE_LAG);
     const int item = blockIdx.x;
     if (item >= sched.items * a.kv_heads) return;
     // consecutive workgroups go to consecutive XCDs: with the key head innermost, an XCD's L2 holds few heads' pages
-    const int kvh = item % a.kv_heads;
+    const int at = int_div(item, a.by_kv_heads), kvh = item - at * a.kv_heads;
     Item it;
-    sched.find(a, item / a.kv_heads, &it);
+    sched.find(a, at, &it);
     if (it.split >= it.splits) return;
     const int k0 = it.k0, k1 = it.k1, r0 = it.tile * C::M, r_end = min(r0 + C::M, it.n * a.group);
     const int row = r0 + w * 32 + l31;                         // this lane's query
     const bool live = row < r_end;
-    const int tok = live ? row / a.group : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
+    const int tok = live ? int_div(row, a.by_group) : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
     const int64_t token = it.first + tok;
     const int lim = live && !it.bad ? it.past + (a.causal ? tok + 1 : 0) : 0;           // keys 0 .. lim - 1 are seen
     const int wr0 = r0 + w * 32, wr1 = min(wr0 + 32, r_end);                            // rows of this wave: [wr0, wr1)
     const bool some = wr0 < wr1 && !it.bad;
-    const int w_end = some ? it.past + (a.causal ? (wr1 - 1) / a.group + 1 : 0) : 0;    // keys any of them sees
-    const int w_all = some ? it.past + (a.causal ? wr0 / a.group + 1 : 0) : 0;          // keys all of them see
+    const int w_end = some ? it.past + (a.causal ? int_div(wr1 - 1, a.by_group) + 1 : 0) : 0;    // keys any of them sees
+    const int w_all = some ? it.past + (a.causal ? int_div(wr0, a.by_group) + 1 : 0) : 0;          // keys all of them see
 
     Pages pg;
     pg.row = a.table + it.seq * a.table_stride; pg.n_pages = a.n_pages; pg.bad = false; pg.base = 0; pg.ids = 0;
@@ -925,21 +960,21 @@ __global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kern
     __shared__ __attribute__((aligned(1024))) char smem[NW * 2 * C::STAGE];
     const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
 
-    Schedule<C::M, KT> sched;
+    Schedule<C::M, KT, false> sched;
     begin(a, sched, STEP_LAG);
     const int item = blockIdx.x;
     if (item >= sched.items * a.kv_heads) return;
-    const int kvh = item % a.kv_heads;
+    const int at = int_div(item, a.by_kv_heads), kvh = item - at * a.kv_heads;
     Item it;
-    sched.find(a, item / a.kv_heads, &it);
+    sched.find(a, at, &it);
     if (it.split >= it.splits) return;
     const int k0 = it.k0, k1 = it.k1, r0 = it.tile * C::M, r_end = min(r0 + C::M, it.n * a.group);
     const int row = r0 + l15;
     const bool live = row < r_end;
-    const int tok = live ? row / a.group : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
+    const int tok = live ? int_div(row, a.by_group) : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
     const int64_t token = it.first + tok;
     const int lim = live && !it.bad ? it.past + (a.causal ? tok + 1 : 0) : 0;
-    const int all = r_end - r0 == C::M && !it.bad ? it.past + (a.causal ? r0 / a.group + 1 : 0) : 0;      // keys every column sees
+    const int all = r_end - r0 == C::M && !it.bad ? it.past + (a.causal ? int_div(r0, a.by_group) + 1 : 0) : 0;      // keys every column sees
 
     Pages pg;
     pg.row = a.table + it.seq * a.table_stride; pg.n_pages = a.n_pages; pg.bad = false; pg.base = 0; pg.ids = 0;
@@ -1075,7 +1110,7 @@ __global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kern
         }
         const bool ruined = sum != sum && (pg.bad || it.bad);
         const float z = fmaf(acc[0], 0.f, fmaf(acc[1], 0.f, fmaf(acc[2], 0.f, fmaf(acc[3], 0.f, sum * 0.f))));
-        const int tk = on ? rr / a.group : 0, hd = kvh * a.group + (on ? rr - tk * a.group : 0);
+        const int tk = on ? int_div(rr, a.by_group) : 0, hd = kvh * a.group + (on ? rr - tk * a.group : 0);
         const int64_t t64 = it.first + tk;
         if (on) {
             if (it.splits > 1) {
@@ -1110,22 +1145,22 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
     __shared__ float weight[RPB == 1 ? MAX_SPLITS : 1], red[8];
     __shared__ f32x4 pieces[RPB == 1 ? 256 : 1];
     const int share = __builtin_bit_cast(int, a.part[0]);
-    Schedule<M, KT> sched;
+    Schedule<M, KT, false> sched;
     sched.share = 0x3fffffff;
     sched.load(a, 0);
-    sched.count(a);
+    sched.number(a);
     const int t = blockIdx.x / PARTS;
     if (t >= sched.items * a.kv_heads) return;
-    const int kvh = t % a.kv_heads;
+    const int at = int_div(t, a.by_kv_heads), kvh = t - at * a.kv_heads;
     Item it;
-    sched.find(a, t / a.kv_heads, &it);
+    sched.find(a, at, &it);
     const int kt = (it.end + KT - 1) / KT, splits = min(kt <= share ? 1 : (kt + share - 1) / share, a.splits);
     if (splits == 1) return;                 // written already
     const int tid = threadIdx.x, piece = tid % LPR, sub = tid / LPR % SP;
     const int row = it.tile * M + (blockIdx.x % PARTS) * RPB + (RPB == 1 ? 0 : tid / LPR);
     const bool live = row < it.n * a.group;
     if (RPB == 1 && !live) return;
-    const int tok = live ? row / a.group : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
+    const int tok = live ? int_div(row, a.by_group) : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
     const int64_t token = it.first + tok, orow = token * a.q_heads + head;
     f32x4 acc = {0, 0, 0, 0};
     float sum = 0.f;
@@ -1190,7 +1225,7 @@ Plan make_plan(const PagedAttnArgs& a, int max_new, int head_dim) {
     const int64_t keys = (int64_t)a.max_pages << a.page_shift, row_bytes = (int64_t)a.tokens * a.q_heads * (head_dim + 2) * 4;
     const bool full = est * a.kv_heads >= SLOTS;
     int64_t s = keys / MIN_SHARE;
-    if (keys <= (p.step ? (full ? 4096 : 1024) : (full ? 1024 : 512))) s = 1;
+    if (keys <= (p.step ? (full ? 4096 : 1024) : (full ? 2048 : 512))) s = 1;
     if (s > MAX_SPLITS) s = MAX_SPLITS;
     if (s > ((int64_t)128 << 20) / row_bytes) s = ((int64_t)128 << 20) / row_bytes;
     p.splits = s < 2 ? 1 : (int)s;
@@ -1201,6 +1236,8 @@ template <typename P, int D>
 hipError_t launch(PagedAttnArgs a, int max_new, hipStream_t s) {
     const Plan p = make_plan(a, max_new, D);
     a.splits = p.splits;
+    a.by_group = make_int_div((uint32_t)a.group);
+    a.by_kv_heads = make_int_div((uint32_t)a.kv_heads);
     // cutting adds at most 2 SLOTS items: a share is no less than a slot's part of a work that counts at least half of every tile's keys
     // (64 more for the roundings of that sum)
     const int64_t groups = (int64_t)p.tiles * a.kv_heads;
