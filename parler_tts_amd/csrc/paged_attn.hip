@@ -714,9 +714,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk_kernel(PagedAttnArgs 
 // =================================================================================================================================
 // Chunks in f32: a workgroup owns 128 rows (32 per wave), the keys pass in tiles of KT through a ring of LDS buffers.
 // =================================================================================================================================
-template <typename P, int D> struct TileCfg {
+template <int D> struct TileCfg {
     static constexpr int M = 128, NW = 4;
-    static constexpr int RB = D * (int)sizeof(typename P::elem_t);
+    static constexpr int RB = D * 4;
     static constexpr int KT = RB <= 256 ? 64 : 32;
     static constexpr int TILE = KT * RB;                       // bytes of K or V of a tile
     static constexpr int NBUF = 65536 / (2 * TILE);            // ring of tiles: 64 KiB, two workgroups on a CU
@@ -724,11 +724,12 @@ template <typename P, int D> struct TileCfg {
     static constexpr int DMA = 2 * TILE / NW / 1024;           // LDS-DMA instructions per wave and tile
 };
 
-template <typename P, int D>
+template <int D>
 __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a) {
-    typedef typename P::elem_t elem_t;
-    typedef TileCfg<P, D> C;
-    constexpr int KT = C::KT, RB = C::RB, EPL = P::EPL, NKS = D / (2 * EPL), NKB = KT / 32, NDB = D / 32;
+    typedef PF32 P;
+    typedef float elem_t;
+    typedef TileCfg<D> C;
+    constexpr int KT = C::KT, RB = C::RB, NKS = D / 8, NKB = KT / 32, NDB = D / 32;
     __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
     const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l31 = lane & 31, h = lane >> 5;
 
@@ -742,11 +743,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     sched.find(a, at, &it);
     if (it.split >= it.splits) return;
     const int k0 = it.k0, k1 = it.k1, r0 = it.tile * C::M, r_end = min(r0 + C::M, it.n * a.group);
-    const int row = r0 + w * 32 + l31;                         // this lane's query
-    const bool live = row < r_end;
-    const int tok = live ? int_div(row, a.by_group) : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
-    const int64_t token = it.first + tok;
-    const int lim = live && !it.bad ? it.past + (a.causal ? tok + 1 : 0) : 0;           // keys 0 .. lim - 1 are seen
+    int row = r0 + w * 32 + l31;                               // this lane's query
+    int lim;                                                   // keys 0 .. lim - 1 are seen
     const int wr0 = r0 + w * 32, wr1 = min(wr0 + 32, r_end);                            // rows of this wave: [wr0, wr1)
     const bool some = wr0 < wr1 && !it.bad;
     const int w_end = some ? it.past + (a.causal ? int_div(wr1 - 1, a.by_group) + 1 : 0) : 0;    // keys any of them sees
@@ -762,18 +760,17 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
         krows.template fetch<KT / C::NW>(pg, a.page_shift, key0, w * (KT / C::NW), k1, to);
         vrows.template fetch<KT / C::NW>(pg, a.page_shift, key0, w * (KT / C::NW), k1, to + C::TILE);
     };
-    // lane parts of the LDS addresses: row l31 of K (chunk 2 t + h at step t); for V the blocks of read_v (bf16) or row 4 h (f32)
-    const unsigned ka = l31 * RB + ((h ^ swizzle<RB, P::IS_BF16>(l31 & 15)) << 4);
-    const int i16 = lane & 15, vr = 4 * h + (i16 >> 2), vc = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
-    const unsigned va = vr * RB + ((vc ^ swizzle<RB, P::IS_BF16>(vr)) << 4) + (i16 & 1) * 8;
-    const unsigned vb = (vr + 8) * RB + ((vc ^ swizzle<RB, P::IS_BF16>(vr + 8)) << 4) + (i16 & 1) * 8;
+    const unsigned ka = l31 * RB + ((h ^ swizzle<RB, false>(l31 & 15)) << 4);        // row l31 of K, chunk 2 t + h at step t
 
-    // B operand of S^T = K Q^T: 16-byte chunk 2 s + h of the lane's query row at step s (and of the lane's key row for A)
-    u32x4 qf[NKS];
+    // B operand of S^T = K Q^T: 16-byte chunk 2 t + h of the lane's query row at step t (and of the lane's key row for A)
+    f32x4 qf[NKS];
     {
-        const elem_t* qp = reinterpret_cast<const elem_t*>(a.q) + token * a.qs[0] + head * a.qs[1];
+        const bool live = row < r_end;
+        const int tok = live ? int_div(row, a.by_group) : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
+        lim = live && !it.bad ? it.past + (a.causal ? tok + 1 : 0) : 0;
+        const elem_t* qp = reinterpret_cast<const elem_t*>(a.q) + (int64_t)(it.first + tok) * a.qs[0] + head * a.qs[1];
 #pragma unroll
-        for (int s = 0; s < NKS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qp + (2 * s + h) * EPL);
+        for (int t = 0; t < NKS; ++t) qf[t] = *reinterpret_cast<const f32x4*>(qp + (2 * t + h) * 4);
     }
     f32x16 o[NDB];
 #pragma unroll
@@ -800,41 +797,37 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
         if (key0 + (C::NBUF - 1) * KT < k1) fetch(key0 + (C::NBUF - 1) * KT, buf == 0 ? C::NBUF - 1 : buf - 1);
         if (key0 >= w_end) continue;         // nothing here for this wave's rows (it keeps moving its share of the tiles)
         const unsigned kt = lds + buf * 2 * C::TILE, vt = kt + C::TILE;
-        // reads of a key block are sent ahead of the products of the block in front (left to itself, hipcc reads, waits and multiplies in turn)
+        // operands are read two steps (of four products each, 256 cycles) ahead; left to itself, hipcc reads, waits and multiplies in turn
         f32x16 s[NKB];
-        u32x4 kf[2][NKS];
+        f32x4 kf[3];
+        const unsigned kat = kt + ka;
+        auto key_fragment = [&](int u) { kf[u % 3] = __builtin_bit_cast(f32x4, read_lds((kat ^ (u % NKS << 5)) + (u / NKS) * 32 * RB)); };
+        key_fragment(0);
+        key_fragment(1);
 #pragma unroll
-        for (int t = 0; t < NKS; ++t) kf[0][t] = read_lds(kt + (ka ^ (t << 5)));
+        for (int u = 0; u < NKB * NKS; ++u) {
+            if (u + 2 < NKB * NKS) key_fragment(u + 2);
+            if (u % NKS == 0) {
 #pragma unroll
-        for (int b = 0; b < NKB; ++b) {
-            if (b + 1 < NKB) {
-#pragma unroll
-                for (int t = 0; t < NKS; ++t) kf[(b + 1) & 1][t] = read_lds(kt + (b + 1) * 32 * RB + (ka ^ (t << 5)));
+                for (int r = 0; r < 16; ++r) s[u / NKS][r] = 0.f;
             }
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
-#pragma unroll
-            for (int t = 0; t < NKS; ++t) {
-                if constexpr (P::IS_BF16) {
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf[b & 1][t]), __builtin_bit_cast(bf16x8, qf[t]), s[b], 0, 0, 0);
-                } else {
-                    const f32x4 kx = __builtin_bit_cast(f32x4, kf[b & 1][t]), qx = __builtin_bit_cast(f32x4, qf[t]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(kx[j], qx[j], s[b], 0, 0, 0);
-                }
-            }
-        }
-        // V of the first steps travels while the softmax runs
-        constexpr int VSTEPS = KT / 16, VAHEAD = NDB == 2 ? VSTEPS : VSTEPS / 2;
-        bf16x8 vf[P::IS_BF16 ? VSTEPS : 1][NDB];
-        if constexpr (P::IS_BF16) {
-#pragma unroll
-            for (int kk = 0; kk < VAHEAD; ++kk)
-#pragma unroll
-                for (int d = 0; d < NDB; ++d) vf[kk][d] = read_v(vt + 16 * kk * RB + (va ^ (d << 6)), vt + 16 * kk * RB + (vb ^ (d << 6)));
+            for (int j = 0; j < 4; ++j) s[u / NKS] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[u % 3][j], qf[u % NKS][j], s[u / NKS], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
+        // the feature l31 of the slot's key, row b 32 + 8 (r / 4) + r % 4 + 4 h at step (b, r)
+        float vx[4][NDB];
+        const unsigned vat = vt + 4 * h * RB + (l31 & 3) * 4;
+        auto value_fragment = [&](int e) {
+            const int row = (e >> 4) * 32 + 8 * ((e & 15) >> 2) + (e & 3);
+            const unsigned sw = swizzle<RB, false>((row + 4 * h) & 15);
+#pragma unroll
+            for (int d = 0; d < NDB; ++d) vx[e & 3][d] = read_lds_f32(vat + row * RB + (((d * 8 + (l31 >> 2)) ^ sw) << 4));
+        };
+        value_fragment(0);
+        value_fragment(1);
+        value_fragment(2);
+        __builtin_amdgcn_sched_barrier(0);
         const uint64_t alive = tile_mask(a, it.seq, key0);
         if (key0 + KT > w_all || alive != ~0ull) {             // some key of the tile is not for some query
             const int left = lim - key0;
@@ -871,37 +864,21 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
                 s[b][r] = exp2_hw(fmaf(s[b][r], a.scale_log2, -mu));
                 l += s[b][r];
             }
-        if constexpr (P::IS_BF16) {
-            // key 16 kk + 4 h + 0 .. 3 in slots 0 .. 3, 8 further on in slots 4 .. 7
 #pragma unroll
-            for (int kk = 0; kk < KT / 16; ++kk) {
-                if (kk + VAHEAD < VSTEPS) {
+        for (int e = 0; e < 16 * NKB; ++e) {
+            if (e + 3 < 16 * NKB) value_fragment(e + 3);
 #pragma unroll
-                    for (int d = 0; d < NDB; ++d)
-                        vf[kk + VAHEAD][d] = read_v(vt + 16 * (kk + VAHEAD) * RB + (va ^ (d << 6)), vt + 16 * (kk + VAHEAD) * RB + (vb ^ (d << 6)));
-                }
-                bf16x8 pf;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) pf[j] = (__bf16)s[kk >> 1][8 * (kk & 1) + j];
-#pragma unroll
-                for (int d = 0; d < NDB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[kk][d], pf, o[d], 0, 0, 0);
-            }
-        } else {
-#pragma unroll
-            for (int b = 0; b < NKB; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int row = b * 32 + 8 * (r >> 2) + (r & 3);               // and 4 h
-                    const unsigned at = vt + (row + 4 * h) * RB + (l31 & 3) * 4;
-                    const unsigned sw = swizzle<RB, P::IS_BF16>((row + 4 * h) & 15);
-#pragma unroll
-                    for (int d = 0; d < NDB; ++d)
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(read_lds_f32(at + (((d * 8 + (l31 >> 2)) ^ sw) << 4)), s[b][r], o[d], 0, 0, 0);
-                }
+            for (int d = 0; d < NDB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vx[e & 3][d], s[e >> 4][e & 15], o[d], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     wait_vm<0>();
-    if ((pg.bad || it.bad) && threadIdx.x == 0) atomicOr(a.status, (pg.bad ? PAGED_BAD_PAGE : 0) | (it.bad ? PAGED_BAD_LENGTH : 0));
+    const PagedAttnArgs z = arguments_again();
+    asm volatile("" : "+v"(row));            // recomputed here, not kept through the loop
+    const bool live = row < r_end;
+    const int tok = live ? int_div(row, z.by_group) : 0, head = kvh * z.group + (live ? row - tok * z.group : 0);
+    const int64_t token = it.first + tok;
+    if ((pg.bad || it.bad) && threadIdx.x == 0) atomicOr(z.status, (pg.bad ? PAGED_BAD_PAGE : 0) | (it.bad ? PAGED_BAD_LENGTH : 0));
     const bool bad = pg.bad || it.bad;
     l += __shfl_xor(l, 32);
     float inv = l == 0.f ? 0.f : 1.f / l;
@@ -918,23 +895,23 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     }
     const uint64_t odds = __ballot(odd);
     if (live) {
-        const int64_t orow = token * a.q_heads + head;
+        const int64_t orow = token * z.q_heads + head;
 #pragma unroll
         for (int d = 0; d < NDB; ++d)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 const int f = d * 32 + 2 * r + 4 * h;
-                if (it.splits > 1) store4<PF32>(part_out<D>(a, it.split, orow) + f, o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
-                else store4<P>(reinterpret_cast<elem_t*>(a.out) + token * a.os[0] + head * a.os[1] + f, o[d][r] * inv, o[d][r + 1] * inv,
+                if (it.splits > 1) store4<PF32>(part_out<D>(z, it.split, orow) + f, o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
+                else store4<P>(reinterpret_cast<elem_t*>(z.out) + token * z.os[0] + head * z.os[1] + f, o[d][r] * inv, o[d][r + 1] * inv,
                                o[d][r + 2] * inv, o[d][r + 3] * inv);
             }
-        if (it.splits > 1 && h == 0) { float* ml = part_ml<D>(a, it.split, orow); ml[0] = m; ml[1] = l; }
+        if (it.splits > 1 && h == 0) { float* ml = part_ml<D>(z, it.split, orow); ml[0] = m; ml[1] = l; }
     }
     uint32_t again = (uint32_t)odds | (uint32_t)(odds >> 32);
     while (again) {
         const int i = __builtin_ctz(again);
         again &= again - 1;
-        store_row_alone<P, D>(a, it, kvh, wr0 + i);
+        store_row_alone<P, D>(z, it, kvh, wr0 + i);
     }
 }
 
@@ -1245,12 +1222,12 @@ hipError_t launch(PagedAttnArgs a, int max_new, hipStream_t s) {
     if (cut > 0x7fffffff / 16) return hipErrorInvalidValue;
     if (p.step) hipLaunchKernelGGL((paged_attn_step_kernel<P, D>), dim3((unsigned)cut), dim3(StepCfg<P, D>::NW * 64), 0, s, a);
     else if constexpr (P::IS_BF16) hipLaunchKernelGGL(paged_attn_chunk_kernel<D>, dim3((unsigned)cut), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((paged_attn_tile_kernel<P, D>), dim3((unsigned)cut), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(paged_attn_tile_kernel<D>, dim3((unsigned)cut), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
     constexpr int RPB = 1024 / D;
     if (p.step) hipLaunchKernelGGL((paged_attn_join_kernel<P, D, 16, 32, 1>), dim3((unsigned)groups * 16), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((paged_attn_join_kernel<P, D, 128, TileCfg<P, D>::KT, RPB>), dim3((unsigned)groups * (128 / RPB)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((paged_attn_join_kernel<P, D, 128, P::IS_BF16 ? 64 : TileCfg<D>::KT, RPB>), dim3((unsigned)groups * (128 / RPB)), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

@@ -34,20 +34,20 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-class _OnDevice:
-    """makes `device` the current one for a launch if it is not; the current stream of it is `stream`"""
+# the current stream's handle without the object around it (2.6 us of a call that launches in 3)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-    def __init__(self, device: torch.device):
-        self.other = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
-    def __enter__(self) -> int:
-        if self.other is not None:
-            self.other.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.other is not None:
-            self.other.__exit__(*exc)
+def _launch(device: torch.device, entry, *args) -> None:
+    """one C entry on the current stream of `device`, which is made the current device for the call if it is not"""
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = entry(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, _raw_stream(index))
+    if rc:
+        _hip.check(rc)
 
 
 def _read_status(status: torch.Tensor, who: str) -> None:
@@ -115,6 +115,7 @@ class RotaryTable:
         self.head_dim, self.positions, self.rotary_dim, self.layout = head_dim, positions, rotary_dim, layout
         self.device = self.cos.device
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._status = self.status.data_ptr()
         self._c = _hip.PttsRotary(self.cos.data_ptr(), self.sin.data_ptr(), positions, rotary_dim, 1 if layout == "interleaved" else 0)
         self._ref = C.addressof(self._c)
 
@@ -150,6 +151,7 @@ class PagedKVCache:
         self.num_pages, self.kv_heads, self.page_tokens, self.head_dim = pages, heads, tokens, dim
         self.dtype, self.device = k.dtype, k.device
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._status = self.status.data_ptr()
         self._c = _hip.PttsPagedKV(k.data_ptr(), v.data_ptr(), (C.c_int64 * 3)(*k.stride()[:3]), (C.c_int64 * 3)(*v.stride()[:3]),
                                    _DTYPES[k.dtype], pages, heads, tokens, dim)
         self._ref = C.addressof(self._c)
@@ -208,7 +210,7 @@ def rotary_embed(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, 
     if positions.shape[0] != tokens:
         raise ValueError(f"{positions.shape[0]} positions for {tokens} tokens")
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     else:
         _rows("out", out, tokens, heads, rotary.head_dim, rotary.device)
         if out.dtype != x.dtype:
@@ -216,10 +218,8 @@ def rotary_embed(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, 
     if heads == 0 or tokens == 0:
         return out
     xs, os = x.stride(), out.stride()
-    with _OnDevice(rotary.device) as stream:
-        _hip.check(_hip.load_library().ptts_rotary_embed(
-            rotary._ref, _DTYPES[x.dtype], tokens, heads, rotary.head_dim, x.data_ptr(), xs[0], xs[1], positions.data_ptr(), out.data_ptr(),
-            os[0], os[1], rotary.status.data_ptr(), stream))
+    _launch(rotary.device, _hip.load_library().ptts_rotary_embed, rotary._ref, _DTYPES[x.dtype], tokens, heads, rotary.head_dim, x.data_ptr(),
+            xs[0], xs[1], positions.data_ptr(), out.data_ptr(), os[0], os[1], rotary._status)
     return out
 
 
@@ -256,7 +256,7 @@ def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, table: torc
         if q.dtype != k.dtype or heads == 0:
             raise ValueError(f"q {tuple(q.shape)} of {q.dtype} beside k of {k.dtype}")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
             _rows("q_out", q_out, tokens, heads, cache.head_dim, device)
             if q_out.dtype != q.dtype:
@@ -266,10 +266,8 @@ def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, table: torc
         raise ValueError("q_out without q")
     if tokens == 0:
         return q_out
-    with _OnDevice(device) as stream:
-        _hip.check(_hip.load_library().ptts_kv_append(
-            cache._ref, C.addressof(batch), _DTYPES[k.dtype], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], rot, at,
-            heads, qp, qs[0], qs[1], qop, qos[0], qos[1], cache.status.data_ptr(), stream))
+    _launch(device, _hip.load_library().ptts_kv_append, cache._ref, C.addressof(batch), _DTYPES[k.dtype], k.data_ptr(), ks[0], ks[1],
+            v.data_ptr(), vs[0], vs[1], rot, at, heads, qp, qs[0], qs[1], qop, qos[0], qos[1], cache._status)
     return q_out
 
 
@@ -304,7 +302,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
             key_mask = key_mask.contiguous()          # one row for every sequence, expanded
             mask = key_mask.data_ptr()
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _rows("out", out, tokens, heads, dim, device)
         if out.dtype != q.dtype:
@@ -324,9 +322,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
         cache._workspace[key] = need
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     qs, os = q.stride(), out.stride()
-    with _OnDevice(device) as stream:
-        _hip.check(lib.ptts_paged_attention(
-            cache._ref, bref, heads, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], dim ** -0.5 if scale is None else scale,
-            1 if causal else 0, mask, mask_stride, mask_width, max_new, workspace.data_ptr() if need else None, need,
-            cache.status.data_ptr(), stream))
+    _launch(device, lib.ptts_paged_attention, cache._ref, bref, heads, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
+            dim ** -0.5 if scale is None else scale, 1 if causal else 0, mask, mask_stride, mask_width, max_new,
+            workspace.data_ptr() if need else None, need, cache._status)
     return out
