@@ -185,10 +185,16 @@ template <int M, int KT, bool SORTED> struct Schedule {
     __device__ __forceinline__ void sort(const PagedAttnArgs& a) {
         const int lane = threadIdx.x & 63, here = min(a.n_seqs - base, 64), key = n > 0 ? key_tiles(a) : 0;
         if (here <= 1) return;
-        int rank = 0;
-        for (int j = 0; j < here; ++j) {
-            const int other = __builtin_amdgcn_readlane(key, j);
-            rank += other > key || (other == key && j < lane) ? 1 : 0;
+        // eight classes of length, longest first, in order within a class
+        const float top = (float)wave_max_u32((unsigned)key);
+        const int cls = 7 - min((int)((float)key * (8.f / (top + 1.f))), 7);
+        int rank = 0, before = 0;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const uint64_t m = __ballot(lane < here && cls == c);
+            const int mine = before + (int)__popcll(m & ((1ull << lane) - 1));
+            rank = cls == c ? mine : rank;
+            before += (int)__popcll(m);
         }
         if (lane >= here) rank = lane;
         seq = __builtin_amdgcn_ds_permute(rank << 2, seq);
