@@ -76,7 +76,8 @@ struct PagedAttnArgs {
     int64_t table_stride, mask_stride;
     float scale_log2;        // softmax scale * log2(e)
     int max_pages, n_pages, page_shift, n_seqs, tokens, mask_width, causal;
-    int q_heads, kv_heads, group, splits;
+    int q_heads, kv_heads, group;
+    int splits, min_share;   // most shares of a tile's keys; least keys of one
     IntDiv by_group, by_kv_heads;
 };
 

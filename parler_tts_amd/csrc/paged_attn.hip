@@ -137,9 +137,9 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // every wave sums the sequences' tiles up for itself, 64 sequences at a time, all lengths in one round trip.  Items are numbered without
 // holes (with holes between the sequences the dispatcher put all work of equal chunks on half of the CUs).
 // Keys are shared out only where that evens the load: SLOTS workgroups run at a time, and a tile whose keys exceed what one of them would
-// get of everything (by the factor LAG) is cut into shares of that size, at least MIN_SHARE keys each (a share costs its rows' f32 partial
+// get of everything (by the factor LAG) is cut into shares of that size, at least min_share keys each (a share costs its rows' f32 partial
 // results, written and read once more).
-constexpr int SLOTS = 512, MIN_SHARE = 256, MAX_SPLITS = 256;
+constexpr int SLOTS = 512, MAX_SPLITS = 256;
 constexpr float TILE_LAG = 2.f, STEP_LAG = 2.f;
 
 struct Item {
@@ -219,7 +219,16 @@ template <int M, int KT, bool SORTED> struct Schedule {
             }
             const float mean = wave_sum(work) * (float)a.kv_heads / SLOTS;
             most = (int)wave_max_u32((unsigned)most);
-            if ((float)most > lag * mean) share = max(max((int)ceilf(mean), MIN_SHARE / KT), (most + a.splits - 1) / a.splits);
+            if ((float)most > lag * mean) {
+                // a slot's part of everything; a little more where the shares' ends would need a second round of a few workgroups
+                const int least = max(a.min_share / KT, (most + a.splits - 1) / a.splits);
+                for (int step = 4; step <= 8; ++step) {
+                    share = max((int)ceilf(mean * 0.25f * (float)step), least);
+                    if (a.n_seqs > 64 || step == 8) break;
+                    const int all = uniform(__builtin_amdgcn_readlane(scan_add(row_tiles(a) * shares(key_tiles(a))), 63));
+                    if (all * a.kv_heads <= SLOTS) break;
+                }
+            }
             share = uniform(share);
             if (a.n_seqs > 64) load(a, 0);
         }
@@ -718,14 +727,13 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk_kernel(PagedAttnArgs 
 }
 
 // =================================================================================================================================
-// Chunks in f32: a workgroup owns 128 rows (32 per wave), the keys pass in tiles of KT through a ring of LDS buffers.
+// Chunks in f32: a workgroup owns 64 rows, 16 per wave (the f32 matrix rate is a sixteenth of bf16's and the same for 16 x 16 x 4 as for
+// 32 x 32 x 2: the smaller shape wastes fewer rows of a ragged batch), the keys pass in tiles of 32 through a ring of LDS buffers.
 // =================================================================================================================================
 template <int D> struct TileCfg {
-    static constexpr int M = 128, NW = 4;
-    static constexpr int RB = D * 4;
-    static constexpr int KT = RB <= 256 ? 64 : 32;
+    static constexpr int M = 64, NW = 4, KT = 32, RB = D * 4;
     static constexpr int TILE = KT * RB;                       // bytes of K or V of a tile
-    static constexpr int NBUF = 65536 / (2 * TILE);            // ring of tiles: 64 KiB, two workgroups on a CU
+    static constexpr int NBUF = D == 64 ? 3 : 2;               // 48 / 64 KiB: three / two workgroups on a CU
     static constexpr int LDS = NBUF * 2 * TILE;                // [buffer][K, V]
     static constexpr int DMA = 2 * TILE / NW / 1024;           // LDS-DMA instructions per wave and tile
 };
@@ -735,26 +743,28 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     typedef PF32 P;
     typedef float elem_t;
     typedef TileCfg<D> C;
-    constexpr int KT = C::KT, RB = C::RB, NKS = D / 8, NKB = KT / 32, NDB = D / 32;
+    constexpr int KT = C::KT, RB = C::RB, NKS = D / 16, NDB = D / 16;
     __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
-    const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l31 = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
 
     Schedule<C::M, KT, true> sched;
     begin(a, sched, TILE_LAG);
     const int item = blockIdx.x;
     if (item >= sched.items * a.kv_heads) return;
-    // consecutive workgroups go to consecutive XCDs: with the key head innermost, an XCD's L2 holds few heads' pages
     const int at = int_div(item, a.by_kv_heads), kvh = item - at * a.kv_heads;
     Item it;
     sched.find(a, at, &it);
     if (it.split >= it.splits) return;
     const int k0 = it.k0, k1 = it.k1, r0 = it.tile * C::M, r_end = min(r0 + C::M, it.n * a.group);
-    int row = r0 + w * 32 + l31;                               // this lane's query
-    int lim;                                                   // keys 0 .. lim - 1 are seen
-    const int wr0 = r0 + w * 32, wr1 = min(wr0 + 32, r_end);                            // rows of this wave: [wr0, wr1)
+    const int row = r0 + w * 16 + l15;                                                  // this lane's query
+    const bool live = row < r_end;
+    const int tok = live ? int_div(row, a.by_group) : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
+    const int64_t token = it.first + tok;
+    const int lim = live && !it.bad ? it.past + (a.causal ? tok + 1 : 0) : 0;           // keys 0 .. lim - 1 are seen
+    const int wr0 = r0 + w * 16, wr1 = min(wr0 + 16, r_end);                            // rows of this wave: [wr0, wr1)
     const bool some = wr0 < wr1 && !it.bad;
     const int w_end = some ? it.past + (a.causal ? int_div(wr1 - 1, a.by_group) + 1 : 0) : 0;    // keys any of them sees
-    const int w_all = some ? it.past + (a.causal ? int_div(wr0, a.by_group) + 1 : 0) : 0;          // keys all of them see
+    const int w_all = some ? it.past + (a.causal ? int_div(wr0, a.by_group) + 1 : 0) : 0;        // keys all of them see
 
     Pages pg;
     pg.row = a.table + it.seq * a.table_stride; pg.n_pages = a.n_pages; pg.bad = false; pg.base = 0; pg.ids = 0;
@@ -766,27 +776,20 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
         krows.template fetch<KT / C::NW>(pg, a.page_shift, key0, w * (KT / C::NW), k1, to);
         vrows.template fetch<KT / C::NW>(pg, a.page_shift, key0, w * (KT / C::NW), k1, to + C::TILE);
     };
-    const unsigned ka = l31 * RB + ((h ^ swizzle<RB, false>(l31 & 15)) << 4);        // row l31 of K, chunk 2 t + h at step t
+    const unsigned ka = l15 * RB + ((g ^ swizzle<RB, false>(l15)) << 4);                // row l15 of K, chunk 4 t + g at step t
 
-    // B operand of S^T = K Q^T: 16-byte chunk 2 t + h of the lane's query row at step t (and of the lane's key row for A)
     f32x4 qf[NKS];
     {
-        const bool live = row < r_end;
-        const int tok = live ? int_div(row, a.by_group) : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
-        lim = live && !it.bad ? it.past + (a.causal ? tok + 1 : 0) : 0;
-        const elem_t* qp = reinterpret_cast<const elem_t*>(a.q) + (int64_t)(it.first + tok) * a.qs[0] + head * a.qs[1];
+        const elem_t* qp = reinterpret_cast<const elem_t*>(a.q) + token * a.qs[0] + head * a.qs[1];
 #pragma unroll
-        for (int t = 0; t < NKS; ++t) qf[t] = *reinterpret_cast<const f32x4*>(qp + (2 * t + h) * 4);
+        for (int t = 0; t < NKS; ++t) qf[t] = *reinterpret_cast<const f32x4*>(qp + (4 * t + g) * 4);
     }
-    f32x16 o[NDB];
+    f32x4 o[NDB];
 #pragma unroll
-    for (int d = 0; d < NDB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-    float m = -INFINITY, l = 0.f;       // maximum of the query's scores (log2 units), sum of the weights of this half's keys
-
-    // the query rows arrive before the first tile is sent for: a wait for them inside the loop would be one for the tiles in flight too
+    for (int d = 0; d < NDB; ++d) o[d] = {0, 0, 0, 0};
+    float m = -INFINITY, l = 0.f;       // maximum of the query's scores (log2 units), sum of the weights of this lane's keys
     if (k0 < k1) pg.load(k0 >> a.page_shift, (k1 - 1) >> a.page_shift);
+    // the query rows arrive before the first tile is sent for: a wait for them inside the loop would be one for the tiles in flight too
 #pragma unroll
     for (int t = 0; t < NKS; ++t) asm volatile("" : "+v"(qf[t]));
 #pragma unroll
@@ -794,152 +797,128 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
         if (k0 + i * KT < k1) fetch(k0 + i * KT, i);
     int buf = 0;
     for (int key0 = k0; key0 < k1; key0 += KT, buf = buf + 1 == C::NBUF ? 0 : buf + 1) {
-        const int ahead = min(C::NBUF - 2, (k1 - key0 - 1) / KT);           // younger tiles that stay in flight
-        if (C::NBUF > 3 && ahead >= 2) wait_vm<2 * C::DMA>();
-        else if (C::NBUF > 2 && ahead >= 1) wait_vm<C::DMA>();
+        if (C::NBUF > 2 && key0 + KT < k1) wait_vm<C::DMA>();                           // the younger tile stays in flight
         else wait_vm<0>();
         wait_lds();
         __builtin_amdgcn_s_barrier();        // the tile has landed, and every wave has left the buffer of the tile before it
         if (key0 + (C::NBUF - 1) * KT < k1) fetch(key0 + (C::NBUF - 1) * KT, buf == 0 ? C::NBUF - 1 : buf - 1);
         if (key0 >= w_end) continue;         // nothing here for this wave's rows (it keeps moving its share of the tiles)
         const unsigned kt = lds + buf * 2 * C::TILE, vt = kt + C::TILE;
-        // operands are read two steps (of four products each, 256 cycles) ahead; left to itself, hipcc reads, waits and multiplies in turn
-        f32x16 s[NKB];
-        f32x4 kf[3];
+        // operands are read two steps (of four products each) ahead; left to itself, hipcc reads, waits and multiplies in turn
+        f32x4 s[2], kf[3];
         const unsigned kat = kt + ka;
-        auto key_fragment = [&](int u) { kf[u % 3] = __builtin_bit_cast(f32x4, read_lds((kat ^ (u % NKS << 5)) + (u / NKS) * 32 * RB)); };
+        auto key_fragment = [&](int u) { kf[u % 3] = __builtin_bit_cast(f32x4, read_lds((kat ^ (u % NKS << 6)) + (u / NKS) * 16 * RB)); };
         key_fragment(0);
         key_fragment(1);
 #pragma unroll
-        for (int u = 0; u < NKB * NKS; ++u) {
-            if (u + 2 < NKB * NKS) key_fragment(u + 2);
-            if (u % NKS == 0) {
+        for (int u = 0; u < 2 * NKS; ++u) {
+            if (u + 2 < 2 * NKS) key_fragment(u + 2);
+            if (u % NKS == 0) s[u / NKS] = {0, 0, 0, 0};
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[u / NKS][r] = 0.f;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[u / NKS] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[u % 3][j], qf[u % NKS][j], s[u / NKS], 0, 0, 0);
+            for (int j = 0; j < 4; ++j) s[u / NKS] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[u % 3][j], qf[u % NKS][j], s[u / NKS], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
-        // the feature l31 of the slot's key, row b 32 + 8 (r / 4) + r % 4 + 4 h at step (b, r)
-        float vx[4][NDB];
-        const unsigned vat = vt + 4 * h * RB + (l31 & 3) * 4;
+        // step e: feature 16 d + l15 of key 16 (e / 4) + 4 g + e % 4
+        float vx[3][NDB];
+        const unsigned vat = vt + 4 * g * RB + (l15 & 3) * 4;
         auto value_fragment = [&](int e) {
-            const int row = (e >> 4) * 32 + 8 * ((e & 15) >> 2) + (e & 3);
-            const unsigned sw = swizzle<RB, false>((row + 4 * h) & 15);
+            const int r = (e >> 2) * 16 + (e & 3);
+            const unsigned sw = swizzle<RB, false>((r + 4 * g) & 15);
 #pragma unroll
-            for (int d = 0; d < NDB; ++d) vx[e & 3][d] = read_lds_f32(vat + row * RB + (((d * 8 + (l31 >> 2)) ^ sw) << 4));
+            for (int d = 0; d < NDB; ++d) vx[e % 3][d] = read_lds_f32(vat + r * RB + (((d * 4 + (l15 >> 2)) ^ sw) << 4));
         };
         value_fragment(0);
         value_fragment(1);
-        value_fragment(2);
         __builtin_amdgcn_sched_barrier(0);
         const uint64_t alive = tile_mask(a, it.seq, key0);
-        if (key0 + KT > w_all || alive != ~0ull) {             // some key of the tile is not for some query
+        if (key0 + KT > w_all || (uint32_t)alive != ~0u) {             // some key of the tile is not for some query
             const int left = lim - key0;
-            const uint64_t see = (left >= 64 ? ~0ull : (left <= 0 ? 0ull : (1ull << left) - 1)) & alive;
-            const uint32_t half[2] = {(uint32_t)(see >> (4 * h)), (uint32_t)(see >> 32 >> (4 * h))};
+            const uint32_t see = (left >= 32 ? ~0u : (left <= 0 ? 0u : (1u << left) - 1)) & (uint32_t)alive;
 #pragma unroll
-            for (int b = 0; b < NKB; ++b)
+            for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    s[b][r] = (half[b] >> ((r & 3) + 8 * (r >> 2))) & 1 ? s[b][r] : -INFINITY;
+                for (int r = 0; r < 4; ++r) s[b][r] = (see >> (16 * b + 4 * g + r)) & 1 ? s[b][r] : -INFINITY;
         }
-        float mx = s[0][0];
-#pragma unroll
-        for (int b = 0; b < NKB; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
-        mx = swap_max32(mx) * a.scale_log2;
-        // weights are kept relative to a maximum that may lag behind by 2^8 (their type holds that range as well as any): the sums
-        // are rescaled only when a query's maximum has risen further
-        if (__any(mx > m + 8.f)) {
+        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        mx = swap_max32(swap_max16(mx)) * a.scale_log2;
+        if (__any(mx > m + 8.f)) {           // as in the chunk kernel
             const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.f : exp2_hw(m - mn);
             m = mn;
             l *= al;
 #pragma unroll
             for (int d = 0; d < NDB; ++d)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[d][r] *= al;
+                for (int r = 0; r < 4; ++r) o[d][r] *= al;
         }
         const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int b = 0; b < NKB; ++b)
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
+            for (int r = 0; r < 4; ++r) {
                 s[b][r] = exp2_hw(fmaf(s[b][r], a.scale_log2, -mu));
                 l += s[b][r];
             }
 #pragma unroll
-        for (int e = 0; e < 16 * NKB; ++e) {
-            if (e + 3 < 16 * NKB) value_fragment(e + 3);
+        for (int e = 0; e < 8; ++e) {
+            if (e + 2 < 8) value_fragment(e + 2);
 #pragma unroll
-            for (int d = 0; d < NDB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vx[e & 3][d], s[e >> 4][e & 15], o[d], 0, 0, 0);
+            for (int d = 0; d < NDB; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[e % 3][d], s[e >> 2][e & 3], o[d], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
     wait_vm<0>();
-    const PagedAttnArgs z = arguments_again();
-    asm volatile("" : "+v"(row));            // recomputed here, not kept through the loop
-    const bool live = row < r_end;
-    const int tok = live ? int_div(row, z.by_group) : 0, head = kvh * z.group + (live ? row - tok * z.group : 0);
-    const int64_t token = it.first + tok;
-    if ((pg.bad || it.bad) && threadIdx.x == 0) atomicOr(z.status, (pg.bad ? PAGED_BAD_PAGE : 0) | (it.bad ? PAGED_BAD_LENGTH : 0));
+    if ((pg.bad || it.bad) && threadIdx.x == 0) atomicOr(a.status, (pg.bad ? PAGED_BAD_PAGE : 0) | (it.bad ? PAGED_BAD_LENGTH : 0));
     const bool bad = pg.bad || it.bad;
+    l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     float inv = l == 0.f ? 0.f : 1.f / l;
     if (bad) { l = NAN; inv = NAN; }
-    // a result that is not finite: of this query's own making, or a key that it does not see
-    bool odd = false;
+    bool odd = false;                        // as in the chunk kernel
     if (!bad) {
         float z = l * 0.f;
 #pragma unroll
         for (int d = 0; d < NDB; ++d)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) z = fmaf(o[d][r], 0.f, z);
+            for (int r = 0; r < 4; ++r) z = fmaf(o[d][r], 0.f, z);
         odd = live && !(z == 0.f);
     }
     const uint64_t odds = __ballot(odd);
     if (live) {
-        const int64_t orow = token * z.q_heads + head;
+        const int64_t orow = token * a.q_heads + head;
 #pragma unroll
-        for (int d = 0; d < NDB; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int f = d * 32 + 2 * r + 4 * h;
-                if (it.splits > 1) store4<PF32>(part_out<D>(z, it.split, orow) + f, o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]);
-                else store4<P>(reinterpret_cast<elem_t*>(z.out) + token * z.os[0] + head * z.os[1] + f, o[d][r] * inv, o[d][r + 1] * inv,
-                               o[d][r + 2] * inv, o[d][r + 3] * inv);
-            }
-        if (it.splits > 1 && h == 0) { float* ml = part_ml<D>(z, it.split, orow); ml[0] = m; ml[1] = l; }
+        for (int d = 0; d < NDB; ++d) {
+            const int f = d * 16 + 4 * g;
+            if (it.splits > 1) store4<P>(part_out<D>(a, it.split, orow) + f, o[d][0], o[d][1], o[d][2], o[d][3]);
+            else store4<P>(reinterpret_cast<elem_t*>(a.out) + token * a.os[0] + head * a.os[1] + f, o[d][0] * inv, o[d][1] * inv, o[d][2] * inv, o[d][3] * inv);
+        }
+        if (it.splits > 1 && g == 0) { float* ml = part_ml<D>(a, it.split, orow); ml[0] = m; ml[1] = l; }
     }
-    uint32_t again = (uint32_t)odds | (uint32_t)(odds >> 32);
+    uint32_t again = (uint32_t)(odds | odds >> 16 | odds >> 32 | odds >> 48) & 0xffffu;
     while (again) {
         const int i = __builtin_ctz(again);
         again &= again - 1;
-        store_row_alone<P, D>(z, it, kvh, wr0 + i);
+        store_row_alone<P, D>(a, it, kvh, wr0 + i);
     }
 }
 
 // =================================================================================================================================
 // Few rows (at most 16 per sequence and key head: single tokens, their groups, short drafts): bound by the stream of the cache.  A wave
-// owns every NW-th tile of 32 keys and two LDS buffers of its own, so that nothing in the loop waits for another wave; the waves'
+// owns every NW-th tile of 32 (f32: 16) keys and two LDS buffers of its own, so that nothing in the loop waits for another wave; the waves'
 // states are joined once at the end.
 // =================================================================================================================================
 template <typename P, int D> struct StepCfg {
-    static constexpr int M = 16, KT = 32;
+    static constexpr int M = 16, KT = P::IS_BF16 ? 32 : 16;
     static constexpr int RB = D * (int)sizeof(typename P::elem_t);
     static constexpr int TILE = KT * RB, STAGE = 2 * TILE;
-    static constexpr int NW = 65536 / (2 * STAGE);             // 4, 2, 2, 1 waves: 64 KiB of LDS, two workgroups on a CU
     static constexpr int DMA = STAGE / 1024;
-    static_assert(NW * 16 * (D + 2) * 4 <= NW * 2 * STAGE, "the waves' states fit where their tiles were");
+    static_assert(16 * (D + 2) * 4 <= 2 * STAGE, "the waves' states fit where their tiles were");
 };
 
-template <typename P, int D>
-__global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kernel(PagedAttnArgs a) {
+template <typename P, int D, int NW>
+__global__ __launch_bounds__(NW * 64) void paged_attn_step_kernel(PagedAttnArgs a) {
     typedef typename P::elem_t elem_t;
     typedef StepCfg<P, D> C;
-    constexpr int KT = C::KT, RB = C::RB, EPL = P::EPL, NKS = D / (4 * EPL), NDB = D / 16, NW = C::NW;
+    constexpr int KT = C::KT, KB = KT / 16, RB = C::RB, EPL = P::EPL, NKS = D / (4 * EPL), NDB = D / 16;
     __shared__ __attribute__((aligned(1024))) char smem[NW * 2 * C::STAGE];
     const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
 
@@ -995,9 +974,9 @@ __global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kern
         if (key0 + NW * KT < k1) { fetch(key0 + NW * KT, buf ^ 1); wait_vm<C::DMA>(); }
         else wait_vm<0>();
         const unsigned kt = ring + buf * C::STAGE, vt = kt + C::TILE;
-        f32x4 s[2];
+        f32x4 s[KB];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < KB; ++b) {
             s[b] = {0, 0, 0, 0};
 #pragma unroll
             for (int t = 0; t < NKS; ++t) {
@@ -1012,15 +991,17 @@ __global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kern
             }
         }
         const uint64_t alive = tile_mask(a, it.seq, key0);
-        if (key0 + KT > all || (uint32_t)alive != ~0u) {
+        constexpr uint32_t seen = KT == 32 ? ~0u : (1u << KT % 32) - 1;
+        if (key0 + KT > all || ((uint32_t)alive & seen) != seen) {
             const int left = lim - key0;
-            const uint32_t see = (left >= 32 ? ~0u : (left <= 0 ? 0u : (1u << left) - 1)) & (uint32_t)alive;
+            const uint32_t see = (left >= KT ? seen : (left <= 0 ? 0u : (1u << left) - 1)) & (uint32_t)alive;
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < KB; ++b)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s[b][r] = (see >> (16 * b + 4 * g + r)) & 1 ? s[b][r] : -INFINITY;
         }
-        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+        if constexpr (KB == 2) mx = fmaxf(mx, fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         mx = swap_max32(swap_max16(mx)) * a.scale_log2;
         if (__any(mx > m + 8.f)) {           // as in the tile kernel
             const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.f : exp2_hw(m - mn);
@@ -1033,7 +1014,7 @@ __global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kern
         }
         const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 s[b][r] = exp2_hw(fmaf(s[b][r], a.scale_log2, -mu));
@@ -1049,7 +1030,7 @@ __global__ __launch_bounds__((StepCfg<P, D>::NW * 64)) void paged_attn_step_kern
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(read_v(vt + (va ^ (d << 5)), vt + 16 * RB + (va ^ (d << 5))), pf, o[d], 0, 0, 0);
         } else {
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < KB; ++b)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int row = 16 * b + 4 * g + r;
@@ -1192,14 +1173,15 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
     }
 }
 
-struct Plan { bool step; int tiles, splits; };
+struct Plan { bool step; int tiles, splits, min_share; };
 
 // max_new tokens a sequence at most (0: not known) make at most max_new * group rows per key head: up to 16 take the step kernel.
-Plan make_plan(const PagedAttnArgs& a, int max_new, int head_dim) {
+Plan make_plan(const PagedAttnArgs& a, int max_new, int head_dim, int dtype) {
+    const int row_of_cache = head_dim * (dtype == PTTS_BF16 ? 2 : 4);
     Plan p;
     const int64_t most = (a.starts ? max_new : 1) * (int64_t)a.group;       // 0: not known
     p.step = most > 0 && most <= 16;
-    const int M = p.step ? 16 : 128;
+    const int M = p.step ? 16 : (dtype == PTTS_BF16 ? 128 : 64);
     const int64_t ub = a.starts ? (int64_t)a.tokens * a.group / M + a.n_seqs : (int64_t)a.n_seqs * ((a.group + M - 1) / M);
     p.tiles = (int)ub;
     int64_t est = most > 0 ? (int64_t)a.n_seqs * ((most + M - 1) / M) : ub;
@@ -1207,18 +1189,33 @@ Plan make_plan(const PagedAttnArgs& a, int max_new, int head_dim) {
     // most shares of a tile: none where the keys a workgroup could be left with alone take less time than joining; 128 MiB of partial results
     const int64_t keys = (int64_t)a.max_pages << a.page_shift, row_bytes = (int64_t)a.tokens * a.q_heads * (head_dim + 2) * 4;
     const bool full = est * a.kv_heads >= SLOTS;
-    int64_t s = keys / MIN_SHARE;
-    if (keys <= (p.step ? (full ? 4096 : 1024) : (full ? 2048 : 512))) s = 1;
+    p.min_share = 32768 / row_of_cache < 32 ? 32 : 32768 / row_of_cache;    // 32 KiB of keys: 256 rows of 64 in bf16, 64 of 128 in f32
+    int64_t s = keys / p.min_share;
+    if (keys <= (p.step ? (full ? 4096 : 1024) : p.min_share * (full ? 8 : 2))) s = 1;
     if (s > MAX_SPLITS) s = MAX_SPLITS;
     if (s > ((int64_t)128 << 20) / row_bytes) s = ((int64_t)128 << 20) / row_bytes;
     p.splits = s < 2 ? 1 : (int)s;
     return p;
 }
 
+// Four waves with stages of 16 KiB have a CU to themselves, two share it with another workgroup: four where the launch gives a CU no
+// second workgroup anyway.
+template <typename P, int D>
+void launch_step(const PagedAttnArgs& a, unsigned items, hipStream_t s) {
+    if constexpr (StepCfg<P, D>::STAGE > 8192) {
+        if (items > 256) {
+            hipLaunchKernelGGL((paged_attn_step_kernel<P, D, 2>), dim3(items), dim3(128), 0, s, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((paged_attn_step_kernel<P, D, 4>), dim3(items), dim3(256), 0, s, a);
+}
+
 template <typename P, int D>
 hipError_t launch(PagedAttnArgs a, int max_new, hipStream_t s) {
-    const Plan p = make_plan(a, max_new, D);
+    const Plan p = make_plan(a, max_new, D, P::IS_BF16 ? PTTS_BF16 : PTTS_F32);
     a.splits = p.splits;
+    a.min_share = p.min_share;
     a.by_group = make_int_div((uint32_t)a.group);
     a.by_kv_heads = make_int_div((uint32_t)a.kv_heads);
     // cutting adds at most 2 SLOTS items: a share is no less than a slot's part of a work that counts at least half of every tile's keys
@@ -1226,21 +1223,22 @@ hipError_t launch(PagedAttnArgs a, int max_new, hipStream_t s) {
     const int64_t groups = (int64_t)p.tiles * a.kv_heads;
     const int64_t cut = groups * p.splits < groups + 2 * SLOTS + 64 ? groups * p.splits : groups + 2 * SLOTS + 64;
     if (cut > 0x7fffffff / 16) return hipErrorInvalidValue;
-    if (p.step) hipLaunchKernelGGL((paged_attn_step_kernel<P, D>), dim3((unsigned)cut), dim3(StepCfg<P, D>::NW * 64), 0, s, a);
+    if (p.step) launch_step<P, D>(a, (unsigned)cut, s);
     else if constexpr (P::IS_BF16) hipLaunchKernelGGL(paged_attn_chunk_kernel<D>, dim3((unsigned)cut), dim3(256), 0, s, a);
     else hipLaunchKernelGGL(paged_attn_tile_kernel<D>, dim3((unsigned)cut), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
     constexpr int RPB = 1024 / D;
-    if (p.step) hipLaunchKernelGGL((paged_attn_join_kernel<P, D, 16, 32, 1>), dim3((unsigned)groups * 16), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((paged_attn_join_kernel<P, D, 128, P::IS_BF16 ? 64 : TileCfg<D>::KT, RPB>), dim3((unsigned)groups * (128 / RPB)), dim3(256), 0, s, a);
+    if (p.step) hipLaunchKernelGGL((paged_attn_join_kernel<P, D, 16, StepCfg<P, D>::KT, 1>), dim3((unsigned)groups * 16), dim3(256), 0, s, a);
+    else if constexpr (P::IS_BF16) hipLaunchKernelGGL((paged_attn_join_kernel<P, D, 128, 64, RPB>), dim3((unsigned)groups * (128 / RPB)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((paged_attn_join_kernel<P, D, 64, 32, RPB>), dim3((unsigned)groups * (64 / RPB)), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t paged_attn_workspace(const PagedAttnArgs& a, int max_new, int head_dim, int) {
-    const Plan p = make_plan(a, max_new, head_dim);
+int64_t paged_attn_workspace(const PagedAttnArgs& a, int max_new, int head_dim, int dtype) {
+    const Plan p = make_plan(a, max_new, head_dim, dtype);
     return p.splits == 1 ? 0 : (PART_HEAD + (int64_t)p.splits * a.tokens * a.q_heads * (head_dim + 2)) * (int64_t)sizeof(float);
 }
 
