@@ -1130,15 +1130,32 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
     float sum = 0.f;
     if constexpr (RPB > 1) {
         float top = -INFINITY;
-        for (int s = 0; s < splits; ++s) top = fmaxf(top, part_ml<D>(a, s, orow)[0]);
-        const float mu = top == -INFINITY ? 0.f : top;
-        for (int s = 0; s < splits; ++s) {
-            const float* ml = part_ml<D>(a, s, orow);
-            const float f = ml[1] == 0.f ? 0.f : exp2_hw(ml[0] - mu);
-            sum = fmaf(ml[1], f, sum);
-            const f32x4 x = *reinterpret_cast<const f32x4*>(part_out<D>(a, s, orow) + piece * 4);
+        for (int s0 = 0; s0 < splits; s0 += 8) {       // eight shares in one round trip
+            float m[8], l[8];
+            f32x4 x[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = f == 0.f ? acc[i] : fmaf(x[i], f, acc[i]);
+            for (int u = 0; u < 8; ++u) {
+                const int s = min(s0 + u, splits - 1);
+                const float* ml = part_ml<D>(a, s, orow);
+                m[u] = ml[0];
+                l[u] = s0 + u < splits ? ml[1] : 0.f;
+                x[u] = *reinterpret_cast<const f32x4*>(part_out<D>(a, s, orow) + piece * 4);
+            }
+            float next = top;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) next = fmaxf(next, m[u]);
+            const float mu = next == -INFINITY ? 0.f : next, keep = exp2_hw(top - mu);
+            top = next;
+            sum *= keep;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = keep == 0.f ? 0.f : acc[i] * keep;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float f = l[u] == 0.f ? 0.f : exp2_hw(m[u] - mu);
+                sum = fmaf(l[u], f, sum);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] = f == 0.f ? acc[i] : fmaf(x[u][i], f, acc[i]);
+            }
         }
     } else {
         float m = -INFINITY, l = 0.f;
@@ -1191,7 +1208,7 @@ Plan make_plan(const PagedAttnArgs& a, int max_new, int head_dim, int dtype) {
     const bool full = est * a.kv_heads >= SLOTS;
     p.min_share = 32768 / row_of_cache < 32 ? 32 : 32768 / row_of_cache;    // 32 KiB of keys: 256 rows of 64 in bf16, 64 of 128 in f32
     int64_t s = keys / p.min_share;
-    if (keys <= (p.step ? (full ? 4096 : 1024) : p.min_share * (full ? 8 : 2))) s = 1;
+    if (keys <= (p.step ? (full ? 4096 : 1024) : dtype == PTTS_BF16 ? (full ? 2048 : 1024) : p.min_share * (full ? 8 : 2))) s = 1;
     if (s > MAX_SPLITS) s = MAX_SPLITS;
     if (s > ((int64_t)128 << 20) / row_bytes) s = ((int64_t)128 << 20) / row_bytes;
     p.splits = s < 2 ? 1 : (int)s;
