@@ -222,11 +222,12 @@ template <int M, int KT, bool SORTED> struct Schedule {
             if ((float)most > lag * mean) {
                 // a slot's part of everything; a little more where the shares' ends would need a second round of a few workgroups
                 const int least = max(a.min_share / KT, (most + a.splits - 1) / a.splits);
+                const int front = a.causal ? min((past + KT) / KT, key_tiles(a)) : key_tiles(a);       // tiles the first row sees
                 for (int step = 4; step <= 8; ++step) {
                     share = max((int)ceilf(mean * 0.25f * (float)step), least);
                     if (a.n_seqs > 64 || step == 8) break;
-                    const int all = uniform(__builtin_amdgcn_readlane(scan_add(row_tiles(a) * shares(key_tiles(a))), 63));
-                    if (all * a.kv_heads <= SLOTS) break;
+                    const int all = uniform(__builtin_amdgcn_readlane(scan_add(row_tiles(a) * (shares(key_tiles(a)) + shares(front))), 63));
+                    if (all * a.kv_heads <= 2 * SLOTS) break;
                 }
             }
             share = uniform(share);
@@ -487,8 +488,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk_kernel(PagedAttnArgs 
 
     Schedule<C::M, KT, true> sched;
     begin(a, sched, TILE_LAG);
-    const int item = blockIdx.x;
-    if (item >= sched.items * a.kv_heads) return;
+    const int all = sched.items * a.kv_heads;
+    int item = blockIdx.x;
+    if (item >= all) return;
+    if (all > SLOTS / 2 && all <= SLOTS && item >= SLOTS / 2) item = all - 1 - (item - SLOTS / 2);
     // consecutive workgroups go to consecutive XCDs: with the key head innermost, an XCD's L2 holds few heads' pages
     const int at = int_div(item, a.by_kv_heads), kvh = item - at * a.kv_heads;
     Item it;
@@ -1205,10 +1208,12 @@ Plan make_plan(const PagedAttnArgs& a, int max_new, int head_dim, int dtype) {
     if (est > ub) est = ub;
     // most shares of a tile: none where the keys a workgroup could be left with alone take less time than joining; 128 MiB of partial results
     const int64_t keys = (int64_t)a.max_pages << a.page_shift, row_bytes = (int64_t)a.tokens * a.q_heads * (head_dim + 2) * 4;
-    const bool full = est * a.kv_heads >= SLOTS;
     p.min_share = 32768 / row_of_cache < 32 ? 32 : 32768 / row_of_cache;    // 32 KiB of keys: 256 rows of 64 in bf16, 64 of 128 in f32
     int64_t s = keys / p.min_share;
-    if (keys <= (p.step ? (full ? 4096 : 1024) : dtype == PTTS_BF16 ? (full ? 2048 : 1024) : p.min_share * (full ? 8 : 2))) s = 1;
+    const int64_t items = est * a.kv_heads, idle = items < 160 ? 256 - items : 0;
+    const int64_t alone = p.step ? 65536 / row_of_cache : dtype == PTTS_BF16 ? 512 : p.min_share * 2;
+    const int64_t limit = p.step ? 4096 : dtype == PTTS_BF16 ? 2048 : p.min_share * 8;
+    if (keys <= limit && keys * idle <= alone * 256) s = 1;
     if (s > MAX_SPLITS) s = MAX_SPLITS;
     if (s > ((int64_t)128 << 20) / row_bytes) s = ((int64_t)128 << 20) / row_bytes;
     p.splits = s < 2 ? 1 : (int)s;
