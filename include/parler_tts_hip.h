@@ -302,7 +302,7 @@ enum {
 typedef struct ptts_paged_kv {
     void* k;
     void* v;
-    int64_t k_strides[3], v_strides[3];    /* page, head, slot; every row starts at a multiple of 16 bytes */
+    int64_t k_strides[3], v_strides[3];    /* page, head, slot (< 128 MiB); every row starts at a multiple of 16 bytes */
     int32_t dtype;                         /* PTTS_DTYPE_* */
     int32_t n_pages, kv_heads;
     int32_t page_tokens;                   /* power of two, 16 .. 4096 */
@@ -312,7 +312,7 @@ typedef struct ptts_paged_kv {
 /* new tokens of n_seqs sequences, one behind the other: tokens starts[s] .. starts[s + 1] - 1 are sequence s's (starts NULL: one each) */
 typedef struct ptts_paged_batch {
     const int32_t* table;                  /* [n_seqs][table_stride]: page ids of the slots 0 .. of every sequence */
-    int64_t table_stride;
+    int64_t table_stride;                  /* >= max_pages; attention only: 0 = one row for all */
     const int32_t* past;                   /* [n_seqs]: tokens in the cache before these */
     const int32_t* starts;                 /* [n_seqs + 1] ascending, or NULL */
     int32_t max_pages;                     /* used width of the table */
@@ -335,7 +335,7 @@ int ptts_rotary_embed(const ptts_rotary* rot, int32_t dtype, int32_t tokens, int
 /* Token i of sequence s goes to slot past[s] + i: k turned by `rot` (NULL: as it is) at its slot, or at positions[token] where
  * positions is given; v as it is.  q (optional: q_heads > 0) is turned at the same positions into q_out, which may be q.
  * dtype is that of k, v and q; f32 rows may go into a bf16 cache (rounded once, behind the rotation).  A token that cannot be placed
- * leaves the cache as it is and its row of q_out becomes zero. */
+ * leaves the cache as it is and its row of q_out becomes zero; rows behind the last sequence are left as they are. */
 int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, int32_t dtype, const void* k, int64_t k_token_stride,
                    int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, const ptts_rotary* rot,
                    const int32_t* positions, int32_t q_heads, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
@@ -343,8 +343,8 @@ int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, in
 
 /* out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j].  causal: token i of sequence s sees the keys 0 .. past[s] + i (the new tokens are in
  * the cache); else all of 0 .. past[s] - 1 (encoder states, say).  key_mask [n_seqs][mask_stride] bytes: keys j < mask_width with a zero
- * are no keys; whatever they hold does not reach the output.  A token that sees no key gets zeros; rows that a bad page, length or start
- * concerns get NaN.  Query head h reads key head h / (q_heads / kv_heads).  q, out: [tokens][q_heads][head_dim] of the cache's type.
+ * are no keys; whatever they hold does not reach the output.  A token that sees no key gets zeros; rows that a bad page or length concerns
+ * get NaN; rows of no sequence (behind the last, or where starts are wrong) are left as they are.  Query head h reads key head h / (q_heads / kv_heads).  q, out: [tokens][q_heads][head_dim] of the cache's type.
  * max_new: an upper bound of the new tokens of one sequence, 0 = not known; it picks the kernel, never the result's validity.
  * workspace: ptts_paged_attention_workspace() bytes (may be 0; negative = PTTS_E_*) at a multiple of 16, not shared with another call
  * in flight. */

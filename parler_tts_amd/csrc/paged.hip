@@ -290,12 +290,13 @@ int check_kv(const ptts_paged_kv* c) {
     return PTTS_OK;
 }
 
-int check_batch(const ptts_paged_batch* b) {
+int check_batch(const ptts_paged_batch* b, bool written) {
     if (!b) REFUSE(PTTS_E_INVALID, "null batch");
     if (b->n_seqs < 0 || b->tokens < 0 || b->max_pages < 0) REFUSE(PTTS_E_INVALID, "negative batch sizes");
     if (b->n_seqs > 0 && (!b->past || (!b->table && b->max_pages > 0))) REFUSE(PTTS_E_INVALID, "null page table or lengths");
     if (!b->starts && b->tokens != b->n_seqs) REFUSE(PTTS_E_INVALID, "%d tokens of %d sequences need starts", b->tokens, b->n_seqs);
-    if (b->table_stride < b->max_pages) REFUSE(PTTS_E_INVALID, "page table rows overlap");
+    // sequences may read the same row of pages; where they write, no two of them own a slot
+    if (b->table_stride < b->max_pages && (written || b->table_stride != 0)) REFUSE(PTTS_E_INVALID, "page table rows overlap");
     if ((int64_t)b->table_stride > INT_MAX) REFUSE(PTTS_E_INVALID, "page table stride out of range");
     return PTTS_OK;
 }
@@ -373,7 +374,7 @@ int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, in
                    const int32_t* positions, int32_t q_heads, const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
                    int64_t q_out_token_stride, int64_t q_out_head_stride, int32_t* status, void* stream) {
     TRY(check_kv(cache));
-    TRY(check_batch(batch));
+    TRY(check_batch(batch, true));
     if (!status) REFUSE(PTTS_E_INVALID, "null status");
     if (dtype != PTTS_DTYPE_F32 && dtype != PTTS_DTYPE_BF16) REFUSE(PTTS_E_INVALID, "dtype must be 0 (f32) or 1 (bf16)");
     if (dtype == PTTS_DTYPE_BF16 && cache->dtype != PTTS_DTYPE_BF16) REFUSE(PTTS_E_UNSUPPORTED, "bf16 rows into an f32 cache");
@@ -407,7 +408,7 @@ int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, in
 namespace {
 int attn_args(const ptts_paged_kv* cache, const ptts_paged_batch* batch, int32_t q_heads, int32_t max_new, PagedAttnArgs* a) {
     TRY(check_kv(cache));
-    TRY(check_batch(batch));
+    TRY(check_batch(batch, false));
     if (q_heads <= 0 || q_heads % cache->kv_heads) REFUSE(PTTS_E_INVALID, "%d query heads over %d key heads", q_heads, cache->kv_heads);
     if (q_heads > 65535) REFUSE(PTTS_E_UNSUPPORTED, "%d query heads", q_heads);
     if (max_new < 0) REFUSE(PTTS_E_INVALID, "max_new %d", max_new);

@@ -191,3 +191,15 @@ def test_public_names():
 
     for name in ("PagedKVCache", "RotaryTable", "rotary_embed", "kv_append", "paged_attention"):
         assert hasattr(p, name)
+
+
+def test_the_matrix_instructions_of_the_attention_kernels_are_guarded_and_waited_for():
+    """on the assembly that hipcc makes of them: no product under EXEC masking alone, no result read by inline assembly too early"""
+    import importlib.util
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    for name in ("check_mfma_guards", "check_mfma_asm_hazard"):
+        spec = importlib.util.spec_from_file_location(name, os.path.join(root, "tools", name + ".py"))
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        assert mod.main([os.path.join(root, "parler_tts_amd", "csrc", "paged_attn.hip")]) == 0
