@@ -110,7 +110,8 @@ class ParlerTTSDecoderConfig(_ConfigBase):
         # ("unpinned"); the defaults are the reference's ops.
         #   norm_type          "layer_norm" | "rms_norm"  (x * rsqrt(mean(x^2) + 1e-5) * weight; the bias tensors are ignored)
         #   position_embedding "sinusoidal" | "rope"      (no additive table; q, k of the SELF-attention rotated per head,
-        #                                                  pairs (i, i + head_dim / 2), angle pos * rope_theta^(-2 i / head_dim))
+        #                                                  pairs (i, i + head_dim / 2), angle pos * rope_theta^(-2 i / head_dim),
+        #                                                  stretched by rope_scaling: paged.rotary_frequencies)
         #   mlp_type           "gelu" | "swiglu"          (fc2(silu(fc1(x)) * fc1_up(x)); extra tensor layers.{l}.fc1_up.weight)
         self.norm_type = kwargs.pop("norm_type", "layer_norm")
         self.position_embedding = kwargs.pop("position_embedding", "sinusoidal")
@@ -119,7 +120,14 @@ class ParlerTTSDecoderConfig(_ConfigBase):
         if self.norm_type not in ("layer_norm", "rms_norm") or self.position_embedding not in ("sinusoidal", "rope") or \
                 self.mlp_type not in ("gelu", "swiglu"):
             raise ValueError("norm_type / position_embedding / mlp_type: unknown variant")
+        if self.position_embedding == "rope" and kwargs.get("rope_scaling") is not None:
+            from .paged import rotary_frequencies
+
+            self.rope_scaling = dict(kwargs.pop("rope_scaling"))
+            rotary_frequencies(self.head_dim, self.rope_theta, self.rope_scaling)      # raises on what it does not know
         self._extra = {k: v for k, v in kwargs.items() if not k.startswith("_")}
+
+    rope_scaling: Optional[Dict[str, Any]] = None       # {"type": "linear" | "ntk" | "yarn", "factor": s, ...}: contexts beyond the trained ones
 
     def to_dict(self):
         d = super().to_dict()

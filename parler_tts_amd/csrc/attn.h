@@ -70,5 +70,6 @@ hipError_t attn_init();
 hipError_t attn_decode_launch(const AttnArgs& a, int B, int H, int cache_dtype, int out_dtype, hipStream_t stream,
                               hipEvent_t ev_start = nullptr, hipEvent_t ev_stop = nullptr);
 // causal self-attention of a prefill chunk (a.npos positions per utterance, B utterances): one wave per query row
+bool attn_causal_fits(int positions);      // whether the score rows of this many cached positions fit the LDS
 hipError_t attn_causal_launch(const AttnArgs& a, int B, int H, int cache_dtype, int out_dtype, hipStream_t stream);
 hipError_t attn_full_launch(const FullAttnArgs& a, int B, int out_dtype, hipStream_t stream);

@@ -293,11 +293,13 @@ hipError_t attn_decode_launch(const AttnArgs& a, int B, int H, int cache_dtype, 
     return hipGetLastError();
 }
 
+bool attn_causal_fits(int positions) { return (size_t)NWAVES * ((positions + 3) & ~3) * sizeof(float) <= 160 * 1024; }
+
 hipError_t attn_causal_launch(const AttnArgs& a, int B, int H, int cache_dtype, int out_dtype, hipStream_t stream) {
     if (a.npos <= 0) return hipErrorInvalidValue;
     const int s_max = (a.pos0 + a.npos + 3) & ~3;
     const size_t lds = (size_t)NWAVES * s_max * sizeof(float);
-    if (lds > 160 * 1024) return hipErrorInvalidValue;
+    if (!attn_causal_fits(a.pos0 + a.npos)) return hipErrorInvalidValue;
     dim3 grid(H, B, (a.npos + NWAVES - 1) / NWAVES), block(NWAVES * 64);
     if (cache_dtype == PTTS_BF16) {
         if (out_dtype == PTTS_BF16) hipLaunchKernelGGL((attn_causal_kernel<PBF16, PBF16>), grid, block, lds, stream, a, s_max);

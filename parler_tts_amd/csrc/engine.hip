@@ -98,6 +98,8 @@ struct Work {
     void *attn_frag = nullptr, *mlp_frag = nullptr, *x_frag = nullptr, *x_frag2 = nullptr;
     float* ffn_raw = nullptr;   // SwiGLU variant only: [rows][2 F] gate | up pre-activations
     int rows = 0;      // capacity (multiple of 32)
+    void* far = nullptr;        // batched prefill behind attn_causal_kernel's reach: workspace of long_prefill_launch
+    int64_t far_bytes = 0;
 };
 
 }  // namespace
@@ -419,6 +421,16 @@ void dump_allocs(const ptts_engine* e) {
     fclose(f);
 }
 
+LongPrefillArgs far_args(const ptts_engine* e, const Work& wk, int layer, int B, int npos, int pos0) {
+    const ptts_config& c = e->cfg;
+    LongPrefillArgs a = {};
+    a.q = wk.q; a.ldq = e->v_rope ? 2 * c.hidden : c.hidden; a.pool = make_pool(e, false); a.layer = layer;
+    a.bias = e->has_self_bias ? e->self_bias : nullptr; a.ld_bias = e->s_cap;
+    a.ofrag = wk.attn_frag; a.D = c.hidden; a.H = c.heads; a.B = B; a.npos = npos; a.pos0 = pos0;
+    if (e->v_rope) { a.cos_t = e->rope_cos; a.sin_t = e->rope_sin; a.positions = c.max_positions; }
+    return a;
+}
+
 int run_layers(ptts_engine* e, hipStream_t s, bool profile, const Work& wk, int M, int npos = 0, int pos0 = 0) {
     const ptts_config& c = e->cfg;
     const int D = c.hidden, F = c.ffn;
@@ -456,11 +468,13 @@ int run_layers(ptts_engine* e, hipStream_t s, bool profile, const Work& wk, int 
         // the kernel-by-kernel debug gate (a pass cut short would leave arrival tags without their attention)
         const bool fuse = qkv_built && npos == 0 && !e->v_rope && e->dbg_stop < 0 && e->fuse_qkv_attn && e->fuse_arrive &&
                           (size_t)c.layers * ((M + 31) / 32) * c.heads * 32 <= e->fuse_arrive_ints && fused_qkv_attn_supported(g, a, e->dt);
+        // a chunk whose score rows do not fit the LDS: the operators over a paged cache (the rotation of the rotary variant among them)
+        const bool far = npos > 0 && !attn_causal_fits(pos0 + npos);
         if (qkv_built && !fuse) {
             DBG_GATE(e);
             STAMP_ARGS(e, g);
             PTTS_TRY(launch_gemm(e, g, s));
-            if (e->v_rope) {
+            if (e->v_rope && !far) {
                 RopeArgs ra;
                 ra.qk = wk.q; ra.ld = 2 * D; ra.D = D; ra.H = c.heads; ra.rows = M; ra.pool = make_pool(e, false); ra.layer = l;
                 ra.state = e->state; ra.npos = npos; ra.pos0 = pos0; ra.cos_t = e->rope_cos; ra.sin_t = e->rope_sin;
@@ -482,6 +496,8 @@ int run_layers(ptts_engine* e, hipStream_t s, bool profile, const Work& wk, int 
             int v = gemm_validate(g, e->dt);
             if (v != 0) return fail(PTTS_E_INVALID, "gemm shape rejected (code %d): M=%d N=%d K=%d pro=%d epi=%d", v, g.M, g.N, g.K, g.pro, g.epi);
             HIP_TRY(fused_qkv_attn_launch(g, a, M, c.heads, e->dt, e->fuse_arrive, e->fuse_err, s, ep ? ep->a : nullptr, ep ? ep->b : nullptr, e->fuse_blackhole));
+        } else if (far) {
+            HIP_TRY(long_prefill_launch(far_args(e, wk, l, B_utt, npos, pos0), e->dt, wk.far, wk.far_bytes, s));
         } else if (npos > 0) {
             a.npos = npos; a.pos0 = pos0;
             HIP_TRY(attn_causal_launch(a, B_utt, c.heads, e->dt, e->dt, s));
@@ -1086,7 +1102,7 @@ int ptts_destroy(ptts_engine* e) {
     drop_graph(e);
     if (e->dac_buf0) (void)hipFree(e->dac_buf0);
     if (e->dac_buf1) (void)hipFree(e->dac_buf1);
-    for (void* p : {(void*)e->pf.x, (void*)e->pf.q, (void*)e->pf.xstat, (void*)e->pf.ffn_raw, e->pf.attn_frag, e->pf.mlp_frag, e->pf.x_frag, e->pf.x_frag2})
+    for (void* p : {(void*)e->pf.x, (void*)e->pf.q, (void*)e->pf.xstat, (void*)e->pf.ffn_raw, e->pf.attn_frag, e->pf.mlp_frag, e->pf.x_frag, e->pf.x_frag2, e->pf.far})
         if (p) (void)hipFree(p);
 #ifdef PTTS_STAMPS
     if (e->stamps) (void)hipFree(e->stamps);
@@ -1407,7 +1423,10 @@ int ptts_prefill(ptts_engine* e, int32_t B, int32_t B_eff, int32_t T, int32_t P,
             Work& w = e->pf;
             for (void* p : {(void*)w.x, (void*)w.q, (void*)w.xstat, w.attn_frag, w.mlp_frag, w.x_frag, w.x_frag2, (void*)w.ffn_raw})
                 if (p) (void)hipFree(p);
+            void* const far = w.far;
+            const int64_t far_bytes = w.far_bytes;
             w = Work();
+            w.far = far; w.far_bytes = far_bytes;
             const size_t D_ = c.hidden, F_ = c.ffn, R = need_rows;
             bool ok = hipMalloc((void**)&w.x, sizeof(float) * R * D_) == hipSuccess &&
                       hipMalloc((void**)&w.q, sizeof(float) * R * D_ * (e->v_rope ? 2 : 1)) == hipSuccess &&
@@ -1425,6 +1444,23 @@ int ptts_prefill(ptts_engine* e, int32_t B, int32_t B_eff, int32_t T, int32_t P,
             HIP_TRY(hipMemsetAsync(w.x_frag, 0, e->esz * R * D_, s));
             HIP_TRY(hipMemsetAsync(w.x_frag2, 0, e->esz * R * D_, s));
             HIP_TRY(hipMemsetAsync(w.x, 0, sizeof(float) * R * D_, s));
+        }
+        if (!attn_causal_fits(total)) {       // the chunks' needs, then one allocation
+            int64_t need = 0;
+            auto look = [&](int pos0, int npos) {
+                if (attn_causal_fits(pos0 + npos)) return;
+                const int64_t n = long_prefill_workspace(far_args(e, e->pf, 0, B_eff, npos, pos0), e->dt);
+                if (n > need) need = n;
+            };
+            for (int p0 = 0; p0 < P; p0 += chunk) look(p0, (P - p0 < chunk) ? P - p0 : chunk);
+            for (int j0 = 0; j0 < n_prefix; j0 += chunk) look(P + j0, (n_prefix - j0 < chunk) ? n_prefix - j0 : chunk);
+            if (need > e->pf.far_bytes) {
+                HIP_TRY(hipStreamSynchronize(s));
+                if (e->pf.far) (void)hipFree(e->pf.far);
+                e->pf.far = nullptr; e->pf.far_bytes = 0;
+                if (hipMalloc(&e->pf.far, need) != hipSuccess) return fail(PTTS_E_NOMEM, "%lld bytes for a prefill of %d positions", (long long)need, total);
+                e->pf.far_bytes = need;
+            }
         }
         const Work& wk = e->pf;
         auto run_chunk = [&](int pos0, int npos, bool prompt_rows) -> int {

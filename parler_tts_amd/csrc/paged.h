@@ -40,7 +40,7 @@ struct RotaryEmbedArgs {
 };
 
 struct AppendArgs {
-    const void *q, *k, *v;
+    const void *q, *k, *v;                   // v null: it is in the cache already
     void *q_out, *k_cache, *v_cache;
     int64_t qs[2], qos[2], ks[2], vs[2];     // token, head
     int64_t kc[3], vc[3];                    // page, head, slot
@@ -86,3 +86,15 @@ hipError_t kv_append_launch(const AppendArgs& a, int in_dtype, int cache_dtype, 
 // rows of one sequence never exceed max_new * group; the choice of kernel and split follows from it and from max_pages
 int64_t paged_attn_workspace(const PagedAttnArgs& a, int max_new, int head_dim, int dtype);
 hipError_t paged_attn_launch(const PagedAttnArgs& a, int max_new, int head_dim, int dtype, hipStream_t s);
+
+// the engine's own long prefill through these operators (long_prefill.hip): npos positions from pos0 on of B utterances
+struct LongPrefillArgs {
+    float* q;                // [B * npos][ldq] fp32, scaled; rotary variant: q | k, unturned
+    KVPool pool;
+    const float* bias;       // additive mask [B][ld_bias] (0 / finfo.min) or null
+    void* ofrag;             // B fragments, feature count D
+    const float *cos_t, *sin_t;   // rotary variant: [positions][32]; null: k is in the cache
+    int ldq, layer, ld_bias, D, H, B, npos, pos0, positions;
+};
+int64_t long_prefill_workspace(const LongPrefillArgs& a, int dtype);
+hipError_t long_prefill_launch(const LongPrefillArgs& a, int dtype, void* workspace, int64_t workspace_bytes, hipStream_t s);

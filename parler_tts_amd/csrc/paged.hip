@@ -214,11 +214,11 @@ hipError_t rotary_embed_launch(const RotaryEmbedArgs& a, int dtype, hipStream_t 
 hipError_t kv_append_launch(const AppendArgs& a, int in_dtype, int cache_dtype, hipStream_t s) {
     const int esz = in_dtype == PTTS_BF16 ? 2 : 4, full = 16 / esz;
     const int csz = cache_dtype == PTTS_BF16 ? 2 : 4;
-    bool wide = a.rot.dims % (2 * full) == 0 && a.head_dim % (2 * full) == 0 && aligned(a.k, a.ks, 2, 16, esz) && aligned(a.v, a.vs, 2, 16, esz) &&
+    bool wide = a.rot.dims % (2 * full) == 0 && a.head_dim % (2 * full) == 0 && aligned(a.k, a.ks, 2, 16, esz) && (!a.v || aligned(a.v, a.vs, 2, 16, esz)) &&
                 aligned(a.k_cache, a.kc, 3, full * csz, csz) && aligned(a.v_cache, a.vc, 3, full * csz, csz);
     if (a.q_heads) wide = wide && aligned(a.q, a.qs, 2, 16, esz) && aligned(a.q_out, a.qos, 2, 16, esz);
     if (a.rot.cos_t) wide = wide && aligned(a.rot.cos_t, nullptr, 0, 16, 4) && aligned(a.rot.sin_t, nullptr, 0, 16, 4);
-    const UnitMap m = make_map(a.q_heads + 2 * a.kv_heads, a.head_dim, a.rot.dims, wide ? full : 1, a.b.tokens, APPEND_TOKENS);
+    const UnitMap m = make_map(a.q_heads + (a.v ? 2 : 1) * a.kv_heads, a.head_dim, a.rot.dims, wide ? full : 1, a.b.tokens, APPEND_TOKENS);
     const dim3 grid((a.b.tokens + m.tokens_per_block - 1) / m.tokens_per_block), block(256);
 #define LAUNCH(T, TC, N)                                                                                      \
     do {                                                                                                      \

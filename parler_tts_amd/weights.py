@@ -44,9 +44,16 @@ def sinusoid_table(num_positions: int, dim: int) -> torch.Tensor:
 def rope_tables(cfg: ParlerTTSDecoderConfig, num_positions: int = 0):
     """(cos, sin), each [positions, head_dim / 2] fp32, of the rotary-position VARIANT (configuration.py: an extension with no
     counterpart in the reference): angle(pos, i) = pos * rope_theta^(-2 i / head_dim), every step in fp32.  The engine and the
-    fp32 PyTorch statement in oracle/cpu_ref.py both read these tables, so they rotate by bit-identical angles."""
+    fp32 PyTorch statement in oracle/cpu_ref.py both read these tables, so they rotate by bit-identical angles.  With
+    cfg.rope_scaling: the angles of paged.rotary_frequencies, formed in 64 bits (positions are far, there) and rounded once."""
     hd = cfg.hidden_size // cfg.num_attention_heads
     n = num_positions or cfg.max_position_embeddings
+    if getattr(cfg, "rope_scaling", None):
+        from .paged import rotary_frequencies
+
+        freq, gain = rotary_frequencies(hd, float(cfg.rope_theta), cfg.rope_scaling)
+        ang = torch.arange(n, dtype=torch.float64)[:, None] * freq
+        return (torch.cos(ang) * gain).float(), (torch.sin(ang) * gain).float()
     inv = torch.pow(torch.tensor(float(cfg.rope_theta), dtype=torch.float32), -torch.arange(0, hd, 2, dtype=torch.float32) / hd)
     ang = torch.arange(n, dtype=torch.float32)[:, None] * inv[None, :]
     return torch.cos(ang), torch.sin(ang)

@@ -203,3 +203,23 @@ def test_the_matrix_instructions_of_the_attention_kernels_are_guarded_and_waited
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
         assert mod.main([os.path.join(root, "parler_tts_amd", "csrc", "paged_attn.hip")]) == 0
+
+
+def test_a_decoder_configuration_carries_its_rotary_scaling():
+    from parler_tts_amd.configuration import ParlerTTSDecoderConfig, tiny_config
+    from parler_tts_amd.weights import rope_tables
+
+    scaling = {"type": "linear", "factor": 4.0}
+    cfg = tiny_config(position_embedding="rope", rope_scaling=scaling).decoder
+    assert ParlerTTSDecoderConfig.from_dict(cfg.to_dict()) == cfg and cfg.rope_scaling == scaling
+    cos, sin = rope_tables(cfg, 9)
+    freq, gain = rotary_frequencies(64, 10000.0, scaling=scaling)
+    angle = torch.arange(9, dtype=torch.float64)[:, None] * freq
+    assert torch.equal(cos, (torch.cos(angle) * gain).float()) and torch.equal(sin, (torch.sin(angle) * gain).float())
+    plain = tiny_config(position_embedding="rope").decoder
+    assert "rope_scaling" not in plain.to_dict()
+    inv = torch.pow(torch.tensor(10000.0), -torch.arange(0, 64, 2, dtype=torch.float32) / 64)
+    assert torch.equal(rope_tables(plain, 9)[0], torch.cos(torch.arange(9, dtype=torch.float32)[:, None] * inv))
+    with pytest.raises(ValueError, match="type"):
+        tiny_config(position_embedding="rope", rope_scaling={"type": "dynamic", "factor": 2.0})
+    assert tiny_config(rope_scaling=scaling).decoder.rope_scaling is None      # no rotary positions: kept as an unknown entry, as before
