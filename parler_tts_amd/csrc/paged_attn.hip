@@ -472,13 +472,13 @@ template <> __device__ __forceinline__ void store4<PF32>(float* p, float a, floa
 template <int D> struct ChunkCfg {
     static constexpr int M = 128, NW = 4, KT = 64, RB = D * 2;
     static constexpr int TILE = KT * RB;
-    static constexpr int NB = 65536 / (2 * TILE);              // 64 KiB of LDS: two workgroups on a CU
+    static constexpr int NB = D == 64 ? 3 : 65536 / (2 * TILE);             // 64 KiB of LDS: two workgroups on a CU
     static constexpr int LDS = 2 * NB * TILE;                  // [K ring][V ring]
     static constexpr int DMA = TILE / NW / 1024;               // LDS-DMA instructions per wave and tile of K or of V
 };
 
 template <int D>
-__global__ __launch_bounds__(256, 2) void paged_attn_chunk_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(256, (D == 64 ? 3 : 2)) void paged_attn_chunk_kernel(PagedAttnArgs a) {
     typedef PBF16 P;
     typedef uint16_t elem_t;
     typedef ChunkCfg<D> C;
@@ -588,7 +588,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk_kernel(PagedAttnArgs 
         }
         buf = knext;
         unsigned dma_lane = lane;
-        asm volatile("" : "+v"(dma_lane));   // the lane offsets of the transfers are computed anew (8 registers)
+        if constexpr (D == 128) asm volatile("" : "+v"(dma_lane));   // the lane offsets of the transfers are computed anew (8 registers)
         if (key0 >= w_end) {                 // nothing here for this wave's rows (it keeps moving its share of the tiles)
             if constexpr (FULL) {
                 each<0, C::DMA>([&](auto I) { krows.template fetch_one<decltype(I)::value>(ksrc, ksend, dma_lane); });
@@ -598,7 +598,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_chunk_kernel(PagedAttnArgs 
         }
         // operand fragments from LDS, AHEAD steps ahead: K of the next tile (steps 0 .. NQ - 1), then V of this one.  (The step is xor-ed into
         // the whole address, not into its lane part: that would be 16 registers kept.)
-        constexpr int RING = D == 64 ? 8 : 6, AHEAD = RING - 1;
+        constexpr int RING = D == 64 ? 4 : 6, AHEAD = RING - 1;
         bf16x8 fr[RING];
         const unsigned kat = kt + ka, vat = vt + va, vbt = vt + vb;
         auto fragment = [&](int u) {
