@@ -1,6 +1,7 @@
 // Attention of new tokens over a paged KV cache: o_i = sum_j softmax_j(scale * q_i . k_j) v_j over the keys j a query may see.
 //
-// Both kernels make ONE pass over the keys with the running maximum and sum of the softmax, and both hold the scores TRANSPOSED:
+// Three kernels (chunks in bf16, chunks in f32, few rows) make ONE pass over the keys with the running maximum and sum of the softmax, and
+// all hold the scores TRANSPOSED:
 // S^T = K Q^T puts a query into a column, so that a lane owns one query and a few of its scores; the maximum is a register maximum
 // plus one or two lane swaps, the running state is one register per lane, and the probabilities are already the B operand of
 // O^T = V^T P^T when the keys of a matrix step are numbered as the accumulator left them (key 8 (j / 4) + 4 h + j % 4 in slot j of
@@ -136,9 +137,10 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // A launch's items are (tile of M rows of a sequence, share of its keys, key head).  Their numbers come from the lengths on the device:
 // every wave sums the sequences' tiles up for itself, 64 sequences at a time, all lengths in one round trip.  Items are numbered without
 // holes (with holes between the sequences the dispatcher put all work of equal chunks on half of the CUs).
-// Keys are shared out only where that evens the load: SLOTS workgroups run at a time, and a tile whose keys exceed what one of them would
-// get of everything (by the factor LAG) is cut into shares of that size, at least min_share keys each (a share costs its rows' f32 partial
-// results, written and read once more).
+// Keys are shared out only where that evens the load: a tile whose keys exceed what one of SLOTS workgroups would get of everything (by the
+// factor LAG) is cut into shares of that size, at least min_share keys each (a share costs its rows' f32 partial results, written and read
+// once more).  SLOTS are two workgroups on each of 256 CUs.  Counting the third that head dim 64 has room for made finer shares and lost
+// more at their ends than it won: prompts of up to 7770 over 2324 keys, 2 heads of 64: 68 us, with two 58; a batch of 24 chunks 81, 76.
 constexpr int SLOTS = 512, MAX_SPLITS = 256;
 constexpr float TILE_LAG = 2.f, STEP_LAG = 2.f;
 
@@ -469,10 +471,16 @@ template <> __device__ __forceinline__ void store4<PF32>(float* p, float a, floa
 // V, so each has a ring of its own: iteration i sends for K(i + NB) and V(i + NB - 1) into the buffers that iteration i - 1 left, one
 // instruction between two products.  Iterations with less in front of the end are written out apart: they wait for all in flight.
 // =================================================================================================================================
+// Three workgroups on a CU at head dim 64 (48 KiB, 168 registers: four fragments read ahead), two at 128 (64 KiB, 248 registers).
+// Bound: at head dim 128 the matrix unit, under a power limit (prompt of 8191 tokens, 16 heads over 4: 280 - 294 us, 935 - 980 TFLOP/s, where
+// the library's product of 8192^3 reaches 1162 - 1202); at 64 the vector unit beside it (per tile and wave 32 exponentials, 130 other
+// operations, 16 products: 8191 tokens, 16 heads: 182 us, 755 TFLOP/s; with two workgroups on a CU 199).  Short chunks: a workgroup's start
+// (lengths, page ids and first tiles are three dependent trips to memory, 5.6 us) and the unequal lengths.
+// Tried and left: the sum of the weights by the matrix unit or by two-element dot products (no change); 64 rows a wave (registers).
 template <int D> struct ChunkCfg {
     static constexpr int M = 128, NW = 4, KT = 64, RB = D * 2;
     static constexpr int TILE = KT * RB;
-    static constexpr int NB = D == 64 ? 3 : 65536 / (2 * TILE);             // 64 KiB of LDS: two workgroups on a CU
+    static constexpr int NB = D == 64 ? 3 : 2;
     static constexpr int LDS = 2 * NB * TILE;                  // [K ring][V ring]
     static constexpr int DMA = TILE / NW / 1024;               // LDS-DMA instructions per wave and tile of K or of V
 };
@@ -491,6 +499,7 @@ __global__ __launch_bounds__(256, (D == 64 ? 3 : 2)) void paged_attn_chunk_kerne
     const int all = sched.items * a.kv_heads;
     int item = blockIdx.x;
     if (item >= all) return;
+    // up to two on a CU: the longest item beside the shortest (4 prompts of 1024, 16 heads of 128 over 2: 34 us, in order 41)
     if (all > SLOTS / 2 && all <= SLOTS && item >= SLOTS / 2) item = all - 1 - (item - SLOTS / 2);
     // consecutive workgroups go to consecutive XCDs: with the key head innermost, an XCD's L2 holds few heads' pages
     const int at = int_div(item, a.by_kv_heads), kvh = item - at * a.kv_heads;
@@ -732,6 +741,9 @@ __global__ __launch_bounds__(256, (D == 64 ? 3 : 2)) void paged_attn_chunk_kerne
 // =================================================================================================================================
 // Chunks in f32: a workgroup owns 64 rows, 16 per wave (the f32 matrix rate is a sixteenth of bf16's and the same for 16 x 16 x 4 as for
 // 32 x 32 x 2: the smaller shape wastes fewer rows of a ragged batch), the keys pass in tiles of 32 through a ring of LDS buffers.
+// Bound: the f32 matrix unit in long chunks (128 tokens over 30000 keys, 16 heads of 128 over 4: 302 us, 104 TFLOP/s; the library's product
+// of 4096^3 reaches 144), starts, joins and unequal lengths in short ones (5 chunks of up to 257 over up to 1290 keys, 16 heads of 64: 43 us
+// and 6 of the join, 13 of them matrix work).
 // =================================================================================================================================
 template <int D> struct TileCfg {
     static constexpr int M = 64, NW = 4, KT = 32, RB = D * 4;
@@ -908,6 +920,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
 // Few rows (at most 16 per sequence and key head: single tokens, their groups, short drafts): bound by the stream of the cache.  A wave
 // owns every NW-th tile of 32 (f32: 16) keys and two LDS buffers of its own, so that nothing in the loop waits for another wave; the waves'
 // states are joined once at the end.
+// Measured: 32 sequences of 700 - 2579 keys, 16 heads of 64 in bf16: 46 us, 4760 GB/s; two of 120001 - 131070 keys, 32 heads of 128 over 4:
+// 93 us and 5 of the join, 5150 GB/s; a copy of 1 GiB reaches 5060.  One sequence of up to 700 keys is a chain of dependent trips: 7 us.
 // =================================================================================================================================
 template <typename P, int D> struct StepCfg {
     static constexpr int M = 16, KT = P::IS_BF16 ? 32 : 16;
@@ -1102,7 +1116,8 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_step_kernel(PagedAttnArgs 
 
 // =================================================================================================================================
 // Joins the partial results of cut tiles.  A workgroup takes RPB rows of a tile: 256 / (D / 4) of them, one 16-byte piece of a row per
-// thread, or (few rows, many shares) a single one, the shares dealt out over its threads.
+// thread, or (few rows, many shares) a single one, the shares dealt out over its threads.  Bound by its launch and two trips to memory: 4 to
+// 6 us (one share after the other: 128 rows of 116 shares took 30).
 // =================================================================================================================================
 template <typename P, int D, int M, int KT, int RPB>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
@@ -1195,19 +1210,29 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
 
 struct Plan { bool step; int tiles, splits, min_share; };
 
-// max_new tokens a sequence at most (0: not known) make at most max_new * group rows per key head: up to 16 take the step kernel.
+// max_new tokens a sequence at most (0: not known) make at most max_new * group rows per key head.  Up to 16 take the step kernel; up to 128
+// where its tiles of 16 are no more than the CUs and the keys are few (128 KiB of them): four waves then share a tile's keys, where the
+// chunk kernel leaves them to one wave a row (bf16, 8 x 32 rows over 500 keys, 8 heads of 64: 9.6 us, 13.3; 4 x 60 rows over 200, 16 heads: 7.2,
+// 9.9; f32: 12.9, 20.6; over more keys it loses: 1 x 120 rows over 6000, head dim 128: 27.9, 22.8).
 Plan make_plan(const PagedAttnArgs& a, int max_new, int head_dim, int dtype) {
     const int row_of_cache = head_dim * (dtype == PTTS_BF16 ? 2 : 4);
     Plan p;
     const int64_t most = (a.starts ? max_new : 1) * (int64_t)a.group;       // 0: not known
-    p.step = most > 0 && most <= 16;
+    const int64_t keys = (int64_t)a.max_pages << a.page_shift;
+    const bool more_rows = most > 16 && most <= 128 && keys * row_of_cache <= 131072 && a.n_seqs * a.kv_heads * ((most + 15) / 16) <= 256;
+    p.step = (most > 0 && most <= 16) || more_rows;
     const int M = p.step ? 16 : (dtype == PTTS_BF16 ? 128 : 64);
     const int64_t ub = a.starts ? (int64_t)a.tokens * a.group / M + a.n_seqs : (int64_t)a.n_seqs * ((a.group + M - 1) / M);
     p.tiles = (int)ub;
     int64_t est = most > 0 ? (int64_t)a.n_seqs * ((most + M - 1) / M) : ub;
     if (est > ub) est = ub;
-    // most shares of a tile: none where the keys a workgroup could be left with alone take less time than joining; 128 MiB of partial results
-    const int64_t keys = (int64_t)a.max_pages << a.page_shift, row_bytes = (int64_t)a.tokens * a.q_heads * (head_dim + 2) * 4;
+    // Most shares of a tile: none where the launch covers most CUs (`idle`: those it leaves over; from 160 items on cutting gains nothing but
+    // evenness) and the keys that a workgroup could be left with alone take less time than the join: 512 keys of chunks in bf16, 64 KiB of
+    // K for few rows, two least shares in f32.  Measured, whole and cut, in us: 12 chunks of 128 over 1900 keys, 16 heads of 64 in bf16
+    // (192 items) 37, 47; 15 x 74 rows over 372, 10/5 heads of 128 16.5, 24; 4 x 259 over 779, 4/2 heads of 64 (40 items) 16.2, 13.8; single
+    // tokens over 1900 keys, 16 x 16 heads of 64 26, 31; over 900, 16 heads of 128 (16 items) 22, 12; over 500 (64 items) 13.5, 12.
+    // Never more than 128 MiB of partial results.
+    const int64_t row_bytes = (int64_t)a.tokens * a.q_heads * (head_dim + 2) * 4;
     p.min_share = 32768 / row_of_cache < 32 ? 32 : 32768 / row_of_cache;    // 32 KiB of keys: 256 rows of 64 in bf16, 64 of 128 in f32
     int64_t s = keys / p.min_share;
     const int64_t items = est * a.kv_heads, idle = items < 160 ? 256 - items : 0;
@@ -1221,7 +1246,7 @@ Plan make_plan(const PagedAttnArgs& a, int max_new, int head_dim, int dtype) {
 }
 
 // Four waves with stages of 16 KiB have a CU to themselves, two share it with another workgroup: four where the launch gives a CU no
-// second workgroup anyway.
+// second workgroup anyway (bf16, head dim 128: 64 tokens over 100 keys, 16/4 heads 6.8 us, 9.1; 30000 keys, 16/4 heads 25.3, 21.1).
 template <typename P, int D>
 void launch_step(const PagedAttnArgs& a, unsigned items, hipStream_t s) {
     if constexpr (StepCfg<P, D>::STAGE > 8192) {

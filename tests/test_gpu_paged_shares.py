@@ -175,3 +175,15 @@ def test_another_current_device_is_left_as_it_was(paged):
         out = paged.paged_attention(q, cache, ints([[0]]), ints([3]))
     torch.cuda.synchronize()
     assert torch.cuda.current_device() == before and (out == 0).all()
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF, 64), (BF, 128), (F32, 64), (F32, 128)])
+@pytest.mark.parametrize("rows", [17, 33, 127, 128, 129])
+def test_some_rows_over_few_keys(paged, rows, dtype, dim):
+    """between the kernel for few rows and the one for chunks, either side of the rule, ragged; keys around the rule's 128 KiB"""
+    edge = 131072 // (dim * (2 if dtype == BF else 4))
+    attend(paged, [(rows, 30), (1, 0), (rows // 2, edge - rows // 2 - 64)], 32, 2, 2, dim, dtype, max_new=rows, padding=1)
+    attend(paged, [(rows, edge - rows), (3, 5)], 64, 2, 2, dim, dtype, max_new=rows)
+    attend(paged, [(max(rows // 4, 1), 40), (rows // 8, 70)], 16, 8, 2, dim, dtype, max_new=rows // 4, causal=False)
+    mask = torch.rand(2, 90, generator=torch.Generator().manual_seed(1)) < 0.5
+    attend(paged, [(rows, 40), (9, 60)], 16, 2, 1, dim, dtype, max_new=rows, mask=mask)
