@@ -281,6 +281,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
     column is no key, whatever the cache holds there; keys behind its last column are seen.  A token without keys gets zeros.
     ``q``'s heads are a multiple of the cache's, in groups: head h reads key head h // (heads / kv_heads).
     ``max_new``: the longest sequence's number of new tokens if the caller knows it (it helps to pick the kernel; 0: unknown).
+    Rows of ``q`` and ``out`` start at multiples of 16 bytes and share no memory.
     Sequences may share pages, or (an expanded ``table``) all of them.  Rows of no sequence (behind the last, or where ``starts`` are wrong)
     are left as they are in ``out``."""
     device, dim = cache.device, cache.head_dim
