@@ -72,6 +72,7 @@ struct PagedAttnArgs {
     const uint8_t* mask;     // [n_seqs][mask_stride], keys < mask_width with 0 are no keys; null: none
     int* status;
     float* part;             // partial results of a split launch: [split][row][D + 2]
+    int* sched;              // what a launch in front left of many sequences, or null
     int64_t qs[2], os[2], kc[3], vc[3];
     int64_t table_stride, mask_stride;
     float scale_log2;        // softmax scale * log2(e)

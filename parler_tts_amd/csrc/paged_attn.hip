@@ -135,14 +135,22 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 
 // ---- which rows and keys a workgroup takes -------------------------------------------------------------------------------------
 // A launch's items are (tile of M rows of a sequence, share of its keys, key head).  Their numbers come from the lengths on the device:
-// every wave sums the sequences' tiles up for itself, 64 sequences at a time, all lengths in one round trip.  Items are numbered without
+// every wave sums the sequences' tiles up for itself, 64 sequences at a time, all lengths in one round trip.  Behind MANY_SEQS sequences one
+// workgroup does that once, in a launch in front (4 us), and leaves its groups of 64 and their first items in the workspace for a search; one
+// token each without shares needs neither.  Items are numbered without
 // holes (with holes between the sequences the dispatcher put all work of equal chunks on half of the CUs).
 // Keys are shared out only where that evens the load: a tile whose keys exceed what one of SLOTS workgroups would get of everything (by the
 // factor LAG) is cut into shares of that size, at least min_share keys each (a share costs its rows' f32 partial results, written and read
 // once more).  SLOTS are two workgroups on each of 256 CUs.  Counting the third that head dim 64 has room for made finer shares and lost
 // more at their ends than it won: prompts of up to 7770 over 2324 keys, 2 heads of 64: 68 us, with two 58; a batch of 24 chunks 81, 76.
 constexpr int SLOTS = 512, MAX_SPLITS = 256;
+constexpr int MANY_SEQS = 128;
 constexpr float TILE_LAG = 2.f, STEP_LAG = 2.f;
+
+// The schedule of a launch in front, in ints: first item of every group of 64 sequences and their number behind them, the same of tiles, and the
+// sequences of the groups in the order of their items: index, first token, new tokens, cached ones.
+__host__ __device__ inline int sched_groups(int n_seqs) { return (n_seqs + 63) / 64; }
+__host__ __device__ inline int64_t sched_ints(int n_seqs) { return 2 * ((int64_t)sched_groups(n_seqs) + 1) + 256 * (int64_t)sched_groups(n_seqs); }
 
 struct Item {
     int seq, first, n, past;    // the sequence, its first token, its new tokens, its cached ones
@@ -170,6 +178,24 @@ template <int M, int KT, bool SORTED> struct Schedule {
         } else { first = i; n = 1; }
         past = a.past[i];
         if (i0 + lane >= a.n_seqs) n = 0;
+    }
+    __device__ __forceinline__ void load_group(const PagedAttnArgs& a, int g) {      // of the launch in front
+        const int lane = threadIdx.x & 63, groups = sched_groups(a.n_seqs);
+        const int* e = a.sched + 2 * (groups + 1) + (int64_t)g * 256 + lane;
+        base = g * 64;
+        seq = e[0]; first = e[64]; n = e[128]; past = e[192];
+    }
+    // group of item (or tile) t among the first items `from`; t becomes its number within the group
+    static __device__ __forceinline__ int find_group(const int* from, int groups, int* t) {
+        const int lane = threadIdx.x & 63;
+        int lo = 0, len = groups;
+        for (;;) {
+            const int step = (len + 63) / 64, i = min(lane * step, len - 1), v = from[lo + i];
+            const int k = uniform((int)__popcll(__ballot(lane * step < len && v <= *t)) - 1);
+            lo += k * step;
+            if (step == 1) { *t -= __builtin_amdgcn_readlane(v, k); return lo; }
+            len = min(step, len - k * step);
+        }
     }
     static __device__ __forceinline__ bool bad_length(const PagedAttnArgs& a, int np, int pp) {
         return pp < 0 || (int64_t)pp + (a.causal ? np : 0) > ((int64_t)a.max_pages << a.page_shift);
@@ -204,6 +230,26 @@ template <int M, int KT, bool SORTED> struct Schedule {
         n = __builtin_amdgcn_ds_permute(rank << 2, n);
         past = __builtin_amdgcn_ds_permute(rank << 2, past);
     }
+    // what the lane's sequence adds to the work of the batch (tiles of rows times the tiles of keys they see on average), and its keys
+    __device__ __forceinline__ void weigh(const PagedAttnArgs& a, float* work, int* most) const {
+        const int rt = row_tiles(a), kt = key_tiles(a);
+        *work += (float)rt * (float)(a.causal ? max(kt - n / (2 * KT), 1) : kt);
+        *most = max(*most, rt > 0 ? kt : 0);
+    }
+    // share for the whole batch: a slot's part of everything; a little more where the shares' ends would need a second round of a few workgroups
+    __device__ __forceinline__ void choose_share(const PagedAttnArgs& a, float mean, int most, float lag, bool one_group) {
+        share = 0x3fffffff;
+        if ((float)most <= lag * mean) return;
+        const int least = max(a.min_share / KT, (most + a.splits - 1) / a.splits);
+        const int front = a.causal ? min((past + KT) / KT, key_tiles(a)) : key_tiles(a);       // tiles the first row sees
+        for (int step = 4; step <= 8; ++step) {
+            share = max((int)ceilf(mean * 0.25f * (float)step), least);
+            if (!one_group || step == 8) break;
+            const int all = uniform(__builtin_amdgcn_readlane(scan_add(row_tiles(a) * (shares(key_tiles(a)) + shares(front))), 63));
+            if (all * a.kv_heads <= 2 * SLOTS) break;
+        }
+        share = uniform(share);
+    }
     // share for the whole batch, the number of items
     __device__ __forceinline__ void plan(const PagedAttnArgs& a, float lag) {
         share = 0x3fffffff;
@@ -212,27 +258,12 @@ template <int M, int KT, bool SORTED> struct Schedule {
             float work = 0.f;
             int most = 0;
             for (int i0 = 0;;) {
-                const int rt = row_tiles(a), kt = key_tiles(a);
-                work += (float)rt * (float)(a.causal ? max(kt - n / (2 * KT), 1) : kt);
-                most = max(most, rt > 0 ? kt : 0);
+                weigh(a, &work, &most);
                 i0 += 64;
                 if (i0 >= a.n_seqs) break;
                 load(a, i0);
             }
-            const float mean = wave_sum(work) * (float)a.kv_heads / SLOTS;
-            most = (int)wave_max_u32((unsigned)most);
-            if ((float)most > lag * mean) {
-                // a slot's part of everything; a little more where the shares' ends would need a second round of a few workgroups
-                const int least = max(a.min_share / KT, (most + a.splits - 1) / a.splits);
-                const int front = a.causal ? min((past + KT) / KT, key_tiles(a)) : key_tiles(a);       // tiles the first row sees
-                for (int step = 4; step <= 8; ++step) {
-                    share = max((int)ceilf(mean * 0.25f * (float)step), least);
-                    if (a.n_seqs > 64 || step == 8) break;
-                    const int all = uniform(__builtin_amdgcn_readlane(scan_add(row_tiles(a) * (shares(key_tiles(a)) + shares(front))), 63));
-                    if (all * a.kv_heads <= 2 * SLOTS) break;
-                }
-            }
-            share = uniform(share);
+            choose_share(a, wave_sum(work) * (float)a.kv_heads / SLOTS, (int)wave_max_u32((unsigned)most), lag, a.n_seqs <= 64);
             if (a.n_seqs > 64) load(a, 0);
         }
         number(a);
@@ -249,8 +280,12 @@ template <int M, int KT, bool SORTED> struct Schedule {
         }
     }
     // item t < items
-    __device__ __forceinline__ void find(const PagedAttnArgs& a, int t, Item* it) {
-        if (a.n_seqs > 64) {
+    __device__ __forceinline__ void find(const PagedAttnArgs& a, int t, Item* it, const int* from) {
+        if (a.sched) {
+            const int groups = sched_groups(a.n_seqs);
+            load_group(a, find_group(from, groups, &t));
+            count(a);
+        } else if (a.n_seqs > 64) {
             load(a, 0);
             for (;;) {
                 if (SORTED) sort(a);
@@ -267,6 +302,10 @@ template <int M, int KT, bool SORTED> struct Schedule {
         it->n = __builtin_amdgcn_readlane(n, sel);
         it->past = __builtin_amdgcn_readlane(past, sel);
         t -= __builtin_amdgcn_readlane(sum - own, sel);
+        place(a, t, it);
+    }
+    // tile and share of the sequence's pair t
+    __device__ __forceinline__ void place(const PagedAttnArgs& a, int t, Item* it) const {
         const int tiles = (it->n * a.group + M - 1) / M;
         it->bad = bad_length(a, it->n, it->past);
         if (it->bad) it->past = 0;
@@ -300,8 +339,66 @@ __device__ __forceinline__ PagedAttnArgs arguments_again() {
 
 template <typename S> __device__ __forceinline__ void begin(const PagedAttnArgs& a, S& sched, float lag) {
     if (blockIdx.x == 0 && a.starts) check_starts(a.starts, a.n_seqs, a.tokens, a.status);
+    if (a.sched) {
+        sched.share = a.splits > 1 ? __builtin_bit_cast(int, a.part[0]) : 0x3fffffff;
+        sched.items = a.sched[sched_groups(a.n_seqs)];
+        return;
+    }
     sched.plan(a, lag);
     if (blockIdx.x == 0 && threadIdx.x == 0 && a.splits > 1) a.part[0] = __builtin_bit_cast(float, sched.share);
+}
+
+template <int M, int KT, bool SORTED>
+__global__ __launch_bounds__(1024) void paged_attn_schedule_kernel(PagedAttnArgs a, float lag) {
+    __shared__ float works[16];
+    __shared__ int mosts[16], items[16], tiles[16];
+    const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), groups = sched_groups(a.n_seqs);
+    int *item0 = a.sched, *tile0 = a.sched + groups + 1, *entry = a.sched + 2 * (groups + 1);
+    Schedule<M, KT, SORTED> sc;
+    sc.share = 0x3fffffff;
+    if (a.splits > 1) {
+        float work = 0.f;
+        int most = 0;
+        for (int g = w; g < groups; g += 16) {
+            sc.load(a, g * 64);
+            sc.weigh(a, &work, &most);
+        }
+        work = wave_sum(work);
+        most = (int)wave_max_u32((unsigned)most);
+        if (lane == 0) { works[w] = work; mosts[w] = most; }
+        __syncthreads();
+        work = 0.f;
+        for (int i = 0; i < 16; ++i) { work += works[i]; most = max(most, mosts[i]); }
+        sc.load(a, 0);
+        sc.choose_share(a, work * (float)a.kv_heads / SLOTS, most, lag, false);
+        if (threadIdx.x == 0) a.part[0] = __builtin_bit_cast(float, sc.share);
+    }
+    int item_at = 0, tile_at = 0;
+    for (int g0 = 0; g0 < groups; g0 += 16) {
+        const int g = g0 + w;
+        int mine = 0, rows = 0;
+        if (g < groups) {
+            sc.load(a, g * 64);
+            if (SORTED) sc.sort(a);
+            sc.count(a);
+            mine = __builtin_amdgcn_readlane(sc.sum, 63);
+            rows = __builtin_amdgcn_readlane(scan_add(sc.row_tiles(a)), 63);
+            int* e = entry + (int64_t)g * 256 + lane;
+            e[0] = sc.seq; e[64] = sc.first; e[128] = sc.n; e[192] = sc.past;
+        }
+        if (lane == 0) { items[w] = mine; tiles[w] = rows; }
+        __syncthreads();
+        int before = item_at, tiles_before = tile_at;
+        for (int i = 0; i < 16; ++i) {
+            if (i == w && g < groups && lane == 0) { item0[g] = before; tile0[g] = tiles_before; }
+            before += items[i];
+            tiles_before += tiles[i];
+        }
+        item_at = before;
+        tile_at = tiles_before;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) { item0[groups] = item_at; tile0[groups] = tile_at; }
 }
 
 // ---- page ids of the keys ahead, one per lane ---------------------------------------------------------------------------------
@@ -504,7 +601,7 @@ __global__ __launch_bounds__(256, (D == 64 ? 3 : 2)) void paged_attn_chunk_kerne
     // consecutive workgroups go to consecutive XCDs: with the key head innermost, an XCD's L2 holds few heads' pages
     const int at = int_div(item, a.by_kv_heads), kvh = item - at * a.kv_heads;
     Item it;
-    sched.find(a, at, &it);
+    sched.find(a, at, &it, a.sched);
     if (it.split >= it.splits) return;
     const int k0 = it.k0, k1 = it.k1, r0 = it.tile * C::M, r_end = min(r0 + C::M, it.n * a.group);
     int row = r0 + w * 32 + l31;                               // this lane's query
@@ -768,7 +865,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     if (item >= sched.items * a.kv_heads) return;
     const int at = int_div(item, a.by_kv_heads), kvh = item - at * a.kv_heads;
     Item it;
-    sched.find(a, at, &it);
+    sched.find(a, at, &it, a.sched);
     if (it.split >= it.splits) return;
     const int k0 = it.k0, k1 = it.k1, r0 = it.tile * C::M, r_end = min(r0 + C::M, it.n * a.group);
     const int row = r0 + w * 16 + l15;                                                  // this lane's query
@@ -940,12 +1037,23 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_step_kernel(PagedAttnArgs 
     const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
 
     Schedule<C::M, KT, false> sched;
-    begin(a, sched, STEP_LAG);
-    const int item = blockIdx.x;
-    if (item >= sched.items * a.kv_heads) return;
-    const int at = int_div(item, a.by_kv_heads), kvh = item - at * a.kv_heads;
     Item it;
-    sched.find(a, at, &it);
+    int kvh;
+    const int item = blockIdx.x;
+    if (!a.starts && a.splits == 1) {        // one token each, whole: items follow from their numbers
+        const int tiles = (a.group + C::M - 1) / C::M, at = int_div(item, a.by_kv_heads), q = tiles == 1 ? at : at / tiles;
+        kvh = item - at * a.kv_heads;
+        it.seq = it.first = q;
+        it.n = 1;
+        it.past = a.past[q];
+        sched.place(a, at - q * tiles, &it);
+    } else {
+        begin(a, sched, STEP_LAG);
+        if (item >= sched.items * a.kv_heads) return;
+        const int at = int_div(item, a.by_kv_heads);
+        kvh = item - at * a.kv_heads;
+        sched.find(a, at, &it, a.sched);
+    }
     if (it.split >= it.splits) return;
     const int k0 = it.k0, k1 = it.k1, r0 = it.tile * C::M, r_end = min(r0 + C::M, it.n * a.group);
     const int row = r0 + l15;
@@ -1129,13 +1237,16 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
     const int share = __builtin_bit_cast(int, a.part[0]);
     Schedule<M, KT, false> sched;
     sched.share = 0x3fffffff;
-    sched.load(a, 0);
-    sched.number(a);
-    const int t = blockIdx.x / PARTS;
+    const int t = blockIdx.x / PARTS, groups = sched_groups(a.n_seqs);
+    if (a.sched) sched.items = a.sched[2 * groups + 1];
+    else {
+        sched.load(a, 0);
+        sched.number(a);
+    }
     if (t >= sched.items * a.kv_heads) return;
     const int at = int_div(t, a.by_kv_heads), kvh = t - at * a.kv_heads;
     Item it;
-    sched.find(a, at, &it);
+    sched.find(a, at, &it, a.sched + groups + 1);
     const int kt = (it.end + KT - 1) / KT, splits = min(kt <= share ? 1 : (kt + share - 1) / share, a.splits);
     if (splits == 1) return;                 // written already
     const int tid = threadIdx.x, piece = tid % LPR, sub = tid / LPR % SP;
@@ -1208,7 +1319,11 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
     }
 }
 
-struct Plan { bool step; int tiles, splits, min_share; };
+struct Plan { bool step, scheduled; int tiles, splits, min_share; };
+// floats of the share and the partial results in the workspace; the schedule lies behind them
+int64_t part_floats(const PagedAttnArgs& a, const Plan& p, int head_dim) {
+    return PART_HEAD + (p.splits == 1 ? 0 : (int64_t)p.splits * a.tokens * a.q_heads * (head_dim + 2));
+}
 
 // max_new tokens a sequence at most (0: not known) make at most max_new * group rows per key head.  Up to 16 take the step kernel; up to 128
 // where its tiles of 16 are no more than the CUs and the keys are few (128 KiB of them): four waves then share a tile's keys, where the
@@ -1242,6 +1357,7 @@ Plan make_plan(const PagedAttnArgs& a, int max_new, int head_dim, int dtype) {
     if (s > MAX_SPLITS) s = MAX_SPLITS;
     if (s > ((int64_t)128 << 20) / row_bytes) s = ((int64_t)128 << 20) / row_bytes;
     p.splits = s < 2 ? 1 : (int)s;
+    p.scheduled = a.n_seqs > MANY_SEQS && !(p.step && !a.starts && p.splits == 1);
     return p;
 }
 
@@ -1270,6 +1386,14 @@ hipError_t launch(PagedAttnArgs a, int max_new, hipStream_t s) {
     const int64_t groups = (int64_t)p.tiles * a.kv_heads;
     const int64_t cut = groups * p.splits < groups + 2 * SLOTS + 64 ? groups * p.splits : groups + 2 * SLOTS + 64;
     if (cut > 0x7fffffff / 16) return hipErrorInvalidValue;
+    a.sched = p.scheduled ? reinterpret_cast<int*>(a.part) + part_floats(a, p, D) : nullptr;
+    if (p.scheduled) {
+        if (p.step) hipLaunchKernelGGL((paged_attn_schedule_kernel<16, StepCfg<P, D>::KT, false>), dim3(1), dim3(1024), 0, s, a, STEP_LAG);
+        else if constexpr (P::IS_BF16) hipLaunchKernelGGL((paged_attn_schedule_kernel<128, 64, true>), dim3(1), dim3(1024), 0, s, a, TILE_LAG);
+        else hipLaunchKernelGGL((paged_attn_schedule_kernel<64, 32, true>), dim3(1), dim3(1024), 0, s, a, TILE_LAG);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
     if (p.step) launch_step<P, D>(a, (unsigned)cut, s);
     else if constexpr (P::IS_BF16) hipLaunchKernelGGL(paged_attn_chunk_kernel<D>, dim3((unsigned)cut), dim3(256), 0, s, a);
     else hipLaunchKernelGGL(paged_attn_tile_kernel<D>, dim3((unsigned)cut), dim3(256), 0, s, a);
@@ -1286,7 +1410,8 @@ hipError_t launch(PagedAttnArgs a, int max_new, hipStream_t s) {
 
 int64_t paged_attn_workspace(const PagedAttnArgs& a, int max_new, int head_dim, int dtype) {
     const Plan p = make_plan(a, max_new, head_dim, dtype);
-    return p.splits == 1 ? 0 : (PART_HEAD + (int64_t)p.splits * a.tokens * a.q_heads * (head_dim + 2)) * (int64_t)sizeof(float);
+    if (p.splits == 1 && !p.scheduled) return 0;
+    return (part_floats(a, p, head_dim) + (p.scheduled ? sched_ints(a.n_seqs) : 0)) * (int64_t)sizeof(float);
 }
 
 hipError_t paged_attn_launch(const PagedAttnArgs& a, int max_new, int head_dim, int dtype, hipStream_t s) {

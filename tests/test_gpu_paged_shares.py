@@ -187,3 +187,61 @@ def test_some_rows_over_few_keys(paged, rows, dtype, dim):
     attend(paged, [(max(rows // 4, 1), 40), (rows // 8, 70)], 16, 8, 2, dim, dtype, max_new=rows // 4, causal=False)
     mask = torch.rand(2, 90, generator=torch.Generator().manual_seed(1)) < 0.5
     attend(paged, [(rows, 40), (9, 60)], 16, 2, 1, dim, dtype, max_new=rows, mask=mask)
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF, 64), (F32, 128)])
+@pytest.mark.parametrize("n", [128, 129, 700, 4200])
+def test_hundreds_of_sequences(paged, n, dtype, dim):
+    """the schedule of a launch in front: groups of 64 searched once and (beyond 64 groups) twice; whole, in shares, ragged with empty ones"""
+    attend(paged, spread_lengths(n, n, top=40), 16, 1, 1, dim, dtype, single=True)
+    attend(paged, spread_lengths(n, n, top=40, long_ones=(3, n // 2, n - 1), long_past=4500), 64, 1, 1, dim, dtype, single=True)
+    attend(paged, spread_lengths(n, n, new=5, top=40), 16, 2, 1, dim, dtype, padding=2, max_new=5)
+    attend(paged, spread_lengths(n, n, new=5, top=40, long_ones=(0, n - 2), long_past=2500), 64, 2, 1, dim, dtype, padding=2)
+    empty = [(0, 3)] * n
+    for i in (0, n // 2, n // 2 + 1, n - 1):
+        empty[i] = (70 + i % 7, 100 + i)
+    attend(paged, empty, 64, 2, 2, dim, dtype, padding=1)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_captured_call_over_hundreds_of_sequences(paged, dtype):
+    n, dim = 300, 64
+    starts, past, table, pages = ref.make_batch([(i % 3, 30 + i) for i in range(n)], 32)
+    cache = paged.PagedKVCache.from_tensors(rnd(2, pages, 1, 32, dim, dtype=dtype).cuda(), rnd(3, pages, 1, 32, dim, dtype=dtype).cuda())
+    q = rnd(1, starts[-1], 2, dim, dtype=dtype).cuda()
+    at, table, begins = ints(past), table.cuda(), ints(starts)
+    call = lambda: paged.paged_attention(q, cache, table, at, begins)
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = call()
+    for i in range(4):
+        at.sub_(7)
+        want = call()
+        g.replay()
+        junk = call()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want) and torch.equal(junk, want), i
+    cache.check()
+
+
+@pytest.mark.parametrize("single", [True, False])
+def test_bad_entries_among_hundreds_of_sequences(paged, single):
+    from parler_tts_amd._hip import PttsError
+
+    n, dim = 200, 64
+    starts, past, table, pages = ref.make_batch([(1 if single else 1 + i % 4, 30 + i % 50) for i in range(n)], 16)
+    kc, vc, q = rnd(2, pages, 1, 16, dim), rnd(3, pages, 1, 16, dim), rnd(1, starts[-1], 1, dim)
+    want, bound = ref.attend(q, kc, vc, table, past, starts, 0.125)
+    cache = paged.PagedKVCache.from_tensors(kc.cuda(), vc.cuda())
+    table[50, 1] = -5
+    past[120], past[130] = -3, 2 ** 31 - 1
+    got = paged.paged_attention(q.cuda(), cache, table.cuda(), ints(past), None if single else ints(starts))
+    keep = torch.ones(starts[-1], dtype=torch.bool)
+    for s in (50, 120, 130):
+        keep[starts[s]:starts[s + 1]] = False
+        assert got[starts[s]:starts[s + 1]].isnan().all()
+    close(got[keep.cuda()], want[keep], bound[keep])
+    with pytest.raises(PttsError, match="page id.*longer|longer.*page id|page id"):
+        cache.check()
