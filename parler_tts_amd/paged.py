@@ -209,6 +209,8 @@ def rotary_embed(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, 
     _ints("positions", positions, 1, rotary.device)
     if positions.shape[0] != tokens:
         raise ValueError(f"{positions.shape[0]} positions for {tokens} tokens")
+    if rotary.device.type != "cuda":
+        raise ValueError(f"the rotary table is on {rotary.device}: a ROCm device is needed to turn rows")
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     else:

@@ -186,6 +186,14 @@ def test_the_wrapper_refuses_what_does_not_fit_the_table():
             rotary_embed(x, p, t)
 
 
+def test_tensors_in_host_memory_are_refused_not_launched_on():
+    t = RotaryTable(64, 16, device="cpu")
+    with pytest.raises(ValueError, match="ROCm device"):
+        rotary_embed(torch.zeros(3, 2, 64), torch.zeros(3, dtype=torch.int32), t)
+    with pytest.raises(ValueError, match="ROCm device"):
+        PagedKVCache(4, 16, 2, 64, device="cpu")
+
+
 def test_public_names():
     import parler_tts_amd as p
 
