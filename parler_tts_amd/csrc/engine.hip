@@ -414,9 +414,9 @@ void dump_allocs(const ptts_engine* e) {
         const char* tag = e->allocs[i] == e->self_pool ? "self_pool" : (e->allocs[i] == e->cross_pool ? "cross_pool" : "");
         fprintf(f, "%p %p %zu %s\n", e->allocs[i], (void*)((char*)e->allocs[i] + e->alloc_bytes[i]), e->alloc_bytes[i], tag);
     }
-    const void* extra[] = {e->pf.x, e->pf.q, e->pf.attn_frag, e->pf.mlp_frag, e->pf.x_frag, e->pf.x_frag2, e->dac_buf0, e->dac_buf1};
-    const char* names[] = {"pf.x", "pf.q", "pf.attn_frag", "pf.mlp_frag", "pf.x_frag", "pf.x_frag2", "dac_buf0", "dac_buf1"};
-    for (int i = 0; i < 8; ++i)
+    const void* extra[] = {e->pf.x, e->pf.q, e->pf.attn_frag, e->pf.mlp_frag, e->pf.x_frag, e->pf.x_frag2, e->pf.far, e->dac_buf0, e->dac_buf1};
+    const char* names[] = {"pf.x", "pf.q", "pf.attn_frag", "pf.mlp_frag", "pf.x_frag", "pf.x_frag2", "pf.far", "dac_buf0", "dac_buf1"};
+    for (int i = 0; i < 9; ++i)
         if (extra[i]) fprintf(f, "%p ? ? %s\n", extra[i], names[i]);
     fclose(f);
 }
