@@ -1,6 +1,7 @@
 // C ABI of the engine (include/parler_tts_hip.h): weight registry, paged KV pools, the decode-step
 // launch sequence (captured once into a hipGraph and replayed per token), prefill, T5 encoder,
 // HIP-event profiling of the dominant kernel.
+#include <climits>
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -131,6 +132,8 @@ struct ptts_engine {
     Work pf;                   // batched-prefill workspaces (lazy)
     bool seq_prefill = false;  // PTTS_PREFILL_SEQ=1: the round-1 prefill, one cached position at a time (A/B, tests)
     int pf_chunk = 128;        // positions per batched-prefill chunk (PTTS_PREFILL_CHUNK)
+    int pf_paged_from = INT_MAX;   // chunks that reach behind this position take long_prefill_launch (PTTS_PREFILL_PAGED_FROM); where the
+                                   // score rows do not fit the LDS they do whatever it says
     bool no_page_kernel = false;   // PTTS_ATTN_NO_PAGE_KERNEL=1: cross-attention on the general kernel (A/B, tests)
     // decoder-op variants (ptts_config.dec_variant; extensions with no counterpart in the reference)
     bool v_rms = false, v_rope = false, v_swiglu = false;
@@ -421,6 +424,8 @@ void dump_allocs(const ptts_engine* e) {
     fclose(f);
 }
 
+bool prefill_is_far(const ptts_engine* e, int end) { return !attn_causal_fits(end) || end > e->pf_paged_from; }
+
 LongPrefillArgs far_args(const ptts_engine* e, const Work& wk, int layer, int B, int npos, int pos0) {
     const ptts_config& c = e->cfg;
     LongPrefillArgs a = {};
@@ -469,7 +474,7 @@ int run_layers(ptts_engine* e, hipStream_t s, bool profile, const Work& wk, int 
         const bool fuse = qkv_built && npos == 0 && !e->v_rope && e->dbg_stop < 0 && e->fuse_qkv_attn && e->fuse_arrive &&
                           (size_t)c.layers * ((M + 31) / 32) * c.heads * 32 <= e->fuse_arrive_ints && fused_qkv_attn_supported(g, a, e->dt);
         // a chunk whose score rows do not fit the LDS: the operators over a paged cache (the rotation of the rotary variant among them)
-        const bool far = npos > 0 && !attn_causal_fits(pos0 + npos);
+        const bool far = npos > 0 && prefill_is_far(e, pos0 + npos);
         if (qkv_built && !fuse) {
             DBG_GATE(e);
             STAMP_ARGS(e, g);
@@ -962,6 +967,7 @@ int ptts_create(const ptts_config* cfg, ptts_engine** out) {
     if (const char* v = getenv("PTTS_FOLD_MASK")) e->fold_mask = atoi(v);
     e->dac_f32_only = getenv("PTTS_DAC_F32") != nullptr;
     e->seq_prefill = getenv("PTTS_PREFILL_SEQ") != nullptr && atoi(getenv("PTTS_PREFILL_SEQ")) != 0;
+    if (const char* from = getenv("PTTS_PREFILL_PAGED_FROM")) e->pf_paged_from = atoi(from) < 0 ? 0 : atoi(from);
     e->self_identity = getenv("PTTS_FORCE_PAGE_TABLE") == nullptr;     // A/B: always go through the table read
     e->skip_finished = getenv("PTTS_NO_SKIP_FINISHED") == nullptr;
     if (const char* v = getenv("PTTS_PREFILL_CHUNK")) { e->pf_chunk = atoi(v); if (e->pf_chunk < 1) e->pf_chunk = 1; }
@@ -1445,10 +1451,10 @@ int ptts_prefill(ptts_engine* e, int32_t B, int32_t B_eff, int32_t T, int32_t P,
             HIP_TRY(hipMemsetAsync(w.x_frag2, 0, e->esz * R * D_, s));
             HIP_TRY(hipMemsetAsync(w.x, 0, sizeof(float) * R * D_, s));
         }
-        if (!attn_causal_fits(total)) {       // the chunks' needs, then one allocation
+        if (prefill_is_far(e, total)) {       // the chunks' needs, then one allocation
             int64_t need = 0;
             auto look = [&](int pos0, int npos) {
-                if (attn_causal_fits(pos0 + npos)) return;
+                if (!prefill_is_far(e, pos0 + npos)) return;
                 const int64_t n = long_prefill_workspace(far_args(e, e->pf, 0, B_eff, npos, pos0), e->dt);
                 if (n > need) need = n;
             };

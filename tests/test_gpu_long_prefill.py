@@ -59,3 +59,17 @@ def test_a_second_call_with_a_longer_prompt_grows_the_workspace(hip):  # noqa: F
         ids.append((n, m.last_raw_ids.clone()))
     same = [x for n, x in ids if n == 5800]
     assert all(torch.equal(x, same[0]) for x in same)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_short_prompts_on_the_long_route(hip, dtype):  # noqa: F811
+    """PTTS_PREFILL_PAGED_FROM: every chunk, and (in chunks of 3) those behind position 4 only, against the default, on the cases and within the bounds of
+    the batched prefill's own equivalence test (tests/test_gpu_parity.py); bf16 rounds the queries once more"""
+    from tests.test_gpu_parity import _fresh_engine_logits
+
+    tol = 2e-5 if dtype == "fp32" else 0.04
+    for name in ("tiny_greedy", "tiny_greedy_ragged", "tiny_cfg"):
+        a = _fresh_engine_logits(name, dtype, {"PTTS_PREFILL_PAGED_FROM": None})
+        for env in ({"PTTS_PREFILL_PAGED_FROM": "0"}, {"PTTS_PREFILL_PAGED_FROM": "4", "PTTS_PREFILL_CHUNK": "3"}):
+            b = _fresh_engine_logits(name, dtype, env)
+            assert (a - b).abs().max().item() < tol, (name, env, (a - b).abs().max().item())
