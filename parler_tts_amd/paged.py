@@ -34,14 +34,14 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-# the current stream's handle without the object around it (2.6 us of a call that launches in 3)
+# the current stream's handle without the object around it (2.6 us of a call that launches in 3); the device likewise
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _launch(device: torch.device, entry, *args) -> None:
-    """one C entry on the current stream of `device`, which is made the current device for the call if it is not"""
-    index = device.index
-    if index == torch.cuda.current_device():
+def _launch(index: int, entry, *args) -> None:
+    """one C entry on the current stream of device `index`, which is made the current device for the call if it is not"""
+    if index == _current_device():
         rc = entry(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -113,7 +113,7 @@ class RotaryTable:
         angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq.to(device)
         self.cos, self.sin = (torch.cos(angle) * gain).float(), (torch.sin(angle) * gain).float()
         self.head_dim, self.positions, self.rotary_dim, self.layout = head_dim, positions, rotary_dim, layout
-        self.device = self.cos.device
+        self.device, self._index = self.cos.device, self.cos.get_device()
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._status = self.status.data_ptr()
         self._c = _hip.PttsRotary(self.cos.data_ptr(), self.sin.data_ptr(), positions, rotary_dim, 1 if layout == "interleaved" else 0)
@@ -149,7 +149,7 @@ class PagedKVCache:
         _need(dim in (64, 128), f"head_dim {dim}: 64 and 128 are served")
         self.k, self.v = k, v
         self.num_pages, self.kv_heads, self.page_tokens, self.head_dim = pages, heads, tokens, dim
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self._index = k.dtype, k.device, k.get_device()
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._status = self.status.data_ptr()
         self._c = _hip.PttsPagedKV(k.data_ptr(), v.data_ptr(), (C.c_int64 * 3)(*k.stride()[:3]), (C.c_int64 * 3)(*v.stride()[:3]),
@@ -162,34 +162,35 @@ class PagedKVCache:
         _read_status(self.status, "paged cache")
 
 
-def _rows(name: str, t: torch.Tensor, tokens: Optional[int], heads: Optional[int], dim: int, device: torch.device) -> None:
+# (device numbers instead of devices, -1 for the host's: a tenth of a microsecond a comparison)
+def _rows(name: str, t: torch.Tensor, tokens: Optional[int], heads: Optional[int], dim: int, index: int) -> None:
     shape = t.shape
     if len(shape) != 3 or shape[2] != dim or (tokens is not None and shape[0] != tokens) or (heads is not None and shape[1] != heads):
         raise ValueError(f"{name} {tuple(shape)}: [{'tokens' if tokens is None else tokens}, {'heads' if heads is None else heads}, {dim}] expected")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, not on device {index}")
     if t.stride(2) != 1:
         raise ValueError(f"the features of a row of {name} have to be contiguous")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient; this operator has none (torch.no_grad(), or detach it)")
 
 
-def _ints(name: str, t: torch.Tensor, dims: int, device: torch.device) -> None:
-    if t.dtype != torch.int32 or t.dim() != dims or t.device != device or (t.numel() > 1 and t.stride(-1) != 1):
-        raise ValueError(f"{name} has to be a contiguous int32 tensor of {dims} dimension(s) on {device}")
+def _ints(name: str, t: torch.Tensor, dims: int, index: int) -> None:
+    if t.dtype is not torch.int32 or t.dim() != dims or t.get_device() != index or (t.stride(-1) != 1 and t.numel() > 1):
+        raise ValueError(f"{name} has to be a contiguous int32 tensor of {dims} dimension(s) on device {index}")
 
 
 def _batch(cache: PagedKVCache, tokens: int, table: torch.Tensor, past: torch.Tensor, starts: Optional[torch.Tensor]):
-    device = cache.device
-    _ints("table", table, 2, device)
-    _ints("past", past, 1, device)
+    index = cache._index
+    _ints("table", table, 2, index)
+    _ints("past", past, 1, index)
     n = past.shape[0]
     rows, width = table.shape
     if rows != n:
         raise ValueError(f"a page table of {rows} rows for {n} sequences")
     at = None
     if starts is not None:
-        _ints("starts", starts, 1, device)
+        _ints("starts", starts, 1, index)
         if starts.shape[0] != n + 1:
             raise ValueError(f"starts of {starts.shape[0]} entries for {n} sequences: one more than sequences")
         at = starts.data_ptr()
@@ -203,24 +204,25 @@ def rotary_embed(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, 
     """``x`` [tokens, heads, head_dim] (float32 or bfloat16) turned by ``positions`` [tokens] int32 -> ``out`` (may be ``x``).
     A row whose position is outside the table becomes zero, and ``rotary.check()`` raises."""
     tokens, heads = x.shape[0], x.shape[1] if x.dim() == 3 else None
-    _rows("x", x, None, None, rotary.head_dim, rotary.device)
+    index = rotary._index
+    _rows("x", x, None, None, rotary.head_dim, index)
     if x.dtype not in _DTYPES:
         raise ValueError(f"x of {x.dtype}: float32 or bfloat16")
-    _ints("positions", positions, 1, rotary.device)
+    _ints("positions", positions, 1, index)
     if positions.shape[0] != tokens:
         raise ValueError(f"{positions.shape[0]} positions for {tokens} tokens")
-    if rotary.device.type != "cuda":
+    if index < 0:
         raise ValueError(f"the rotary table is on {rotary.device}: a ROCm device is needed to turn rows")
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     else:
-        _rows("out", out, tokens, heads, rotary.head_dim, rotary.device)
+        _rows("out", out, tokens, heads, rotary.head_dim, index)
         if out.dtype != x.dtype:
             raise ValueError(f"out of {out.dtype} for x of {x.dtype}")
     if heads == 0 or tokens == 0:
         return out
     xs, os = x.stride(), out.stride()
-    _launch(rotary.device, _hip.load_library().ptts_rotary_embed, rotary._ref, _DTYPES[x.dtype], tokens, heads, rotary.head_dim, x.data_ptr(),
+    _launch(index, _hip.load_library().ptts_rotary_embed, rotary._ref, _DTYPES[x.dtype], tokens, heads, rotary.head_dim, x.data_ptr(),
             xs[0], xs[1], positions.data_ptr(), out.data_ptr(), os[0], os[1], rotary._status)
     return out
 
@@ -231,36 +233,36 @@ def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, table: torc
     """Stores ``k``, ``v`` [tokens, kv_heads, head_dim]: token i of sequence s at slot ``past[s] + i``, k turned by ``rotary`` at that
     position (or at ``positions`` [tokens] int32).  ``q`` [tokens, heads, head_dim] is turned in the same launch into ``q_out`` (may be ``q``),
     which is returned.  float32 rows may be stored in a bfloat16 cache.  Rows behind the last sequence are left alone, in ``q_out`` too."""
-    device = cache.device
+    index = cache._index
     tokens = k.shape[0]
-    _rows("k", k, tokens, cache.kv_heads, cache.head_dim, device)
-    _rows("v", v, tokens, cache.kv_heads, cache.head_dim, device)
+    _rows("k", k, tokens, cache.kv_heads, cache.head_dim, index)
+    _rows("v", v, tokens, cache.kv_heads, cache.head_dim, index)
     if k.dtype not in _DTYPES or v.dtype != k.dtype or (k.dtype != cache.dtype and k.dtype != torch.float32):
         raise ValueError(f"k of {k.dtype} and v of {v.dtype} for a cache of {cache.dtype}")
     batch = _batch(cache, tokens, table, past, starts)
     rot = at = None
     if rotary is not None:
-        if rotary.device != device or rotary.head_dim != cache.head_dim:
-            raise ValueError(f"a rotary table for heads of {rotary.head_dim} on {rotary.device}; the cache has {cache.head_dim} on {device}")
+        if rotary._index != index or rotary.head_dim != cache.head_dim:
+            raise ValueError(f"a rotary table for heads of {rotary.head_dim} on {rotary.device}; the cache has {cache.head_dim} on {cache.device}")
         rot = rotary._ref
     if positions is not None:
         if rotary is None:
             raise ValueError("positions without a rotary table")
-        _ints("positions", positions, 1, device)
+        _ints("positions", positions, 1, index)
         if positions.shape[0] != tokens:
             raise ValueError(f"{positions.shape[0]} positions for {tokens} tokens")
         at = positions.data_ptr()
     ks, vs = k.stride(), v.stride()
     heads, qp, qop, qs, qos = 0, None, None, (0, 0), (0, 0)
     if q is not None:
-        _rows("q", q, tokens, None, cache.head_dim, device)
+        _rows("q", q, tokens, None, cache.head_dim, index)
         heads = q.shape[1]
         if q.dtype != k.dtype or heads == 0:
             raise ValueError(f"q {tuple(q.shape)} of {q.dtype} beside k of {k.dtype}")
         if q_out is None:
             q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
-            _rows("q_out", q_out, tokens, heads, cache.head_dim, device)
+            _rows("q_out", q_out, tokens, heads, cache.head_dim, index)
             if q_out.dtype != q.dtype:
                 raise ValueError(f"q_out of {q_out.dtype} for q of {q.dtype}")
         qp, qop, qs, qos = q.data_ptr(), q_out.data_ptr(), q.stride(), q_out.stride()
@@ -268,7 +270,7 @@ def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, table: torc
         raise ValueError("q_out without q")
     if tokens == 0:
         return q_out
-    _launch(device, _hip.load_library().ptts_kv_append, cache._ref, C.addressof(batch), _DTYPES[k.dtype], k.data_ptr(), ks[0], ks[1],
+    _launch(index, _hip.load_library().ptts_kv_append, cache._ref, C.addressof(batch), _DTYPES[k.dtype], k.data_ptr(), ks[0], ks[1],
             v.data_ptr(), vs[0], vs[1], rot, at, heads, qp, qs[0], qs[1], qop, qos[0], qos[1], cache._status)
     return q_out
 
@@ -286,9 +288,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
     Rows of ``q`` and ``out`` start at multiples of 16 bytes and share no memory.
     Sequences may share pages, or (an expanded ``table``) all of them.  Rows of no sequence (behind the last, or where ``starts`` are wrong)
     are left as they are in ``out``."""
-    device, dim = cache.device, cache.head_dim
+    index, dim = cache._index, cache.head_dim
     tokens = q.shape[0]
-    _rows("q", q, None, None, dim, device)
+    _rows("q", q, None, None, dim, index)
     heads = q.shape[1]
     if q.dtype != cache.dtype:
         raise ValueError(f"q of {q.dtype} over a cache of {cache.dtype}")
@@ -298,8 +300,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
     mask, mask_stride, mask_width = None, 0, 0
     if key_mask is not None:
         if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.dim() != 2 or key_mask.shape[0] != past.shape[0] or \
-                key_mask.device != device or (key_mask.shape[1] > 1 and key_mask.stride(1) != 1):
-            raise ValueError(f"key_mask has to be a bool tensor [{past.shape[0]}, columns] on {device}")
+                key_mask.get_device() != index or (key_mask.shape[1] > 1 and key_mask.stride(1) != 1):
+            raise ValueError(f"key_mask has to be a bool tensor [{past.shape[0]}, columns] on {cache.device}")
         mask_width = key_mask.shape[1]
         mask, mask_stride = key_mask.data_ptr() if mask_width else None, max(key_mask.stride(0), mask_width)
         if key_mask.shape[0] > 1 and key_mask.stride(0) < mask_width:
@@ -308,7 +310,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        _rows("out", out, tokens, heads, dim, device)
+        _rows("out", out, tokens, heads, dim, index)
         if out.dtype != q.dtype:
             raise ValueError(f"out of {out.dtype} for q of {q.dtype}")
     if tokens == 0:
@@ -324,9 +326,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
         if len(cache._workspace) > 4096:
             cache._workspace.clear()
         cache._workspace[key] = need
-    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    workspace = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
     qs, os = q.stride(), out.stride()
-    _launch(device, lib.ptts_paged_attention, cache._ref, bref, heads, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
+    _launch(index, lib.ptts_paged_attention, cache._ref, bref, heads, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
             dim ** -0.5 if scale is None else scale, 1 if causal else 0, mask, mask_stride, mask_width, max_new,
             workspace.data_ptr() if need else None, need, cache._status)
     return out
