@@ -317,12 +317,16 @@ int check_rows(const char* name, const void* p, const int64_t* st, int64_t token
     return PTTS_OK;
 }
 
-// byte range of a strided tensor of rows
+// whether the byte ranges of two strided tensors of rows meet; slices of one buffer's rows (the same token stride) may lie beside each other
 bool ranges_meet(const void* a, const int64_t* as, const void* b, const int64_t* bs, int64_t tokens, int64_t heads, int64_t d, int esz) {
     const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
     const uintptr_t ea = pa + (uintptr_t)(((tokens - 1) * as[0] + (heads - 1) * as[1] + d) * esz);
     const uintptr_t eb = pb + (uintptr_t)(((tokens - 1) * bs[0] + (heads - 1) * bs[1] + d) * esz);
-    return pa < eb && pb < ea;
+    if (!(pa < eb && pb < ea)) return false;
+    const int64_t stride = as[0] * esz, la = ((heads - 1) * as[1] + d) * esz, lb = ((heads - 1) * bs[1] + d) * esz;
+    if (as[0] != bs[0] || la > stride || lb > stride) return true;
+    const int64_t apart = pb >= pa ? (int64_t)((pb - pa) % (uintptr_t)stride) : (stride - (int64_t)((pa - pb) % (uintptr_t)stride)) % stride;
+    return apart < la || apart + lb > stride;
 }
 
 PagedBatchArgs batch_args(const ptts_paged_kv* c, const ptts_paged_batch* b) {

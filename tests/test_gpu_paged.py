@@ -388,6 +388,15 @@ def test_strides_of_q_out_and_cache_agree_to_the_bit(paged):
         close(paged.paged_attention(q, cache, wide, *args[1:]), want.double().cpu(), 2 ** -7 * want.double().abs().cpu() + 2 ** -7, "wider table")
         with pytest.raises(Exception, match="share"):
             paged.paged_attention(q, cache, *args, out=q)
+        both = torch.full((starts[-1], 2 * heads + 1, dim), 5.0, dtype=BF, device="cuda")     # q and out beside each other in one buffer's rows
+        for at, to in ((0, heads + 1), (heads + 1, 1)):
+            both.fill_(5.0)
+            both[:, at:at + heads] = q
+            got = paged.paged_attention(both[:, at:at + heads], cache, *args, out=both[:, to:to + heads])
+            rest = [i for i in range(2 * heads + 1) if not (at <= i < at + heads or to <= i < to + heads)]
+            assert torch.equal(got, want) and torch.equal(both[:, at:at + heads], q) and (both[:, rest] == 5.0).all()
+        with pytest.raises(Exception, match="share"):
+            paged.paged_attention(both[:, :heads], cache, *args, out=both[:, heads - 1:2 * heads - 1])
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
