@@ -60,9 +60,8 @@ template <int N> __device__ inline void unit_offsets(const RotaryArgs& r, int ro
 
 // Bound by the stream of rows (a product and a sum a feature): a thread moves two 16-byte pieces, the two runs of its pairs, in the widest
 // loads that strides, alignment and the rotated width allow (else element by element); a workgroup takes whole tokens, so that a token's
-// position is one address for many lanes and the table rows stay in the cache.  As many pieces as threads where the launch is small (a token
-// a workgroup: latency), four a thread where it is not.  Measured: 41283 tokens x 24 heads of 64 in f32, 507 MB: 104.7 us, 4850 GB/s (a
-// copy of 1 GiB reaches 5060); 32 tokens x 16 heads in bf16: 3.1 us on the device, 7.8 with the call.
+// position is one address for many lanes and the table rows stay in the cache.  Measured: 41283 tokens x 24 heads of 64 in f32, 507 MB:
+// 94 us, 5400 GB/s (a copy of 1 GiB reaches 5060, of 256 MiB 5400); 32 tokens x 16 heads in bf16: 3.1 us on the device, 7.8 with the call.
 template <typename T, int N, bool IL>
 __global__ __launch_bounds__(256) void rotary_embed_kernel(RotaryEmbedArgs a, UnitMap m) {
     const int t0 = blockIdx.x * m.tokens_per_block;
@@ -178,18 +177,20 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, UnitMap m)
 
 SmallDiv make_div(int d) { return SmallDiv{d == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + d - 1) / d)}; }
 
-UnitMap make_map(int heads, int head_dim, int rot_dims, int n, int tokens, int most_tokens) {
+UnitMap make_map(int heads, int head_dim, int rot_dims, int n, int tokens, bool looks_up) {
     UnitMap m;
     m.uph = head_dim / (2 * n);
     m.upt = heads * m.uph;
     m.rotated = rot_dims / (2 * n);
     m.per_token = make_div(m.upt);
     m.per_head = make_div(m.uph);
-    const int64_t total = (int64_t)tokens * m.upt;
-    const int want = total <= 256 * 256 ? 256 : 1024;
-    m.tokens_per_block = want / m.upt;
+    // One unit a thread; two (the nearest number of tokens) where a launch is large and a block's look-ups have to pay.  Measured, one, two and
+    // four units in us: rotation of 41283 tokens x 24 heads of 64 in f32 94, 98.7, 106.5; appends of 24 prompts, 16 heads of 64: 64.4, 56.0, 59.0,
+    // and of 24 chunks, 16/8 heads: 11.5, 10.2, 11.3.
+    const bool two = looks_up && (int64_t)tokens * m.upt > 256 * 256;
+    m.tokens_per_block = two ? (512 + m.upt / 2) / m.upt : 256 / m.upt;
     if (m.tokens_per_block < 1) m.tokens_per_block = 1;
-    if (m.tokens_per_block > most_tokens) m.tokens_per_block = most_tokens;
+    if (looks_up && m.tokens_per_block > APPEND_TOKENS) m.tokens_per_block = APPEND_TOKENS;
     return m;
 }
 
@@ -206,7 +207,7 @@ hipError_t rotary_embed_launch(const RotaryEmbedArgs& a, int dtype, hipStream_t 
     const int esz = dtype == PTTS_BF16 ? 2 : 4, full = 16 / esz;
     const bool wide = a.rot.dims % (2 * full) == 0 && a.head_dim % (2 * full) == 0 && aligned(a.x, a.xs, 2, 16, esz) &&
                       aligned(a.out, a.os, 2, 16, esz) && aligned(a.rot.cos_t, nullptr, 0, 16, 4) && aligned(a.rot.sin_t, nullptr, 0, 16, 4);
-    const UnitMap m = make_map(a.heads, a.head_dim, a.rot.dims, wide ? full : 1, a.tokens, 1 << 20);
+    const UnitMap m = make_map(a.heads, a.head_dim, a.rot.dims, wide ? full : 1, a.tokens, false);
     const dim3 grid((a.tokens + m.tokens_per_block - 1) / m.tokens_per_block), block(256);
 #define LAUNCH(T, N)                                                                                        \
     do {                                                                                                    \
@@ -226,7 +227,7 @@ hipError_t kv_append_launch(const AppendArgs& a, int in_dtype, int cache_dtype, 
                 aligned(a.k_cache, a.kc, 3, full * csz, csz) && aligned(a.v_cache, a.vc, 3, full * csz, csz);
     if (a.q_heads) wide = wide && aligned(a.q, a.qs, 2, 16, esz) && aligned(a.q_out, a.qos, 2, 16, esz);
     if (a.rot.cos_t) wide = wide && aligned(a.rot.cos_t, nullptr, 0, 16, 4) && aligned(a.rot.sin_t, nullptr, 0, 16, 4);
-    const UnitMap m = make_map(a.q_heads + (a.v ? 2 : 1) * a.kv_heads, a.head_dim, a.rot.dims, wide ? full : 1, a.b.tokens, APPEND_TOKENS);
+    const UnitMap m = make_map(a.q_heads + (a.v ? 2 : 1) * a.kv_heads, a.head_dim, a.rot.dims, wide ? full : 1, a.b.tokens, true);
     const dim3 grid((a.b.tokens + m.tokens_per_block - 1) / m.tokens_per_block), block(256);
 #define LAUNCH(T, TC, N)                                                                                      \
     do {                                                                                                      \
