@@ -231,3 +231,41 @@ def test_a_decoder_configuration_carries_its_rotary_scaling():
     with pytest.raises(ValueError, match="type"):
         tiny_config(position_embedding="rope", rope_scaling={"type": "dynamic", "factor": 2.0})
     assert tiny_config(rope_scaling=scaling).decoder.rope_scaling is None      # no rotary positions: kept as an unknown entry, as before
+
+
+def test_scalar_addresses_of_the_asynchronous_loads_are_written_in_time(tmp_path):
+    """A vector instruction's write of a scalar register has to be five wait states old when a memory instruction reads it; hipcc sees to
+    that for instructions it models, and the loads into LDS are inline assembly.  (Scalar instructions' writes need none.)"""
+    import re
+    import subprocess
+
+    csrc = os.path.join(ROOT, "parler_tts_amd", "csrc")
+    out = tmp_path / "paged_attn.s"
+    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+                    "--cuda-device-only", "-S", os.path.join(csrc, "paged_attn.hip"), "-o", str(out)], check=True, capture_output=True)
+
+    def early(lines):
+        loads, found = 0, []
+        for i, line in enumerate(lines):
+            m = re.match(r"global_load_lds_dwordx4 v\d+, s\[(\d+):(\d+)\]", line)
+            if not m:
+                continue
+            loads += 1
+            waited = 0
+            for x in reversed(lines[max(i - 40, 0):i]):
+                if x.endswith(":"):
+                    continue
+                w = re.match(r"v_(?:readlane|readfirstlane)_b32 s(\d+)", x)
+                if w and int(m[1]) <= int(w[1]) <= int(m[2]):
+                    found.append((x, line))
+                    break
+                s = re.match(r"s_nop (\d+)", x)
+                waited += 1 + (int(s[1]) if s else 0)
+                if waited >= 5:
+                    break
+        return loads, found
+
+    text = [t.split(";")[0].strip() for t in out.read_text().split("\n")]
+    loads, found = early([t for t in text if t and (not t.startswith(".") or t.startswith(".LBB"))])
+    assert loads > 100 and not found, found[:3]
+    assert early(["v_readlane_b32 s5, v1, 3", "s_mov_b32 m0, s9", "s_nop 0", "global_load_lds_dwordx4 v2, s[4:5]"])[1]
