@@ -39,17 +39,6 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda in
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _launch(index: int, entry, *args) -> None:
-    """one C entry on the current stream of device `index`, which is made the current device for the call if it is not"""
-    if index == _current_device():
-        rc = entry(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = entry(*args, _raw_stream(index))
-    if rc:
-        _hip.check(rc)
-
-
 def _read_status(status: torch.Tensor, who: str) -> None:
     bits = int(status.item())
     if bits:
@@ -221,9 +210,14 @@ def rotary_embed(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, 
             raise ValueError(f"out of {out.dtype} for x of {x.dtype}")
     if heads == 0 or tokens == 0:
         return out
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return rotary_embed(x, positions, rotary, out)
     xs, os = x.stride(), out.stride()
-    _launch(index, _hip.load_library().ptts_rotary_embed, rotary._ref, _DTYPES[x.dtype], tokens, heads, rotary.head_dim, x.data_ptr(),
-            xs[0], xs[1], positions.data_ptr(), out.data_ptr(), os[0], os[1], rotary._status)
+    rc = _hip.load_library().ptts_rotary_embed(rotary._ref, _DTYPES[x.dtype], tokens, heads, rotary.head_dim, x.data_ptr(), xs[0], xs[1],
+                                               positions.data_ptr(), out.data_ptr(), os[0], os[1], rotary._status, _raw_stream(index))
+    if rc:
+        _hip.check(rc)
     return out
 
 
@@ -270,8 +264,13 @@ def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, table: torc
         raise ValueError("q_out without q")
     if tokens == 0:
         return q_out
-    _launch(index, _hip.load_library().ptts_kv_append, cache._ref, C.addressof(batch), _DTYPES[k.dtype], k.data_ptr(), ks[0], ks[1],
-            v.data_ptr(), vs[0], vs[1], rot, at, heads, qp, qs[0], qs[1], qop, qos[0], qos[1], cache._status)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return kv_append(cache, k, v, table, past, starts, rotary=rotary, positions=positions, q=q, q_out=q_out)
+    rc = _hip.load_library().ptts_kv_append(cache._ref, C.addressof(batch), _DTYPES[k.dtype], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                                            rot, at, heads, qp, qs[0], qs[1], qop, qos[0], qos[1], cache._status, _raw_stream(index))
+    if rc:
+        _hip.check(rc)
     return q_out
 
 
@@ -315,6 +314,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
             raise ValueError(f"out of {out.dtype} for q of {q.dtype}")
     if tokens == 0:
         return out
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return paged_attention(q, cache, table, past, starts, scale=scale, causal=causal, key_mask=key_mask, max_new=max_new, out=out)
     lib = _hip.load_library()
     bref = C.addressof(batch)
     key = (tokens, batch.n_seqs, batch.max_pages, heads, max_new, starts is None)
@@ -328,7 +330,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
         cache._workspace[key] = need
     workspace = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
     qs, os = q.stride(), out.stride()
-    _launch(index, lib.ptts_paged_attention, cache._ref, bref, heads, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
-            dim ** -0.5 if scale is None else scale, 1 if causal else 0, mask, mask_stride, mask_width, max_new,
-            workspace.data_ptr() if need else None, need, cache._status)
+    rc = lib.ptts_paged_attention(cache._ref, bref, heads, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
+                                  dim ** -0.5 if scale is None else scale, 1 if causal else 0, mask, mask_stride, mask_width, max_new,
+                                  workspace.data_ptr() if need else None, need, cache._status, _raw_stream(index))
+    if rc:
+        _hip.check(rc)
     return out
