@@ -159,13 +159,14 @@ struct Item {
     bool bad;                   // the length leads behind the row of the page table: every row becomes NaN
 };
 
-// SORTED: of every 64 sequences the longest first, so that what starts last is short.
+// SORTED (and by_length): of every 64 sequences the longest first, so that what starts last is short.
 template <int M, int KT, bool SORTED> struct Schedule {
     int seq, first, n, past;    // this lane's sequence of the current 64
     int base;                   // number of the first of these
     int sum, own;               // (tile, share) pairs of the lane's sequence, and of all up to it
     int share;                  // tiles of KT keys of a share (of all keys: not cut)
     int items;                  // pairs of the batch
+    bool by_length = true;      // sort at all (few items have a CU each, in any order)
 
     __device__ __forceinline__ void load(const PagedAttnArgs& a, int i0) {
         const int lane = threadIdx.x & 63, i = min(i0 + lane, a.n_seqs - 1);
@@ -271,7 +272,7 @@ template <int M, int KT, bool SORTED> struct Schedule {
     __device__ __forceinline__ void number(const PagedAttnArgs& a) {
         items = 0;
         for (int i0 = 0;;) {
-            if (SORTED) sort(a);
+            if (SORTED && by_length) sort(a);
             count(a);
             items += __builtin_amdgcn_readlane(sum, 63);
             i0 += 64;
@@ -288,7 +289,7 @@ template <int M, int KT, bool SORTED> struct Schedule {
         } else if (a.n_seqs > 64) {
             load(a, 0);
             for (;;) {
-                if (SORTED) sort(a);
+                if (SORTED && by_length) sort(a);
                 count(a);
                 const int here = __builtin_amdgcn_readlane(sum, 63);
                 if (t < here || base + 64 >= a.n_seqs) break;
@@ -421,8 +422,10 @@ struct Pages {
 // Rows at or behind `end` are read from the last row in front of it: what lies there is seen by nobody, and may be anything.  A wave
 // instruction moves RPI rows, which share a page (pages hold 16 tokens or more); its address is a scalar base and a 32-bit lane offset
 // (slot strides are below 2^27 bytes).  The LDS-DMA is written out: behind its builtin hipcc drains every transfer in flight in front of
-// the next transposing read, wherever that reads.  It has no register results; the kernels wait for it by counted vmcnt.
-template <typename P, int D> struct Rows {
+// the next transposing read, wherever that reads.  It has no register results; the kernels wait for it by counted vmcnt.  ONCE: rows that no
+// other workgroup reads pass the caches by (32 x 2000 keys, 16 heads of 64: 45.9 us, 51.9 through them; chunks, whose tiles share their keys,
+// lose as much: 4 prompts of 1024 over 2 heads of 128 38, 35).
+template <typename P, int D, bool ONCE = false> struct Rows {
     static constexpr int RB = D * (int)sizeof(typename P::elem_t), RPI = 1024 / RB, CPR = RB / 16;
     const char* base;
     int64_t page_bytes;
@@ -450,7 +453,9 @@ template <typename P, int D> struct Rows {
     }
     static __device__ __forceinline__ void send(const char* src, unsigned off, unsigned lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(src) : "memory");
+        const int to = __builtin_amdgcn_readfirstlane(lds);
+        if constexpr (ONCE) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(to), "v"(off), "s"(src) : "memory");
+        else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(src) : "memory");
 #endif
     }
     // 16 rows that are all there (key a multiple of 16: they share a page), one instruction a time
@@ -1017,8 +1022,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
 // Few rows (at most 16 per sequence and key head: single tokens, their groups, short drafts): bound by the stream of the cache.  A wave
 // owns every NW-th tile of 32 (f32: 16) keys and two LDS buffers of its own, so that nothing in the loop waits for another wave; the waves'
 // states are joined once at the end.
-// Measured: 32 sequences of 700 - 2579 keys, 16 heads of 64 in bf16: 46 us, 4760 GB/s; two of 120001 - 131070 keys, 32 heads of 128 over 4:
-// 93 us and 5 of the join, 5150 GB/s; a copy of 1 GiB reaches 5060.  One sequence of up to 700 keys is a chain of dependent trips: 7 us.
+// Lengths in order, long beside short on a CU: 32 sequences of 100 - 2500 keys, 16 heads of 64 33 us, as they come 40; up to 8 tokens each 33, 37.
+// Measured: 32 sequences of 700 - 2579 keys, 16 heads of 64 in bf16: 40 us, 5450 GB/s; two of 120001 - 131070 keys, 32 heads of 128 over 4:
+// 92 us and 5 of the join, 5150 GB/s; a copy of 1 GiB reaches 5060.  One sequence of up to 700 keys is a chain of dependent trips: 7 us.
 // =================================================================================================================================
 template <typename P, int D> struct StepCfg {
     static constexpr int M = 16, KT = P::IS_BF16 ? 32 : 16;
@@ -1036,22 +1042,36 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_step_kernel(PagedAttnArgs 
     __shared__ __attribute__((aligned(1024))) char smem[NW * 2 * C::STAGE];
     const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
 
-    Schedule<C::M, KT, false> sched;
+    Schedule<C::M, KT, true> sched;
+    sched.by_length = a.n_seqs <= 64 && a.n_seqs * a.kv_heads > SLOTS / 2;
     Item it;
     int kvh;
     const int item = blockIdx.x;
     if (!a.starts && a.splits == 1) {        // one token each, whole: items follow from their numbers
-        const int tiles = (a.group + C::M - 1) / C::M, at = int_div(item, a.by_kv_heads), q = tiles == 1 ? at : at / tiles;
-        kvh = item - at * a.kv_heads;
-        it.seq = it.first = q;
+        const int tiles = (a.group + C::M - 1) / C::M, all = a.n_seqs * tiles * a.kv_heads;
+        const bool order = all > SLOTS / 2 && a.n_seqs <= 64;          // long ones first, up to two on a CU beside short ones, as in chunks
+        const int number = order && all <= SLOTS && item >= SLOTS / 2 ? all - 1 - (item - SLOTS / 2) : item;
+        const int at = int_div(number, a.by_kv_heads), q = tiles == 1 ? at : at / tiles;
+        kvh = number - at * a.kv_heads;
         it.n = 1;
-        it.past = a.past[q];
+        if (order) {
+            sched.load(a, 0);
+            sched.sort(a);
+            it.seq = __builtin_amdgcn_readlane(sched.seq, q);
+            it.past = __builtin_amdgcn_readlane(sched.past, q);
+        } else {
+            it.seq = q;
+            it.past = a.past[q];
+        }
+        it.first = it.seq;
         sched.place(a, at - q * tiles, &it);
     } else {
         begin(a, sched, STEP_LAG);
-        if (item >= sched.items * a.kv_heads) return;
-        const int at = int_div(item, a.by_kv_heads);
-        kvh = item - at * a.kv_heads;
+        const int all = sched.items * a.kv_heads;
+        if (item >= all) return;
+        const int number = sched.by_length && all > SLOTS / 2 && all <= SLOTS && item >= SLOTS / 2 ? all - 1 - (item - SLOTS / 2) : item;
+        const int at = int_div(number, a.by_kv_heads);
+        kvh = number - at * a.kv_heads;
         sched.find(a, at, &it, a.sched);
     }
     if (it.split >= it.splits) return;
@@ -1065,7 +1085,7 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_step_kernel(PagedAttnArgs 
 
     Pages pg;
     pg.row = a.table + it.seq * a.table_stride; pg.n_pages = a.n_pages; pg.bad = false; pg.base = 0; pg.ids = 0;
-    const Rows<P, D> krows(a.k, a.kc, kvh), vrows(a.v, a.vc, kvh);
+    const Rows<P, D, true> krows(a.k, a.kc, kvh), vrows(a.v, a.vc, kvh);
     const unsigned ring = lds_address(smem) + w * 2 * C::STAGE;
     const int first = k0 + w * KT;
     auto fetch = [&](int key0, int buf) {
