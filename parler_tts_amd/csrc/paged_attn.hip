@@ -422,9 +422,9 @@ struct Pages {
 // Rows at or behind `end` are read from the last row in front of it: what lies there is seen by nobody, and may be anything.  A wave
 // instruction moves RPI rows, which share a page (pages hold 16 tokens or more); its address is a scalar base and a 32-bit lane offset
 // (slot strides are below 2^27 bytes).  The LDS-DMA is written out: behind its builtin hipcc drains every transfer in flight in front of
-// the next transposing read, wherever that reads.  It has no register results; the kernels wait for it by counted vmcnt.  ONCE: rows that no
-// other workgroup reads pass the caches by (32 x 2000 keys, 16 heads of 64: 45.9 us, 51.9 through them; chunks, whose tiles share their keys,
-// lose as much: 4 prompts of 1024 over 2 heads of 128 38, 35).
+// the next transposing read, wherever that reads.  It has no register results; the kernels wait for it by counted vmcnt.  ONCE: rows that one
+// workgroup reads, as a rule, are not kept by the caches (32 x 2000 keys, 16 heads of 64: 45.9 us, kept 51.9; where all sequences share their
+// pages 29.4, 28.8; chunks, whose tiles share their keys, lose by it: 4 prompts of 1024 over 2 heads of 128 38, 35).
 template <typename P, int D, bool ONCE = false> struct Rows {
     static constexpr int RB = D * (int)sizeof(typename P::elem_t), RPI = 1024 / RB, CPR = RB / 16;
     const char* base;
@@ -1043,13 +1043,15 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_step_kernel(PagedAttnArgs 
     const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
 
     Schedule<C::M, KT, true> sched;
-    sched.by_length = a.n_seqs <= 64 && a.n_seqs * a.kv_heads > SLOTS / 2;
+    // up to 512 keys the order saves less than it takes (32 x 201 keys, 16 heads: 6.9 us, in order 7.5)
+    const bool unequal = a.n_seqs <= 64 && (a.max_pages << a.page_shift) > 512;
+    sched.by_length = unequal && a.n_seqs * a.kv_heads > SLOTS / 2;
     Item it;
     int kvh;
     const int item = blockIdx.x;
     if (!a.starts && a.splits == 1) {        // one token each, whole: items follow from their numbers
         const int tiles = (a.group + C::M - 1) / C::M, all = a.n_seqs * tiles * a.kv_heads;
-        const bool order = all > SLOTS / 2 && a.n_seqs <= 64;          // long ones first, up to two on a CU beside short ones, as in chunks
+        const bool order = unequal && all > SLOTS / 2;          // long ones first, up to two on a CU beside short ones, as in chunks
         const int number = order && all <= SLOTS && item >= SLOTS / 2 ? all - 1 - (item - SLOTS / 2) : item;
         const int at = int_div(number, a.by_kv_heads), q = tiles == 1 ? at : at / tiles;
         kvh = number - at * a.kv_heads;
