@@ -497,7 +497,7 @@ __device__ __forceinline__ void row_alone(const PagedAttnArgs& a, int seq, int k
         int page = -1;
         if (j < k1 && (!a.mask || j >= a.mask_width || a.mask[seq * a.mask_stride + j])) {
             page = table[j >> a.page_shift];
-            if ((unsigned)page >= (unsigned)a.n_pages) page = 0;        // the caller of this has found it already
+            if ((unsigned)page >= (unsigned)a.n_pages) page = 0;        // rows that meet a bad page are NaN and do not come here
             const elem_t* kp = kb + page * a.kc[0] + (j & mask) * a.kc[2];
             float d = 0.f;
             for (int c = 0; c < D; c += V) {
@@ -1031,7 +1031,7 @@ template <typename P, int D> struct StepCfg {
     static constexpr int RB = D * (int)sizeof(typename P::elem_t);
     static constexpr int TILE = KT * RB, STAGE = 2 * TILE;
     static constexpr int DMA = STAGE / 1024;
-    static_assert(16 * (D + 2) * 4 <= 2 * STAGE, "the waves' states fit where their tiles were");
+    static_assert(16 * (D + 2) * 4 + 4 <= 2 * STAGE, "the waves' states fit where their tiles were");
 };
 
 template <typename P, int D, int NW>
@@ -1194,14 +1194,20 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_step_kernel(PagedAttnArgs 
     l += __shfl_xor(l, 32);
     if (pg.bad || it.bad) l = NAN;
 
-    // join the waves: outputs [NW][16][D] (16-byte pieces XOR-swizzled by the row) and maxima, sums [NW][16] in the place of the tiles
+    // join the waves: outputs [NW][16][D] (16-byte pieces XOR-swizzled by the row), maxima, sums [NW][16] and whether the wave met a bad page
+    // [NW] in the place of the tiles
     __syncthreads();
     float* sm = reinterpret_cast<float*>(smem) + NW * 16 * D;
+    int* met_bad = reinterpret_cast<int*>(sm + 2 * NW * 16);
 #pragma unroll
     for (int d = 0; d < NDB; ++d)
         *reinterpret_cast<f32x4*>(smem + ((w * 16 + l15) * D + (((d * 4 + g) ^ (l15 & 7)) << 2)) * 4) = o[d];
     if (g == 0) { sm[w * 16 + l15] = m; sm[(NW + w) * 16 + l15] = l; }
+    if (lane == 0) met_bad[w] = pg.bad;
     __syncthreads();
+    bool bad = it.bad;                       // every wave looks at the pages of its own tiles, and finishes rows of all
+#pragma unroll
+    for (int v = 0; v < NW; ++v) bad = bad || met_bad[v] != 0;
     constexpr int PPR = D / 4;               // pieces per row
     for (int i = threadIdx.x; i < 16 * PPR; i += NW * 64) {
         const int q = i / PPR, piece = i % PPR, rr = r0 + q;
@@ -1219,7 +1225,6 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_step_kernel(PagedAttnArgs 
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[j] = fmaf(x[j], f[v], acc[j]);
         }
-        const bool ruined = sum != sum && (pg.bad || it.bad);
         const float z = fmaf(acc[0], 0.f, fmaf(acc[1], 0.f, fmaf(acc[2], 0.f, fmaf(acc[3], 0.f, sum * 0.f))));
         const int tk = on ? int_div(rr, a.by_group) : 0, hd = kvh * a.group + (on ? rr - tk * a.group : 0);
         const int64_t t64 = it.first + tk;
@@ -1234,7 +1239,7 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_step_kernel(PagedAttnArgs 
             }
         }
         // rows of this wave's pieces whose result is not finite (64 lanes hold 64 / PPR rows), again and alone
-        uint64_t odds = __ballot(on && !ruined && !(z == 0.f));
+        uint64_t odds = __ballot(on && !bad && !(z == 0.f));
         while (odds) {
             const int src = __builtin_ctzll(odds), rw = (i - lane + src) / PPR;
             const uint64_t same = PPR == 64 ? ~0ull : (((1ull << PPR) - 1) << (src / PPR * PPR));
