@@ -425,7 +425,7 @@ int attn_args(const ptts_paged_kv* cache, const ptts_paged_batch* batch, int32_t
     if (q_heads <= 0 || q_heads % cache->kv_heads) REFUSE(PTTS_E_INVALID, "%d query heads over %d key heads", q_heads, cache->kv_heads);
     if (q_heads > 65535) REFUSE(PTTS_E_UNSUPPORTED, "%d query heads", q_heads);
     if (max_new < 0) REFUSE(PTTS_E_INVALID, "max_new %d", max_new);
-    if ((int64_t)batch->max_pages * cache->page_tokens > INT_MAX - 4096) REFUSE(PTTS_E_UNSUPPORTED, "a page table row reaches past 2^31 tokens");
+    if ((int64_t)batch->max_pages * cache->page_tokens > INT_MAX - 4095) REFUSE(PTTS_E_UNSUPPORTED, "a page table row reaches past 2^31 - 4096 tokens");
     if ((int64_t)batch->tokens * (q_heads / cache->kv_heads) > INT_MAX - 65536) REFUSE(PTTS_E_UNSUPPORTED, "too many query rows");
     *a = PagedAttnArgs();
     a->k = cache->k; a->v = cache->v;

@@ -322,7 +322,8 @@ template <int M, int KT, bool SORTED> struct Schedule {
         it->splits = a.splits > 1 ? shares(kt) : 1;
         it->k0 = 0;
         it->k1 = it->end;
-        if (it->splits > 1) { it->k0 = min(it->split * share * KT, it->end); it->k1 = min(it->k0 + share * KT, it->end); }
+        // a share is shorter than the keys it is cut from; the end of the last one may lie past 2^31
+        if (it->splits > 1) { it->k0 = min(it->split * share * KT, it->end); it->k1 = it->k0 + min(share * KT, it->end - it->k0); }
     }
 };
 

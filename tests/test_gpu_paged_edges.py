@@ -36,3 +36,26 @@ def test_every_head_of_a_row_that_meets_a_bad_page_is_nan(paged, page, heads, kv
                 close(got[1:], want[1:], bound[1:], "the other sequence")
                 with pytest.raises(PttsError, match="page id"):
                     cache.check()
+
+
+@pytest.mark.parametrize("kv_heads,keys", [(3, 2143000000), (3, 2 ** 31 - 4096), (1, 2 ** 31 - 8192)])
+def test_contexts_near_the_largest(paged, kv_heads, keys):
+    """Two pages of 4096 tokens under a context of two thousand million keys: zeros everywhere but on the last page, whose keys score 13 and
+    hold ones.  The weights' sum counts whole numbers in float32 (less than 2^24 per lane), the last page's share of it is exact but
+    for the exponential (argument 13 log2(e) = 18.8, off by 2 roundings, exp2 by one more: 2^-18 relative) and 257 additions of shares; then
+    the output's rounding."""
+    page, dim = 4096, 64
+    pages = -(-keys // page)
+    k = torch.zeros(2, kv_heads, page, dim, dtype=BF)
+    k[1] = 1.625                                                          # 64 x 1.625 / 8 = 13
+    v = torch.zeros_like(k)
+    v[1] = 1.0
+    table = torch.zeros(1, pages, dtype=torch.int32)
+    table[0, -1] = 1
+    cache = paged.PagedKVCache.from_tensors(k.cuda(), v.cuda())
+    got = paged.paged_attention(torch.ones(1, kv_heads, dim, dtype=BF, device="cuda"), cache, table.cuda(), ints([keys - 1]))
+    last = keys - (pages - 1) * page
+    want = last * math.exp(13.0) / (last * math.exp(13.0) + (keys - last))
+    assert want > 0.2
+    assert (got.double() - want).abs().max() <= want * (2.0 ** -8 + 2.0 ** -17 + 260 * 2.0 ** -24)
+    cache.check()
