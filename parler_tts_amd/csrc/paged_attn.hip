@@ -175,7 +175,7 @@ template <int M, int KT, bool SORTED> struct Schedule {
         if (a.starts) {
             first = a.starts[i];
             const int end = a.starts[i + 1];
-            n = first >= 0 && end <= a.tokens ? max(end - first, 0) : 0;      // starts that are wrong own no rows
+            n = first >= 0 && end > first && end <= a.tokens ? end - first : 0;      // starts that are wrong own no rows
         } else { first = i; n = 1; }
         past = a.past[i];
         if (i0 + lane >= a.n_seqs) n = 0;

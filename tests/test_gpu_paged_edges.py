@@ -59,3 +59,27 @@ def test_contexts_near_the_largest(paged, kv_heads, keys):
     assert want > 0.2
     assert (got.double() - want).abs().max() <= want * (2.0 ** -8 + 2.0 ** -17 + 260 * 2.0 ** -24)
     cache.check()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("seqs", [3, 100, 300])
+@pytest.mark.parametrize("max_new", [0, 1])
+def test_starts_at_the_ends_of_their_type_own_no_rows(paged, max_new, seqs, dtype):
+    """an end of -2^31 behind a first token of 5 would be 2^31 - 5 tokens in 32-bit arithmetic"""
+    from parler_tts_amd._hip import PttsError
+
+    low, high = -2 ** 31, 2 ** 31 - 1
+    page, heads, dim, total = 16, 4, 64, 20
+    kc, vc, q = rnd(2, 2, 2, page, dim, dtype=dtype), rnd(3, 2, 2, page, dim, dtype=dtype), rnd(1, total, heads, dim, dtype=dtype)
+    cache = paged.PagedKVCache.from_tensors(kc.cuda(), vc.cuda())
+    table = torch.tensor([[0, 1]], dtype=torch.int32).expand(seqs, -1).contiguous()
+    past = [3] * seqs
+    want, bound = ref.attend(q, kc, vc, table, past[:1], [0, 5], dim ** -0.5)
+    for tail in ([low, total], [low, high], [high, low], [low + 1, high], [high, total]):
+        starts = [0] + [5] * (seqs - 2) + tail
+        out = torch.full(q.shape, 5.0, dtype=dtype, device="cuda")
+        paged.paged_attention(q.cuda(), cache, table.cuda(), ints(past), ints(starts), max_new=max_new, out=out)
+        close(out[:5], want[:5], bound[:5], tail)
+        assert (out[5:] == 5.0).all(), tail
+        with pytest.raises(PttsError, match="starts"):
+            cache.check()
