@@ -344,7 +344,9 @@ int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, in
 /* out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j].  causal: token i of sequence s sees the keys 0 .. past[s] + i (the new tokens are in
  * the cache); else all of 0 .. past[s] - 1 (encoder states, say).  key_mask [n_seqs][mask_stride] bytes: keys j < mask_width with a zero
  * are no keys; whatever they hold does not reach the output.  A token that sees no key gets zeros; rows that a bad page or length concerns
- * get NaN; rows of no sequence (behind the last, or where starts are wrong) are left as they are.  Query head h reads key head h / (q_heads / kv_heads).  q, out: [tokens][q_heads][head_dim] of the cache's type.
+ * get NaN; rows of no sequence (behind the last, or where starts are wrong) are left as they are, rows that descending starts give to
+ * several hold the result of one of these.  Query head h reads key head h / (q_heads / kv_heads).  q, out: [tokens][q_heads][head_dim] of
+ * the cache's type.
  * max_new: an upper bound of the new tokens of one sequence, 0 = not known; it picks the kernel, never the result's validity.
  * workspace: ptts_paged_attention_workspace() bytes (may be 0; negative = PTTS_E_*) at a multiple of 16, not shared with another call
  * in flight. */

@@ -168,6 +168,11 @@ template <int M, int KT, bool SORTED> struct Schedule {
     int items;                  // pairs of the batch
     bool by_length = true;      // sort at all (few items have a CU each, in any order)
 
+    // Starts that descend can give the same rows to any number of sequences: sums over groups stay at the largest number instead of wrapping,
+    // so that they ascend whatever starts say.  (64 sequences cannot wrap: each has 2^25 - 1024 tiles at most, see make_plan.)
+    static __host__ __device__ __forceinline__ int add_items(int x, int y) { return x > 0x7fffffff - y ? 0x7fffffff : x + y; }
+    __device__ __forceinline__ int launch_items(const PagedAttnArgs& a) const { return (int)min((int64_t)items * a.kv_heads, (int64_t)0x7fffffff); }
+
     __device__ __forceinline__ void load(const PagedAttnArgs& a, int i0) {
         const int lane = threadIdx.x & 63, i = min(i0 + lane, a.n_seqs - 1);
         base = i0;
@@ -274,7 +279,7 @@ template <int M, int KT, bool SORTED> struct Schedule {
         for (int i0 = 0;;) {
             if (SORTED && by_length) sort(a);
             count(a);
-            items += __builtin_amdgcn_readlane(sum, 63);
+            items = add_items(items, __builtin_amdgcn_readlane(sum, 63));
             i0 += 64;
             if (i0 >= a.n_seqs) break;
             load(a, i0);
@@ -393,8 +398,8 @@ __global__ __launch_bounds__(1024) void paged_attn_schedule_kernel(PagedAttnArgs
         int before = item_at, tiles_before = tile_at;
         for (int i = 0; i < 16; ++i) {
             if (i == w && g < groups && lane == 0) { item0[g] = before; tile0[g] = tiles_before; }
-            before += items[i];
-            tiles_before += tiles[i];
+            before = sc.add_items(before, items[i]);
+            tiles_before = sc.add_items(tiles_before, tiles[i]);
         }
         item_at = before;
         tile_at = tiles_before;
@@ -599,7 +604,7 @@ __global__ __launch_bounds__(256, (D == 64 ? 3 : 2)) void paged_attn_chunk_kerne
 
     Schedule<C::M, KT, true> sched;
     begin(a, sched, TILE_LAG);
-    const int all = sched.items * a.kv_heads;
+    const int all = sched.launch_items(a);
     int item = blockIdx.x;
     if (item >= all) return;
     // up to two on a CU: the longest item beside the shortest (4 prompts of 1024, 16 heads of 128 over 2: 34 us, in order 41)
@@ -868,7 +873,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(PagedAttnArgs a
     Schedule<C::M, KT, true> sched;
     begin(a, sched, TILE_LAG);
     const int item = blockIdx.x;
-    if (item >= sched.items * a.kv_heads) return;
+    if (item >= sched.launch_items(a)) return;
     const int at = int_div(item, a.by_kv_heads), kvh = item - at * a.kv_heads;
     Item it;
     sched.find(a, at, &it, a.sched);
@@ -1070,7 +1075,7 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_step_kernel(PagedAttnArgs 
         sched.place(a, at - q * tiles, &it);
     } else {
         begin(a, sched, STEP_LAG);
-        const int all = sched.items * a.kv_heads;
+        const int all = sched.launch_items(a);
         if (item >= all) return;
         const int number = sched.by_length && all > SLOTS / 2 && all <= SLOTS && item >= SLOTS / 2 ? all - 1 - (item - SLOTS / 2) : item;
         const int at = int_div(number, a.by_kv_heads);
@@ -1271,7 +1276,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
         sched.load(a, 0);
         sched.number(a);
     }
-    if (t >= sched.items * a.kv_heads) return;
+    if (t >= sched.launch_items(a)) return;
     const int at = int_div(t, a.by_kv_heads), kvh = t - at * a.kv_heads;
     Item it;
     sched.find(a, at, &it, a.sched + groups + 1);
@@ -1364,6 +1369,8 @@ Plan make_plan(const PagedAttnArgs& a, int max_new, int head_dim, int dtype) {
     const int64_t keys = (int64_t)a.max_pages << a.page_shift;
     const bool more_rows = most > 16 && most <= 128 && keys * row_of_cache <= 131072 && a.n_seqs * a.kv_heads * ((most + 15) / 16) <= 256;
     p.step = (most > 0 && most <= 16) || more_rows;
+    // the tiles of 64 sequences are summed in 32 bits, and starts may give all rows to each of them
+    if (a.starts && (int64_t)a.tokens * a.group > ((int64_t)1 << 29) - 65536) p.step = false;
     const int M = p.step ? 16 : (dtype == PTTS_BF16 ? 128 : 64);
     const int64_t ub = a.starts ? (int64_t)a.tokens * a.group / M + a.n_seqs : (int64_t)a.n_seqs * ((a.group + M - 1) / M);
     p.tiles = (int)ub;

@@ -12,7 +12,8 @@ the caller owns (grouped heads, head dim 64 or 128, float32 or bfloat16), as cal
 this call, ``starts`` [sequences + 1] int32 where its new tokens begin in q / k / v (None: one new token each).  They are read on the
 device when the work runs, so a captured graph serves other lengths after an in-place update.  What they say wrongly is never followed
 out of a buffer: it sets ``cache.status`` / ``rotary.status``, which ``check()`` turns into an error, and the rows concerned come out as
-zeros (``kv_append``, ``rotary_embed``) or NaN (``paged_attention``; where ``starts`` are wrong, as ``out`` held them).
+zeros (``kv_append``, ``rotary_embed``) or NaN (``paged_attention``; where ``starts`` are wrong, as ``out`` held them or one
+of the sequences' that claim them).
 
 Work goes to the current stream of the tensors' device and nothing is synchronised.  No gradients: forward only.
 """
@@ -286,7 +287,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
     ``max_new``: the longest sequence's number of new tokens if the caller knows it (it helps to pick the kernel; 0: unknown).
     Rows of ``q`` and ``out`` start at multiples of 16 bytes and share no memory.
     Sequences may share pages, or (an expanded ``table``) all of them.  Rows of no sequence (behind the last, or where ``starts`` are wrong)
-    are left as they are in ``out``."""
+    are left as they are in ``out``; rows that descending ``starts`` give to several hold the result of one of these."""
     index, dim = cache._index, cache.head_dim
     tokens = q.shape[0]
     _rows("q", q, None, None, dim, index)

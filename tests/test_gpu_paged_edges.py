@@ -83,3 +83,25 @@ def test_starts_at_the_ends_of_their_type_own_no_rows(paged, max_new, seqs, dtyp
         assert (out[5:] == 5.0).all(), tail
         with pytest.raises(PttsError, match="starts"):
             cache.check()
+
+
+@pytest.mark.parametrize("max_new,seqs", [(0, 1 << 21), (1, 1 << 18)], ids=["chunks", "few rows"])
+def test_descending_starts_that_give_all_rows_to_every_other_sequence(paged, max_new, seqs):
+    """2^31 tiles by number: counts stay at the largest number and ascend.  All sequences read the same keys, so that every row has one result."""
+    from parler_tts_amd._hip import PttsError
+
+    tokens, heads, dim, page = 1 << 15, 8, 64, 16
+    kc, vc, q = rnd(2, 1, 1, page, dim, dtype=BF), rnd(3, 1, 1, page, dim, dtype=BF), rnd(1, tokens, heads, dim, dtype=BF).cuda()
+    cache = paged.PagedKVCache.from_tensors(kc.cuda(), vc.cuda())
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    starts = torch.zeros(seqs + 1, dtype=torch.int32, device="cuda")
+    starts[1::2] = tokens
+    past = torch.full((seqs,), page, dtype=torch.int32, device="cuda")
+    got = paged.paged_attention(q, cache, table.expand(seqs, -1), past, starts, causal=False, max_new=max_new)
+    with pytest.raises(PttsError, match="starts"):
+        cache.check()
+    want = paged.paged_attention(q, cache, table, past[:1], ints([0, tokens]), causal=False, max_new=max_new)
+    assert torch.equal(got, want)
+    one, bound = ref.attend(q[:64].cpu(), kc, vc, table.cpu(), [page], [0, 64], dim ** -0.5, causal=False)
+    close(got[:64], one, bound)
+    cache.check()
