@@ -333,7 +333,8 @@ int ptts_rotary_embed(const ptts_rotary* rot, int32_t dtype, int32_t tokens, int
                       int64_t out_head_stride, int32_t* status, void* stream);
 
 /* Token i of sequence s goes to slot past[s] + i: k turned by `rot` (NULL: as it is) at its slot, or at positions[token] where
- * positions is given; v as it is.  q (optional: q_heads > 0) is turned at the same positions into q_out, which may be q.
+ * positions is given; v as it is.  q (optional: q_heads > 0) is turned at the same positions into q_out, which may be q, but
+ * shares no memory with k or v.
  * dtype is that of k, v and q; f32 rows may go into a bf16 cache (rounded once, behind the rotation).  A token that cannot be placed
  * leaves the cache as it is and its row of q_out becomes zero; rows behind the last sequence are left as they are. */
 int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, int32_t dtype, const void* k, int64_t k_token_stride,

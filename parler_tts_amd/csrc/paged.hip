@@ -318,16 +318,62 @@ int check_rows(const char* name, const void* p, const int64_t* st, int64_t token
     return PTTS_OK;
 }
 
-// whether the byte ranges of two strided tensors of rows meet; slices of one buffer's rows (the same token stride) may lie beside each other
-bool ranges_meet(const void* a, const int64_t* as, const void* b, const int64_t* bs, int64_t tokens, int64_t heads, int64_t d, int esz) {
-    const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
-    const uintptr_t ea = pa + (uintptr_t)(((tokens - 1) * as[0] + (heads - 1) * as[1] + d) * esz);
-    const uintptr_t eb = pb + (uintptr_t)(((tokens - 1) * bs[0] + (heads - 1) * bs[1] + d) * esz);
-    if (!(pa < eb && pb < ea)) return false;
-    const int64_t stride = as[0] * esz, la = ((heads - 1) * as[1] + d) * esz, lb = ((heads - 1) * bs[1] + d) * esz;
-    if (as[0] != bs[0] || la > stride || lb > stride) return true;
-    const int64_t apart = pb >= pa ? (int64_t)((pb - pa) % (uintptr_t)stride) : (stride - (int64_t)((pa - pb) % (uintptr_t)stride)) % stride;
-    return apart < la || apart + lb > stride;
+// a tensor of rows of `inner` contiguous elements
+struct Strided { const void* p; const int64_t *st, *n; int dims, esz; int64_t inner; };
+
+// Whether two of them have a byte in common: whether the distance of their first bytes plus indices times strides plus places within the rows
+// can be 0.  Indices of equal strides count as one (their difference), as slices of one buffer's rows have them.  Places that reach
+// everything between two ends are an interval; a stride no longer than it extends it, the longer ones are tried, longest first (few of a
+// stride can fit, where the shorter ones reach less far than it).  Exact, up to 4096 trials; what would take more counts as shared.
+struct Meeting {
+    int64_t st[6], lo[6], hi[6];     // bytes, least and largest index; ascending
+    int64_t low, high;               // the interval
+    int dims = 0, trials = 0;
+    void add(int64_t s, int64_t l, int64_t h) {
+        int i = dims++;
+        for (; i > 0 && st[i - 1] > s; --i) { st[i] = st[i - 1]; lo[i] = lo[i - 1]; hi[i] = hi[i - 1]; }
+        st[i] = s; lo[i] = l; hi[i] = h;
+    }
+    static int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }       // b > 0
+    bool reaches(int64_t x, int left) {        // 0 from x, by the first `left` strides and the interval
+        if (++trials > 4096) return true;
+        if (left == 0) return x + low <= 0 && x + high >= 0;
+        int64_t l = low, h = high;
+        for (int i = 0; i < left - 1; ++i) { l += lo[i] * st[i]; h += hi[i] * st[i]; }
+        const int64_t s = st[left - 1];
+        const int64_t from = -floor_div(x + h, s), to = floor_div(-x - l, s);
+        for (int64_t d = from > lo[left - 1] ? from : lo[left - 1]; d <= to && d <= hi[left - 1]; ++d)
+            if (reaches(x + d * s, left - 1)) return true;
+        return false;
+    }
+};
+
+int64_t bytes_spanned(const Strided& t) {
+    int64_t e = t.inner;
+    for (int i = 0; i < t.dims; ++i) e += (t.n[i] - 1) * t.st[i];
+    return e * t.esz;
+}
+
+bool share_memory(const Strided& a, const Strided& b) {
+    const uintptr_t pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
+    if (pb >= pa ? (int64_t)(pb - pa) >= bytes_spanned(a) : (int64_t)(pa - pb) >= bytes_spanned(b)) return false;
+    Meeting m;
+    bool taken[3] = {false, false, false};
+    for (int i = 0; i < a.dims; ++i) {
+        if (a.n[i] <= 1 || a.st[i] == 0) continue;
+        int64_t hi = 0;
+        for (int j = 0; j < b.dims; ++j)
+            if (!taken[j] && b.n[j] > 1 && b.st[j] * b.esz == a.st[i] * a.esz) { taken[j] = true; hi = b.n[j] - 1; break; }
+        m.add(a.st[i] * a.esz, 1 - a.n[i], hi);
+    }
+    for (int j = 0; j < b.dims; ++j)
+        if (!taken[j] && b.n[j] > 1 && b.st[j] != 0) m.add(b.st[j] * b.esz, 0, b.n[j] - 1);
+    m.low = 1 - a.inner * a.esz;
+    m.high = b.inner * b.esz - 1;
+    int k = 0;
+    for (; k < m.dims && m.st[k] <= m.high - m.low + 1; ++k) { m.low += m.lo[k] * m.st[k]; m.high += m.hi[k] * m.st[k]; }
+    for (int i = k; i < m.dims; ++i) { m.st[i - k] = m.st[i]; m.lo[i - k] = m.lo[i]; m.hi[i - k] = m.hi[i]; }
+    return m.reaches((int64_t)(pb - pa), m.dims - k);
 }
 
 PagedBatchArgs batch_args(const ptts_paged_kv* c, const ptts_paged_batch* b) {
@@ -376,7 +422,9 @@ int ptts_rotary_embed(const ptts_rotary* rot, int32_t dtype, int32_t tokens, int
     TRY(check_rows("x", x, a.xs, tokens, heads, head_dim, false));
     TRY(check_rows("out", out, a.os, tokens, heads, head_dim, true));
     const int esz = dtype == PTTS_DTYPE_BF16 ? 2 : 4;
-    if (!(x == out && a.xs[0] == a.os[0] && a.xs[1] == a.os[1]) && ranges_meet(x, a.xs, out, a.os, tokens, heads, head_dim, esz))
+    const int64_t n[2] = {tokens, heads};
+    if (!(x == out && a.xs[0] == a.os[0] && a.xs[1] == a.os[1]) &&
+        share_memory(Strided{x, a.xs, n, 2, esz, head_dim}, Strided{out, a.os, n, 2, esz, head_dim}))
         REFUSE(PTTS_E_INVALID, "x and out share memory in another layout than in place");
     a.pos = positions; a.rot = rotary_args(rot); a.status = status; a.tokens = tokens; a.heads = heads; a.head_dim = head_dim;
     return launched("ptts_rotary_embed", rotary_embed_launch(a, dtype, (hipStream_t)stream));
@@ -403,12 +451,16 @@ int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, in
     a.ks[0] = k_token_stride; a.ks[1] = k_head_stride; a.vs[0] = v_token_stride; a.vs[1] = v_head_stride;
     TRY(check_rows("k", k, a.ks, T, cache->kv_heads, D, false));
     TRY(check_rows("v", v, a.vs, T, cache->kv_heads, D, false));
+    const int esz = dtype == PTTS_DTYPE_BF16 ? 2 : 4;
+    const int64_t n[2] = {T, cache->kv_heads}, nq[2] = {T, q_heads};
+    const Strided ks = {k, a.ks, n, 2, esz, D}, vs = {v, a.vs, n, 2, esz, D};
     if (q_heads) {
-        const int esz = dtype == PTTS_DTYPE_BF16 ? 2 : 4;
         TRY(check_rows("q", q, a.qs, T, q_heads, D, false));
         TRY(check_rows("q_out", q_out, a.qos, T, q_heads, D, true));
-        if (!(q == q_out && a.qs[0] == a.qos[0] && a.qs[1] == a.qos[1]) && ranges_meet(q, a.qs, q_out, a.qos, T, q_heads, D, esz))
+        const Strided qs = {q, a.qs, nq, 2, esz, D}, qos = {q_out, a.qos, nq, 2, esz, D};
+        if (!(q == q_out && a.qs[0] == a.qos[0] && a.qs[1] == a.qos[1]) && share_memory(qs, qos))
             REFUSE(PTTS_E_INVALID, "q and q_out share memory in another layout than in place");
+        if (share_memory(ks, qos) || share_memory(vs, qos)) REFUSE(PTTS_E_INVALID, "q_out shares memory with k or v");
     }
     for (int i = 0; i < 3; ++i) { a.kc[i] = cache->k_strides[i]; a.vc[i] = cache->v_strides[i]; }
     a.b = batch_args(cache, batch); a.rot = rotary_args(rot); a.pos = rot ? positions : nullptr; a.status = status;
@@ -464,7 +516,8 @@ int ptts_paged_attention(const ptts_paged_kv* cache, const ptts_paged_batch* bat
     TRY(check_rows("out", out, a.os, T, q_heads, D, true));
     const int esz = cache->dtype == PTTS_DTYPE_BF16 ? 2 : 4;
     if (!aligned(q, a.qs, 2, 16, esz) || !aligned(out, a.os, 2, 16, esz)) REFUSE(PTTS_E_INVALID, "rows of q and out must start at multiples of 16 bytes");
-    if (ranges_meet(q, a.qs, out, a.os, T, q_heads, D, esz)) REFUSE(PTTS_E_INVALID, "q and out share memory");
+    const int64_t n[2] = {T, q_heads};
+    if (share_memory(Strided{q, a.qs, n, 2, esz, D}, Strided{out, a.os, n, 2, esz, D})) REFUSE(PTTS_E_INVALID, "q and out share memory");
     a.mask = key_mask && mask_width > 0 ? key_mask : nullptr; a.mask_stride = mask_stride; a.mask_width = a.mask ? mask_width : 0;
     a.scale_log2 = scale * 1.4426950408889634f; a.causal = causal ? 1 : 0; a.status = status;
     const int64_t need = paged_attn_workspace(a, max_new, cache->head_dim, cache->dtype);

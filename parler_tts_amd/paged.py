@@ -226,8 +226,8 @@ def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, table: torc
               starts: Optional[torch.Tensor] = None, *, rotary: Optional[RotaryTable] = None, positions: Optional[torch.Tensor] = None,
               q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Stores ``k``, ``v`` [tokens, kv_heads, head_dim]: token i of sequence s at slot ``past[s] + i``, k turned by ``rotary`` at that
-    position (or at ``positions`` [tokens] int32).  ``q`` [tokens, heads, head_dim] is turned in the same launch into ``q_out`` (may be ``q``),
-    which is returned.  float32 rows may be stored in a bfloat16 cache.  Rows behind the last sequence are left alone, in ``q_out`` too."""
+    position (or at ``positions`` [tokens] int32).  ``q`` [tokens, heads, head_dim] is turned in the same launch into ``q_out`` (may be ``q``,
+    and shares no memory with ``k`` or ``v``), which is returned.  float32 rows may be stored in a bfloat16 cache.  Rows behind the last sequence are left alone, in ``q_out`` too."""
     index = cache._index
     tokens = k.shape[0]
     _rows("k", k, tokens, cache.kv_heads, cache.head_dim, index)
