@@ -334,7 +334,7 @@ int ptts_rotary_embed(const ptts_rotary* rot, int32_t dtype, int32_t tokens, int
 
 /* Token i of sequence s goes to slot past[s] + i: k turned by `rot` (NULL: as it is) at its slot, or at positions[token] where
  * positions is given; v as it is.  q (optional: q_heads > 0) is turned at the same positions into q_out, which may be q, but
- * shares no memory with k or v.
+ * shares no memory with k or v.  None of these rows lies in the cache, and its keys and values share no memory.
  * dtype is that of k, v and q; f32 rows may go into a bf16 cache (rounded once, behind the rotation).  A token that cannot be placed
  * leaves the cache as it is and its row of q_out becomes zero; rows behind the last sequence are left as they are. */
 int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, int32_t dtype, const void* k, int64_t k_token_stride,
@@ -347,7 +347,7 @@ int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, in
  * are no keys; whatever they hold does not reach the output.  A token that sees no key gets zeros; rows that a bad page or length concerns
  * get NaN; rows of no sequence (behind the last, or where starts are wrong) are left as they are, rows that descending starts give to
  * several hold the result of one of these.  Query head h reads key head h / (q_heads / kv_heads).  q, out: [tokens][q_heads][head_dim] of
- * the cache's type.
+ * the cache's type; out shares no memory with q or the cache.
  * max_new: an upper bound of the new tokens of one sequence, 0 = not known; it picks the kernel, never the result's validity.
  * workspace: ptts_paged_attention_workspace() bytes (may be 0; negative = PTTS_E_*) at a multiple of 16, not shared with another call
  * in flight. */

@@ -376,6 +376,13 @@ bool share_memory(const Strided& a, const Strided& b) {
     return m.reaches((int64_t)(pb - pa), m.dims - k);
 }
 
+// whether a tensor and the cache's keys or values do
+bool in_cache(const ptts_paged_kv* c, const Strided& t) {
+    const int esz = c->dtype == PTTS_DTYPE_BF16 ? 2 : 4;
+    const int64_t n[3] = {c->n_pages, c->kv_heads, c->page_tokens};
+    return share_memory(Strided{c->k, c->k_strides, n, 3, esz, c->head_dim}, t) || share_memory(Strided{c->v, c->v_strides, n, 3, esz, c->head_dim}, t);
+}
+
 PagedBatchArgs batch_args(const ptts_paged_kv* c, const ptts_paged_batch* b) {
     PagedBatchArgs r;
     r.table = b->table; r.table_stride = b->table_stride; r.past = b->past; r.starts = b->starts;
@@ -461,7 +468,14 @@ int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, in
         if (!(q == q_out && a.qs[0] == a.qos[0] && a.qs[1] == a.qos[1]) && share_memory(qs, qos))
             REFUSE(PTTS_E_INVALID, "q and q_out share memory in another layout than in place");
         if (share_memory(ks, qos) || share_memory(vs, qos)) REFUSE(PTTS_E_INVALID, "q_out shares memory with k or v");
+        if (in_cache(cache, qs) || in_cache(cache, qos)) REFUSE(PTTS_E_INVALID, "q or q_out share memory with the cache");
     }
+    // rows may be stored over while another workgroup still reads them, and which slots are stored to is known on the device only
+    if (in_cache(cache, ks) || in_cache(cache, vs)) REFUSE(PTTS_E_INVALID, "k or v share memory with the cache");
+    const int64_t nc[3] = {cache->n_pages, cache->kv_heads, cache->page_tokens};
+    const int csz = cache->dtype == PTTS_DTYPE_BF16 ? 2 : 4;
+    if (share_memory(Strided{cache->k, cache->k_strides, nc, 3, csz, D}, Strided{cache->v, cache->v_strides, nc, 3, csz, D}))
+        REFUSE(PTTS_E_INVALID, "keys and values of the cache share memory");
     for (int i = 0; i < 3; ++i) { a.kc[i] = cache->k_strides[i]; a.vc[i] = cache->v_strides[i]; }
     a.b = batch_args(cache, batch); a.rot = rotary_args(rot); a.pos = rot ? positions : nullptr; a.status = status;
     a.q_heads = q_heads; a.kv_heads = cache->kv_heads; a.head_dim = cache->head_dim;
@@ -517,7 +531,9 @@ int ptts_paged_attention(const ptts_paged_kv* cache, const ptts_paged_batch* bat
     const int esz = cache->dtype == PTTS_DTYPE_BF16 ? 2 : 4;
     if (!aligned(q, a.qs, 2, 16, esz) || !aligned(out, a.os, 2, 16, esz)) REFUSE(PTTS_E_INVALID, "rows of q and out must start at multiples of 16 bytes");
     const int64_t n[2] = {T, q_heads};
-    if (share_memory(Strided{q, a.qs, n, 2, esz, D}, Strided{out, a.os, n, 2, esz, D})) REFUSE(PTTS_E_INVALID, "q and out share memory");
+    const Strided os = {out, a.os, n, 2, esz, D};
+    if (share_memory(Strided{q, a.qs, n, 2, esz, D}, os)) REFUSE(PTTS_E_INVALID, "q and out share memory");
+    if (in_cache(cache, os)) REFUSE(PTTS_E_INVALID, "out shares memory with the cache");
     a.mask = key_mask && mask_width > 0 ? key_mask : nullptr; a.mask_stride = mask_stride; a.mask_width = a.mask ? mask_width : 0;
     a.scale_log2 = scale * 1.4426950408889634f; a.causal = causal ? 1 : 0; a.status = status;
     const int64_t need = paged_attn_workspace(a, max_new, cache->head_dim, cache->dtype);

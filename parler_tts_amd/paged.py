@@ -227,7 +227,9 @@ def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, table: torc
               q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Stores ``k``, ``v`` [tokens, kv_heads, head_dim]: token i of sequence s at slot ``past[s] + i``, k turned by ``rotary`` at that
     position (or at ``positions`` [tokens] int32).  ``q`` [tokens, heads, head_dim] is turned in the same launch into ``q_out`` (may be ``q``,
-    and shares no memory with ``k`` or ``v``), which is returned.  float32 rows may be stored in a bfloat16 cache.  Rows behind the last sequence are left alone, in ``q_out`` too."""
+    and shares no memory with ``k`` or ``v``), which is returned.  float32 rows may be stored in a bfloat16 cache.  Rows behind the last
+    sequence are left alone, in ``q_out`` too.  None of the rows may lie in the cache (copy what is to move within it), and ``cache.k`` and
+    ``cache.v`` share no memory."""
     index = cache._index
     tokens = k.shape[0]
     _rows("k", k, tokens, cache.kv_heads, cache.head_dim, index)
@@ -285,7 +287,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
     column is no key, whatever the cache holds there; keys behind its last column are seen.  A token without keys gets zeros.
     ``q``'s heads are a multiple of the cache's, in groups: head h reads key head h // (heads / kv_heads).
     ``max_new``: the longest sequence's number of new tokens if the caller knows it (it helps to pick the kernel; 0: unknown).
-    Rows of ``q`` and ``out`` start at multiples of 16 bytes and share no memory.
+    Rows of ``q`` and ``out`` start at multiples of 16 bytes; ``out`` shares no memory with ``q`` or the cache.
     Sequences may share pages, or (an expanded ``table``) all of them.  Rows of no sequence (behind the last, or where ``starts`` are wrong)
     are left as they are in ``out``; rows that descending ``starts`` give to several hold the result of one of these."""
     index, dim = cache._index, cache.head_dim

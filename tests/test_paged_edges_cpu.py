@@ -79,3 +79,48 @@ def test_rows_that_share_memory_are_told_from_rows_beside_each_other(lib, seed):
             rc = append(lib, far, one, int(bf16), *rows, None, heads, 256 * P, (1 << 12, 64), at, b)
             assert verdict(lib, rc, b"q_out shares memory with k or v") == over
     assert 50 < shared < 250
+
+
+@no_gpu
+@pytest.mark.parametrize("seed", range(2))
+def test_rows_within_the_cache_are_told_from_rows_beside_it(lib, seed):
+    """out of an attention and all rows of an append against the sets of the cache's bytes: gaps of a cache may hold rows, its slots may not"""
+    rng = random.Random(100 + seed)
+    refused = 0
+    for _ in range(60):
+        tokens, pages, dim = rng.randint(1, 20), rng.randint(1, 3), 64
+        bf16 = rng.random() < 0.5
+        esz = 2 if bf16 else 4
+        nc, n = [pages, 2, 16], [tokens, 2]
+        st = [8 * x for x in layout(rng, nc, dim // 8)]
+        rows = rng.choice([[8 * x for x in layout(rng, n, dim // 8)], [st[2], st[1]]])
+        inner, outer = sorted(zip(rows, n))
+        if outer[1] > 1 and outer[0] < dim + (inner[1] - 1) * inner[0] or inner[1] > 1 and inner[0] < dim:
+            rows = [2 * dim, dim]                         # extents that are not nested count as rows that meet themselves
+        span = sum((m - 1) * x for m, x in zip(nc, st)) + dim
+        at = 64 * P + 16 * rng.randint(-tokens * 20, span * esz // 16)
+        cached = places(64 * P, st, nc, esz)
+        meets = bool(cached & places(at, rows, n, esz))
+        refused += meets
+        one = batch(starts=None, tokens=tokens, n_seqs=tokens)
+        for which in ("k", "v"):
+            pools = dict(k=64 * P, v=512 * P) if which == "k" else dict(k=512 * P, v=64 * P)
+            c = kv(dtype=int(bf16), k_strides=strides(*st), v_strides=strides(*st), n_pages=pages, page_tokens=16, **pools)
+            rc = attend(lib, c, one, 2, 128 * P, (128, 64), at, rows, ws=1024 * P)
+            assert verdict(lib, rc, b"out shares memory with the cache") == meets
+            clear = [(128 * P, (128, 64)), (136 * P, (128, 64)), (144 * P, (128, 64)), (152 * P, (128, 64))]
+            for i in range(4):                            # k, v, q, q_out
+                k, v, q, qo = clear[:i] + [(at, rows)] + clear[i + 1:]
+                rc = append(lib, c, one, int(bf16), *k, *v, None, 2, *q, *qo)
+                assert verdict(lib, rc, b"share memory with the cache") == meets
+        c = kv(dtype=int(bf16), k=64 * P, v=at, k_strides=strides(*st), v_strides=strides(*st), n_pages=pages, page_tokens=16)
+        rc = append(lib, c, one, int(bf16), 512 * P, (128, 64), 520 * P, (128, 64))
+        assert verdict(lib, rc, b"keys and values of the cache share memory") == bool(cached & places(at, st, nc, esz))
+    assert 5 < refused < 55, refused
+
+
+def test_keys_that_are_the_values_too_can_be_read_but_not_appended_to(lib):
+    c = kv(k=64 * P, v=64 * P)
+    assert append(lib, c) == -1 and b"keys and values" in lib.ptts_last_error()
+    if not torch.cuda.is_available():
+        assert attend(lib, c, ws=1024 * P) == LAUNCHED
