@@ -10,6 +10,7 @@
 #include "paged.h"
 #include <climits>
 #include <cmath>
+#include <initializer_list>
 
 namespace {
 
@@ -194,10 +195,13 @@ UnitMap make_map(int heads, int head_dim, int rot_dims, int n, int tokens, bool 
     return m;
 }
 
-bool aligned(const void* p, const int64_t* strides, int ns, int64_t bytes, int64_t esz) {
+// all rows of a tensor of these extents at multiples of `bytes` (the stride of a single entry addresses nothing and may be anything)
+bool aligned(const void* p, const int64_t* strides, std::initializer_list<int64_t> extents, int64_t bytes, int64_t esz) {
     if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
-    for (int i = 0; i < ns; ++i)
-        if (strides[i] * esz % bytes) return false;
+    for (const int64_t n : extents) {
+        if (n > 1 && *strides * esz % bytes) return false;
+        ++strides;
+    }
     return true;
 }
 
@@ -205,8 +209,9 @@ bool aligned(const void* p, const int64_t* strides, int ns, int64_t bytes, int64
 
 hipError_t rotary_embed_launch(const RotaryEmbedArgs& a, int dtype, hipStream_t s) {
     const int esz = dtype == PTTS_BF16 ? 2 : 4, full = 16 / esz;
-    const bool wide = a.rot.dims % (2 * full) == 0 && a.head_dim % (2 * full) == 0 && aligned(a.x, a.xs, 2, 16, esz) &&
-                      aligned(a.out, a.os, 2, 16, esz) && aligned(a.rot.cos_t, nullptr, 0, 16, 4) && aligned(a.rot.sin_t, nullptr, 0, 16, 4);
+    const bool wide = a.rot.dims % (2 * full) == 0 && a.head_dim % (2 * full) == 0 && aligned(a.x, a.xs, {a.tokens, a.heads}, 16, esz) &&
+                      aligned(a.out, a.os, {a.tokens, a.heads}, 16, esz) && aligned(a.rot.cos_t, nullptr, {}, 16, 4) &&
+                      aligned(a.rot.sin_t, nullptr, {}, 16, 4);
     const UnitMap m = make_map(a.heads, a.head_dim, a.rot.dims, wide ? full : 1, a.tokens, false);
     const dim3 grid((a.tokens + m.tokens_per_block - 1) / m.tokens_per_block), block(256);
 #define LAUNCH(T, N)                                                                                        \
@@ -223,10 +228,12 @@ hipError_t rotary_embed_launch(const RotaryEmbedArgs& a, int dtype, hipStream_t 
 hipError_t kv_append_launch(const AppendArgs& a, int in_dtype, int cache_dtype, hipStream_t s) {
     const int esz = in_dtype == PTTS_BF16 ? 2 : 4, full = 16 / esz;
     const int csz = cache_dtype == PTTS_BF16 ? 2 : 4;
-    bool wide = a.rot.dims % (2 * full) == 0 && a.head_dim % (2 * full) == 0 && aligned(a.k, a.ks, 2, 16, esz) && (!a.v || aligned(a.v, a.vs, 2, 16, esz)) &&
-                aligned(a.k_cache, a.kc, 3, full * csz, csz) && aligned(a.v_cache, a.vc, 3, full * csz, csz);
-    if (a.q_heads) wide = wide && aligned(a.q, a.qs, 2, 16, esz) && aligned(a.q_out, a.qos, 2, 16, esz);
-    if (a.rot.cos_t) wide = wide && aligned(a.rot.cos_t, nullptr, 0, 16, 4) && aligned(a.rot.sin_t, nullptr, 0, 16, 4);
+    bool wide = a.rot.dims % (2 * full) == 0 && a.head_dim % (2 * full) == 0 && aligned(a.k, a.ks, {a.b.tokens, a.kv_heads}, 16, esz) &&
+                (!a.v || aligned(a.v, a.vs, {a.b.tokens, a.kv_heads}, 16, esz)) &&
+                aligned(a.k_cache, a.kc, {a.b.n_pages, a.kv_heads, 1 << a.b.page_shift}, full * csz, csz) &&
+                aligned(a.v_cache, a.vc, {a.b.n_pages, a.kv_heads, 1 << a.b.page_shift}, full * csz, csz);
+    if (a.q_heads) wide = wide && aligned(a.q, a.qs, {a.b.tokens, a.q_heads}, 16, esz) && aligned(a.q_out, a.qos, {a.b.tokens, a.q_heads}, 16, esz);
+    if (a.rot.cos_t) wide = wide && aligned(a.rot.cos_t, nullptr, {}, 16, 4) && aligned(a.rot.sin_t, nullptr, {}, 16, 4);
     const UnitMap m = make_map(a.q_heads + (a.v ? 2 : 1) * a.kv_heads, a.head_dim, a.rot.dims, wide ? full : 1, a.b.tokens, true);
     const dim3 grid((a.b.tokens + m.tokens_per_block - 1) / m.tokens_per_block), block(256);
 #define LAUNCH(T, TC, N)                                                                                      \
@@ -265,8 +272,9 @@ bool overlaps_itself(const int64_t* st, const int64_t* n, int dims, int64_t inne
 bool fits(const int64_t* st, const int64_t* n, int dims) {     // offsets are formed in 64 bits; keep them far from the end
     int64_t span = 0;
     for (int i = 0; i < dims; ++i) {
+        if (n[i] <= 1) continue;
         if (st[i] < 0 || st[i] > ((int64_t)1 << 44)) return false;
-        span += st[i] * (n[i] > 0 ? n[i] - 1 : 0) / 4;
+        span += st[i] * (n[i] - 1) / 4;
         if (span > ((int64_t)1 << 56)) return false;
     }
     return true;
@@ -294,7 +302,7 @@ int check_kv(const ptts_paged_kv* c) {
     const int esz = c->dtype == PTTS_DTYPE_BF16 ? 2 : 4;
     if (c->k_strides[2] * esz >= ((int64_t)1 << 27) || c->v_strides[2] * esz >= ((int64_t)1 << 27))
         REFUSE(PTTS_E_UNSUPPORTED, "slots of a page 128 MiB or more apart");
-    if (!aligned(c->k, c->k_strides, 3, 16, esz) || !aligned(c->v, c->v_strides, 3, 16, esz))
+    if (!aligned(c->k, c->k_strides, {n[0], n[1], n[2]}, 16, esz) || !aligned(c->v, c->v_strides, {n[0], n[1], n[2]}, 16, esz))
         REFUSE(PTTS_E_INVALID, "cache rows must start at multiples of 16 bytes");
     return PTTS_OK;
 }
@@ -305,6 +313,7 @@ int check_batch(const ptts_paged_batch* b, bool written) {
     if (b->n_seqs > 0 && (!b->past || (!b->table && b->max_pages > 0))) REFUSE(PTTS_E_INVALID, "null page table or lengths");
     if (!b->starts && b->tokens != b->n_seqs) REFUSE(PTTS_E_INVALID, "%d tokens of %d sequences need starts", b->tokens, b->n_seqs);
     // sequences may read the same row of pages; where they write, no two of them own a slot
+    if (b->n_seqs <= 1) return PTTS_OK;
     if (b->table_stride < b->max_pages && (written || b->table_stride != 0)) REFUSE(PTTS_E_INVALID, "page table rows overlap");
     if ((int64_t)b->table_stride > INT_MAX) REFUSE(PTTS_E_INVALID, "page table stride out of range");
     return PTTS_OK;
@@ -521,7 +530,7 @@ int ptts_paged_attention(const ptts_paged_kv* cache, const ptts_paged_batch* bat
     TRY(attn_args(cache, batch, q_heads, max_new, &a));
     if (!status) REFUSE(PTTS_E_INVALID, "null status");
     if (!(scale > 0.f) || !std::isfinite(scale)) REFUSE(PTTS_E_INVALID, "softmax scale must be positive and finite");
-    if (key_mask && (mask_width < 0 || mask_stride < mask_width)) REFUSE(PTTS_E_INVALID, "key mask of %d columns", mask_width);
+    if (key_mask && (mask_width < 0 || (mask_stride < mask_width && batch->n_seqs > 1))) REFUSE(PTTS_E_INVALID, "key mask of %d columns", mask_width);
     const int64_t T = batch->tokens, D = cache->head_dim;
     if (T == 0 || batch->n_seqs == 0) return PTTS_OK;
     a.q = q; a.out = out;
@@ -529,7 +538,7 @@ int ptts_paged_attention(const ptts_paged_kv* cache, const ptts_paged_batch* bat
     TRY(check_rows("q", q, a.qs, T, q_heads, D, false));
     TRY(check_rows("out", out, a.os, T, q_heads, D, true));
     const int esz = cache->dtype == PTTS_DTYPE_BF16 ? 2 : 4;
-    if (!aligned(q, a.qs, 2, 16, esz) || !aligned(out, a.os, 2, 16, esz)) REFUSE(PTTS_E_INVALID, "rows of q and out must start at multiples of 16 bytes");
+    if (!aligned(q, a.qs, {T, q_heads}, 16, esz) || !aligned(out, a.os, {T, q_heads}, 16, esz)) REFUSE(PTTS_E_INVALID, "rows of q and out must start at multiples of 16 bytes");
     const int64_t n[2] = {T, q_heads};
     const Strided os = {out, a.os, n, 2, esz, D};
     if (share_memory(Strided{q, a.qs, n, 2, esz, D}, os)) REFUSE(PTTS_E_INVALID, "q and out share memory");

@@ -166,7 +166,7 @@ def _rows(name: str, t: torch.Tensor, tokens: Optional[int], heads: Optional[int
 
 
 def _ints(name: str, t: torch.Tensor, dims: int, index: int) -> None:
-    if t.dtype is not torch.int32 or t.dim() != dims or t.get_device() != index or (t.stride(-1) != 1 and t.numel() > 1):
+    if t.dtype is not torch.int32 or t.dim() != dims or t.get_device() != index or (t.stride(-1) != 1 and t.shape[-1] > 1):
         raise ValueError(f"{name} has to be a contiguous int32 tensor of {dims} dimension(s) on device {index}")
 
 

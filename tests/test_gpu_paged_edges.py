@@ -105,3 +105,42 @@ def test_descending_starts_that_give_all_rows_to_every_other_sequence(paged, max
     one, bound = ref.attend(q[:64].cpu(), kc, vc, table.cpu(), [page], [0, 64], dim ** -0.5, causal=False)
     close(got[:64], one, bound)
     cache.check()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_strides_of_a_single_entry_are_not_looked_at(paged, dtype):
+    """one token, one head, one page, one key head, one column of a table, each with an odd stride there: the bits of the contiguous call"""
+    page, dim = 16, 64
+
+    def odd(t, dim_of_one, stride):
+        st = list(t.stride())
+        st[dim_of_one] = stride
+        return torch.as_strided(t, t.shape, st)
+
+    for heads, tokens, pages in ((4, 1, 3), (1, 5, 3), (2, 3, 1)):
+        kv_heads = 1
+        kc, vc = rnd(2, pages, kv_heads, page, dim, dtype=dtype).cuda(), rnd(3, pages, kv_heads, page, dim, dtype=dtype).cuda()
+        q, k, v = (rnd(i, tokens, h, dim, dtype=dtype).cuda() for i, h in ((4, heads), (5, kv_heads), (6, kv_heads)))
+        table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+        rotary = paged.RotaryTable(dim, 64)
+        at = [table, ints([page * (pages - 1) + 3]), ints([0, tokens])]
+        pos = torch.arange(tokens, dtype=torch.int32, device="cuda")
+
+        def calls(kc, vc, q, k, v, out, table):
+            cache = paged.PagedKVCache.from_tensors(kc, vc)
+            x = paged.kv_append(cache, k, v, table, *at[1:], rotary=rotary, q=q)
+            o = paged.paged_attention(x, cache, table, *at[1:], out=out)
+            cache.check()
+            return x, o, paged.rotary_embed(q, pos, rotary), kc, vc
+
+        want = calls(kc.clone(), vc.clone(), q, k, v, torch.empty_like(q), table)
+        ones = [i for i, m in enumerate((tokens, heads)) if m == 1]
+        q2, out = q.clone(), torch.empty_like(q)
+        for i in ones:
+            q2, out = odd(q2, i, 3), odd(out, i, 5)
+        rows = [odd(t, 1, 7) if tokens > 1 else odd(odd(t, 1, 7), 0, 9) for t in (k, v)]
+        pools = [odd(t.clone(), 1, 11) if pages > 1 else odd(odd(t.clone(), 1, 11), 0, 13) for t in (kc, vc)]
+        wide = torch.zeros(1, 2 * pages, dtype=torch.int32, device="cuda")
+        wide[:, ::2] = table
+        got = calls(*pools, q2, *rows, out, wide[:, ::2] if pages == 1 else table)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), (heads, tokens, pages)

@@ -124,3 +124,23 @@ def test_keys_that_are_the_values_too_can_be_read_but_not_appended_to(lib):
     assert append(lib, c) == -1 and b"keys and values" in lib.ptts_last_error()
     if not torch.cuda.is_available():
         assert attend(lib, c, ws=1024 * P) == LAUNCHED
+
+
+@no_gpu
+def test_strides_of_a_single_entry_are_not_looked_at(lib):
+    """they address nothing and may be anything; of two entries they count"""
+    odd = 3
+    c1 = kv(k_strides=strides(odd, 4096, 64), v_strides=strides(-odd, 4096, 64), n_pages=1, k=64 * P, v=128 * P)
+    h1 = kv(k_strides=strides(8192, odd, 64), v_strides=strides(8192, 1 << 50, 64), kv_heads=1, k=64 * P, v=128 * P)
+    far = kv(k=64 * P, v=128 * P)
+    one, two = batch(starts=None, tokens=1, n_seqs=1, table_stride=-odd), batch(starts=None, tokens=2, n_seqs=2)
+    for c, b, heads, qs, os in ((far, one, 4, (odd, 64), (odd, 64)), (far, one, 4, (-odd, 64), (1 << 50, 64)), (h1, two, 1, (128, odd), (64, -odd)),
+                                (c1, two, 2, (128, 64), (128, 64)), (h1, two, 2, (128, 64), (128, 64))):
+        assert attend(lib, c, b, heads, qs=qs, os=os, ws=1024 * P, mask=256 * P, mstride=4, mwidth=4) == LAUNCHED, lib.ptts_last_error()
+        row = (64, odd) if c.kv_heads == 1 else ((odd, 64) if b is one else (128, 64))
+        assert append(lib, c, b, 1, 256 * P, row, 512 * P, row, None, heads, P, qs, 2 * P, os) == LAUNCHED, lib.ptts_last_error()
+    assert attend(lib, far, one, 4, ws=1024 * P, mask=256 * P, mstride=0, mwidth=4) == LAUNCHED
+    assert attend(lib, far, two, 4, qs=(260, 64), ws=1024 * P) == attend(lib, far, two, 4, os=(260, 64), ws=1024 * P) == -1
+    assert attend(lib, far, two, 4, ws=1024 * P, mask=256 * P, mstride=0, mwidth=4) == -1
+    assert attend(lib, kv(k=64 * P, v=128 * P, k_strides=strides(8196, 4096, 64)), two, 4, ws=1024 * P) == -1
+    assert append(lib, far, batch(starts=None, tokens=2, n_seqs=2, table_stride=3)) == -1
