@@ -40,10 +40,22 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda in
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
+def _new_status(device: torch.device) -> torch.Tensor:
+    status = torch.zeros(1, dtype=torch.int32, device=device)
+    if status.is_cuda:                  # calls on other streams find it cleared (and a rotary table made)
+        with torch.cuda.device(device):
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().synchronize()
+    return status
+
+
 def _read_status(status: torch.Tensor, who: str) -> None:
+    wait = torch.cuda.synchronize if status.is_cuda else lambda device: None
+    wait(status.device)                 # calls on any stream
     bits = int(status.item())
     if bits:
         status.zero_()
+        wait(status.device)             # what follows on another stream sets its bits behind the clearing
         raise _hip.PttsError(-1, f"{who}: " + "; ".join(t for b, t in _hip.PAGED_STATUS.items() if bits & b))
 
 
@@ -104,13 +116,14 @@ class RotaryTable:
         self.cos, self.sin = (torch.cos(angle) * gain).float(), (torch.sin(angle) * gain).float()
         self.head_dim, self.positions, self.rotary_dim, self.layout = head_dim, positions, rotary_dim, layout
         self.device, self._index = self.cos.device, self.cos.get_device()
-        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.status = _new_status(self.device)
         self._status = self.status.data_ptr()
         self._c = _hip.PttsRotary(self.cos.data_ptr(), self.sin.data_ptr(), positions, rotary_dim, 1 if layout == "interleaved" else 0)
         self._ref = C.addressof(self._c)
 
     def check(self) -> None:
-        """waits for the device; raises if a call since the last check met a position outside the table"""
+        """waits for the device (every stream); raises if a call since the last check met a position outside the table.  Not to be called while
+        another thread makes calls."""
         _read_status(self.status, "rotary_embed")
 
 
@@ -140,7 +153,7 @@ class PagedKVCache:
         self.k, self.v = k, v
         self.num_pages, self.kv_heads, self.page_tokens, self.head_dim = pages, heads, tokens, dim
         self.dtype, self.device, self._index = k.dtype, k.device, k.get_device()
-        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.status = _new_status(self.device)
         self._status = self.status.data_ptr()
         self._c = _hip.PttsPagedKV(k.data_ptr(), v.data_ptr(), (C.c_int64 * 3)(*k.stride()[:3]), (C.c_int64 * 3)(*v.stride()[:3]),
                                    _DTYPES[k.dtype], pages, heads, tokens, dim)
@@ -148,7 +161,8 @@ class PagedKVCache:
         self._workspace: Dict[tuple, int] = {}      # bytes by sizes
 
     def check(self) -> None:
-        """waits for the device; raises if a call since the last check met a page, length, position or start it could not follow"""
+        """waits for the device (every stream); raises if a call since the last check met a page, length, position or start it could not follow.
+        Not to be called while another thread makes calls."""
         _read_status(self.status, "paged cache")
 
 

@@ -144,3 +144,55 @@ def test_strides_of_a_single_entry_are_not_looked_at(paged, dtype):
         wide[:, ::2] = table
         got = calls(*pools, q2, *rows, out, wide[:, ::2] if pages == 1 else table)
         assert all(torch.equal(a, b) for a, b in zip(got, want)), (heads, tokens, pages)
+
+
+def busy():
+    """some 20 ms of work on the current stream (float32 products, 144 TFLOP/s at most)"""
+    a = torch.ones(8192, 8192, device="cuda")
+    for _ in range(3):
+        a = a @ a * 0
+    return a
+
+
+def test_a_check_sees_calls_of_every_stream(paged):
+    """a call behind other work on another stream, and a cache made behind it: neither is ready when the host goes on"""
+    from parler_tts_amd._hip import PttsError
+
+    k = rnd(1, 4, 2, 16, 64).cuda()
+    q, table, past = rnd(2, 1, 2, 64).cuda(), ints([[9, 1]]), ints([3])
+    cache, rotary = paged.PagedKVCache.from_tensors(k, k.clone()), paged.RotaryTable(64, 10)
+    busy()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        keep = busy()
+        paged.paged_attention(q, cache, table, past)
+        paged.rotary_embed(q, past + 9, rotary)
+    with pytest.raises(PttsError, match="page id"):
+        cache.check()
+    with torch.cuda.stream(side):
+        paged.rotary_embed(q, past, rotary)
+        keep = busy()
+        late = paged.PagedKVCache.from_tensors(k, k.clone())
+    paged.paged_attention(q, late, table, past)
+    torch.cuda.synchronize()
+    with pytest.raises(PttsError, match="page id"):
+        late.check()
+    with pytest.raises(PttsError, match="position"):
+        rotary.check()
+    for x in (cache, late, rotary):
+        x.check()
+    assert (keep == 0).all()
+
+
+def test_a_cache_made_while_a_graph_is_captured(paged):
+    k, v, q, table, past = rnd(1, 4, 2, 16, 64).cuda(), rnd(2, 4, 2, 16, 64).cuda(), rnd(3, 1, 2, 64).cuda(), ints([[0, 1]]), ints([3])
+    want = paged.paged_attention(q, paged.PagedKVCache.from_tensors(k, v), table, past)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = paged.paged_attention(q, paged.PagedKVCache.from_tensors(k, v), table, past)
+    for _ in range(3):
+        got.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)

@@ -144,3 +144,23 @@ def test_strides_of_a_single_entry_are_not_looked_at(lib):
     assert attend(lib, far, two, 4, ws=1024 * P, mask=256 * P, mstride=0, mwidth=4) == -1
     assert attend(lib, kv(k=64 * P, v=128 * P, k_strides=strides(8196, 4096, 64)), two, 4, ws=1024 * P) == -1
     assert append(lib, far, batch(starts=None, tokens=2, n_seqs=2, table_stride=3)) == -1
+
+
+def test_a_check_waits_for_every_stream_before_it_reads_and_after_it_clears(monkeypatch):
+    done = []
+
+    class Status:
+        is_cuda, device = True, torch.device("cuda", 3)
+
+        def item(self):
+            done.append("read")
+            return 2
+
+        def zero_(self):
+            done.append("clear")
+
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device: done.append(f"wait {device.index}"))
+    with pytest.raises(_hip.PttsError, match="page id"):
+        paged._read_status(Status(), "paged cache")
+    assert done == ["wait 3", "read", "clear", "wait 3"]
+    paged.RotaryTable(64, 4, device="cpu").check()        # nothing to wait for
