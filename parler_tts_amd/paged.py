@@ -15,7 +15,8 @@ out of a buffer: it sets ``cache.status`` / ``rotary.status``, which ``check()``
 zeros (``kv_append``, ``rotary_embed``) or NaN (``paged_attention``; where ``starts`` are wrong, as ``out`` held them or one
 of the sequences' that claim them).
 
-Work goes to the current stream of the tensors' device and nothing is synchronised.  No gradients: forward only.
+Work goes to the current stream of the tensors' device and nothing is synchronised.  No gradients: forward only (tensors that ask for one are
+refused, those of the cache too).
 """
 from __future__ import annotations
 
@@ -24,6 +25,7 @@ import math
 from typing import Any, Dict, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _hip
 
@@ -38,6 +40,13 @@ def _need(ok: bool, what: str) -> None:
 # the current stream's handle without the object around it (2.6 us of a call that launches in 3); the device likewise
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _no_gradient(name: str, t: torch.Tensor) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient; this operator has none (torch.no_grad(), or detach it)")
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} has a tangent; this operator has no forward-mode gradient")
 
 
 def _new_status(device: torch.device) -> torch.Tensor:
@@ -146,6 +155,8 @@ class PagedKVCache:
         _need(k.dtype in _DTYPES and k.dtype == v.dtype, f"a cache of {k.dtype} / {v.dtype}: float32 or bfloat16")
         _need(k.device.type == "cuda" and k.device == v.device, "the cache has to be on one ROCm device")
         _need(k.stride(3) == 1 and v.stride(3) == 1, "the features of a cache row have to be contiguous")
+        _no_gradient("k", k)
+        _no_gradient("v", v)
         pages, heads, tokens, dim = k.shape
         _need(pages > 0 and heads > 0, f"a cache of {pages} pages and {heads} heads")
         _need(16 <= tokens <= 4096 and tokens & (tokens - 1) == 0, f"pages of {tokens} tokens: a power of two from 16 to 4096 is served")
@@ -175,8 +186,7 @@ def _rows(name: str, t: torch.Tensor, tokens: Optional[int], heads: Optional[int
         raise ValueError(f"{name} is on {t.device}, not on device {index}")
     if t.stride(2) != 1:
         raise ValueError(f"the features of a row of {name} have to be contiguous")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient; this operator has none (torch.no_grad(), or detach it)")
+    _no_gradient(name, t)
 
 
 def _ints(name: str, t: torch.Tensor, dims: int, index: int) -> None:
@@ -186,6 +196,8 @@ def _ints(name: str, t: torch.Tensor, dims: int, index: int) -> None:
 
 def _batch(cache: PagedKVCache, tokens: int, table: torch.Tensor, past: torch.Tensor, starts: Optional[torch.Tensor]):
     index = cache._index
+    _no_gradient("cache.k", cache.k)
+    _no_gradient("cache.v", cache.v)
     _ints("table", table, 2, index)
     _ints("past", past, 1, index)
     n = past.shape[0]

@@ -196,3 +196,17 @@ def test_a_cache_made_while_a_graph_is_captured(paged):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+def test_gradients_of_a_cache_are_refused(paged):
+    k, q, table, past = rnd(1, 4, 2, 16, 64).cuda(), rnd(3, 1, 2, 64).cuda(), ints([[0, 1]]), ints([3])
+    leaf = k.clone().requires_grad_()
+    with pytest.raises(ValueError, match="requires a gradient"):
+        paged.PagedKVCache.from_tensors(k, leaf)
+    with torch.no_grad():
+        kept = paged.PagedKVCache.from_tensors(leaf, k)
+        paged.paged_attention(q, kept, table, past)
+    with pytest.raises(ValueError, match="cache.k requires a gradient"):
+        paged.paged_attention(q, kept, table, past)
+    with pytest.raises(ValueError, match="cache.k requires a gradient"):
+        paged.kv_append(kept, q, q, table, past)

@@ -164,3 +164,40 @@ def test_a_check_waits_for_every_stream_before_it_reads_and_after_it_clears(monk
         paged._read_status(Status(), "paged cache")
     assert done == ["wait 3", "read", "clear", "wait 3"]
     paged.RotaryTable(64, 4, device="cpu").check()        # nothing to wait for
+
+
+class StubCache:
+    """what the argument checks of the wrapper look at, on the host"""
+    _index = -1
+
+    def __init__(self, k, v):
+        self.k, self.v = k, v
+
+
+def test_gradients_and_tangents_that_would_be_lost_are_refused():
+    import torch.autograd.forward_ad as fwad
+
+    table, pos = RotaryTableOnHost(), torch.zeros(3, dtype=torch.int32)
+    x, page = torch.randn(3, 2, 64), torch.randn(2, 1, 16, 64)
+    with fwad.dual_level():
+        for t in (fwad.make_dual(x, torch.ones_like(x)), fwad.make_dual(x.clone(), torch.zeros_like(x))):
+            with pytest.raises(ValueError, match="tangent"):
+                paged.rotary_embed(t, pos, table)
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                paged.rotary_embed(t, pos, table)
+        with pytest.raises(ValueError, match="ROCm device"):
+            paged.rotary_embed(x, pos, table)
+    cached = lambda k, v: paged._batch(StubCache(k, v), 3, pos[None].expand(3, -1).contiguous(), pos, None)
+    cached(page, page)
+    leaf = page.clone().requires_grad_()
+    for k, v, name in ((leaf, page, "cache.k"), (page, leaf * 2, "cache.v")):
+        with pytest.raises(ValueError, match=f"{name} requires a gradient"):
+            cached(k, v)
+        with torch.no_grad():
+            cached(k, v)
+    with fwad.dual_level(), pytest.raises(ValueError, match="cache.v has a tangent"):
+        cached(page, fwad.make_dual(page, page))
+
+
+def RotaryTableOnHost():
+    return paged.RotaryTable(64, 16, device="cpu")
