@@ -16,7 +16,7 @@ zeros (``kv_append``, ``rotary_embed``) or NaN (``paged_attention``; where ``sta
 of the sequences' that claim them).
 
 Work goes to the current stream of the tensors' device and nothing is synchronised.  No gradients: forward only (tensors that ask for one are
-refused, those of the cache too).
+refused, those of the cache too); what a call writes counts as changed in place.
 """
 from __future__ import annotations
 
@@ -26,6 +26,7 @@ from typing import Any, Dict, Optional
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _hip
 
@@ -245,6 +246,7 @@ def rotary_embed(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, 
                                                positions.data_ptr(), out.data_ptr(), os[0], os[1], rotary._status, _raw_stream(index))
     if rc:
         _hip.check(rc)
+    increment_version(out)              # what autograd saved of it is no longer there
     return out
 
 
@@ -300,6 +302,7 @@ def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, table: torc
                                             rot, at, heads, qp, qs[0], qs[1], qop, qos[0], qos[1], cache._status, _raw_stream(index))
     if rc:
         _hip.check(rc)
+    increment_version((cache.k, cache.v) if q_out is None else (cache.k, cache.v, q_out))      # what autograd saved of them is no longer there
     return q_out
 
 
@@ -364,4 +367,5 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
                                   workspace.data_ptr() if need else None, need, cache._status, _raw_stream(index))
     if rc:
         _hip.check(rc)
+    increment_version(out)
     return out

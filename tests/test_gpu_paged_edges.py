@@ -210,3 +210,27 @@ def test_gradients_of_a_cache_are_refused(paged):
         paged.paged_attention(q, kept, table, past)
     with pytest.raises(ValueError, match="cache.k requires a gradient"):
         paged.kv_append(kept, q, q, table, past)
+
+
+def test_what_a_call_writes_counts_as_changed_in_place(paged):
+    """autograd notices that what it saved is no longer there"""
+    k, q, table, past = rnd(1, 4, 2, 16, 64).cuda(), rnd(3, 1, 2, 64).cuda(), ints([[0, 1]]), ints([3])
+    pool = torch.stack([k, k])
+    cache, rotary = paged.PagedKVCache.from_tensors(pool[0], pool[1]), paged.RotaryTable(64, 10)
+    w = torch.ones((), device="cuda", requires_grad=True)
+    out = torch.empty_like(q)
+    for write, tensor in ((lambda: paged.kv_append(cache, q, q, table, past), cache.k), (lambda: paged.kv_append(cache, q, q, table, past), pool),
+                          (lambda: paged.kv_append(cache, q, q, table, past, rotary=rotary, q=q, q_out=out), out),
+                          (lambda: paged.paged_attention(q, cache, table, past, out=out), out),
+                          (lambda: paged.rotary_embed(q, past, rotary, out=out), out)):
+        loss = (w * tensor).sum()
+        write()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    for read in (cache.k, q):                               # what a call only reads keeps its version
+        loss = (w * read).sum()
+        paged.paged_attention(q, cache, table, past, out=out)
+        paged.rotary_embed(q, past, rotary, out=out)
+        loss.backward()
+    with torch.inference_mode():
+        paged.kv_append(cache, q, q, table, past, q=q, q_out=torch.empty_like(q))
