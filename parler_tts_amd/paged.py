@@ -109,7 +109,27 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optiona
     return freq, gain
 
 
-class RotaryTable:
+class _Held:
+    """Tensors whose addresses, strides and sizes the kernels are told of once: the attributes stay as they were made (others may be added),
+    and a tensor that was given other memory since is noticed by the next call."""
+
+    def _hold(self, one: str, two: str) -> None:
+        self._names, self._one, self._two = (one, two), getattr(self, one), getattr(self, two)
+        self._at = (self._one.data_ptr(), self._two.data_ptr())
+        self._made = frozenset(self.__dict__) | {"_made"}
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__.get("_made", ()):
+            raise AttributeError(f"{type(self).__name__}.{name} is fixed: make another {type(self).__name__}")
+        object.__setattr__(self, name, value)
+
+    def _check_held(self) -> None:
+        if (self._one.data_ptr(), self._two.data_ptr()) != self._at:
+            raise ValueError(f"{self._names[self._one.data_ptr() == self._at[0]]} has other memory than when the {type(self).__name__} was made: "
+                             "make another around it")
+
+
+class RotaryTable(_Held):
     """cos and sin of every position's angles, float32 on the device from float64 angles; made once, kept with the model.
 
     ``layout``: "half" turns the pairs (i, i + rotary_dim / 2), "interleaved" the pairs (2 i, 2 i + 1) of the first ``rotary_dim`` (default:
@@ -130,6 +150,7 @@ class RotaryTable:
         self._status = self.status.data_ptr()
         self._c = _hip.PttsRotary(self.cos.data_ptr(), self.sin.data_ptr(), positions, rotary_dim, 1 if layout == "interleaved" else 0)
         self._ref = C.addressof(self._c)
+        self._hold("cos", "sin")
 
     def check(self) -> None:
         """waits for the device (every stream); raises if a call since the last check met a position outside the table.  Not to be called while
@@ -137,7 +158,7 @@ class RotaryTable:
         _read_status(self.status, "rotary_embed")
 
 
-class PagedKVCache:
+class PagedKVCache(_Held):
     """One layer's keys and values in pages: ``k``, ``v`` [pages, kv_heads, page_tokens, head_dim]."""
 
     def __init__(self, num_pages: int, page_tokens: int, kv_heads: int, head_dim: int, *, dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -171,6 +192,7 @@ class PagedKVCache:
                                    _DTYPES[k.dtype], pages, heads, tokens, dim)
         self._ref = C.addressof(self._c)
         self._workspace: Dict[tuple, int] = {}      # bytes by sizes
+        self._hold("k", "v")
 
     def check(self) -> None:
         """waits for the device (every stream); raises if a call since the last check met a page, length, position or start it could not follow.
@@ -197,6 +219,7 @@ def _ints(name: str, t: torch.Tensor, dims: int, index: int) -> None:
 
 def _batch(cache: PagedKVCache, tokens: int, table: torch.Tensor, past: torch.Tensor, starts: Optional[torch.Tensor]):
     index = cache._index
+    cache._check_held()
     _no_gradient("cache.k", cache.k)
     _no_gradient("cache.v", cache.v)
     _ints("table", table, 2, index)
@@ -228,6 +251,7 @@ def rotary_embed(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, 
     _ints("positions", positions, 1, index)
     if positions.shape[0] != tokens:
         raise ValueError(f"{positions.shape[0]} positions for {tokens} tokens")
+    rotary._check_held()
     if index < 0:
         raise ValueError(f"the rotary table is on {rotary.device}: a ROCm device is needed to turn rows")
     if out is None:
@@ -269,6 +293,7 @@ def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, table: torc
     if rotary is not None:
         if rotary._index != index or rotary.head_dim != cache.head_dim:
             raise ValueError(f"a rotary table for heads of {rotary.head_dim} on {rotary.device}; the cache has {cache.head_dim} on {cache.device}")
+        rotary._check_held()
         rot = rotary._ref
     if positions is not None:
         if rotary is None:

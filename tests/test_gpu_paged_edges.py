@@ -234,3 +234,22 @@ def test_what_a_call_writes_counts_as_changed_in_place(paged):
         loss.backward()
     with torch.inference_mode():
         paged.kv_append(cache, q, q, table, past, q=q, q_out=torch.empty_like(q))
+
+
+def test_the_tensors_of_a_cache_stay_those_the_kernels_know(paged):
+    cache, table, past = paged.PagedKVCache(4, 16, 2, 64, dtype=F32), ints([[0, 1]]), ints([3])
+    q = rnd(1, 1, 2, 64).cuda()
+    for name in ("k", "v", "status", "kv_heads", "device"):
+        with pytest.raises(AttributeError, match=f"PagedKVCache.{name} is fixed"):
+            setattr(cache, name, getattr(cache, name))
+    cache.layer = 7
+    cache.k[:] = 1.0                                        # their contents are the caller's
+    paged.paged_attention(q, cache, table, past)
+    rotary = paged.RotaryTable(64, 16)
+    rotary.sin.data = rotary.sin.data.clone()
+    with pytest.raises(ValueError, match="sin has other memory"):
+        paged.kv_append(cache, q, q, table, past, rotary=rotary)
+    cache.v.data = cache.v.data.clone()
+    for call in (lambda: paged.paged_attention(q, cache, table, past), lambda: paged.kv_append(cache, q, q, table, past)):
+        with pytest.raises(ValueError, match="v has other memory"):
+            call()

@@ -173,6 +173,9 @@ class StubCache:
     def __init__(self, k, v):
         self.k, self.v = k, v
 
+    def _check_held(self):
+        pass
+
 
 def test_gradients_and_tangents_that_would_be_lost_are_refused():
     import torch.autograd.forward_ad as fwad
@@ -201,3 +204,18 @@ def test_gradients_and_tangents_that_would_be_lost_are_refused():
 
 def RotaryTableOnHost():
     return paged.RotaryTable(64, 16, device="cpu")
+
+
+def test_the_tensors_of_a_table_stay_those_the_kernels_know():
+    table = RotaryTableOnHost()
+    for name in ("cos", "sin", "status", "positions", "rotary_dim", "_c"):
+        with pytest.raises(AttributeError, match=f"RotaryTable.{name} is fixed"):
+            setattr(table, name, getattr(table, name))
+    table.note = "mine"                                    # a user's own attributes are theirs
+    table.note = "still"
+    pos, x = torch.zeros(3, dtype=torch.int32), torch.zeros(3, 2, 64)
+    with pytest.raises(ValueError, match="ROCm device"):
+        paged.rotary_embed(x, pos, table)
+    table.cos.data = table.cos.data.clone()
+    with pytest.raises(ValueError, match="cos has other memory"):
+        paged.rotary_embed(x, pos, table)
