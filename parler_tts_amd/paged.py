@@ -180,7 +180,7 @@ class PagedKVCache(_Held):
         _no_gradient("k", k)
         _no_gradient("v", v)
         pages, heads, tokens, dim = k.shape
-        _need(pages > 0 and heads > 0, f"a cache of {pages} pages and {heads} heads")
+        _need(0 < pages < 2 ** 31 and 0 < heads < 2 ** 31, f"a cache of {pages} pages and {heads} heads")
         _need(16 <= tokens <= 4096 and tokens & (tokens - 1) == 0, f"pages of {tokens} tokens: a power of two from 16 to 4096 is served")
         _need(dim in (64, 128), f"head_dim {dim}: 64 and 128 are served")
         self.k, self.v = k, v
@@ -226,6 +226,8 @@ def _batch(cache: PagedKVCache, tokens: int, table: torch.Tensor, past: torch.Te
     _ints("past", past, 1, index)
     n = past.shape[0]
     rows, width = table.shape
+    if (tokens | n | width) >> 31:      # sizes travel in 32 bits, and ctypes would cut them
+        raise ValueError(f"{tokens} tokens of {n} sequences over {width} pages: less than 2^31 of each")
     if rows != n:
         raise ValueError(f"a page table of {rows} rows for {n} sequences")
     at = None
@@ -251,6 +253,8 @@ def rotary_embed(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, 
     _ints("positions", positions, 1, index)
     if positions.shape[0] != tokens:
         raise ValueError(f"{positions.shape[0]} positions for {tokens} tokens")
+    if (tokens | heads) >> 31:
+        raise ValueError(f"{tokens} tokens of {heads} heads: less than 2^31 of each")
     rotary._check_held()
     if index < 0:
         raise ValueError(f"the rotary table is on {rotary.device}: a ROCm device is needed to turn rows")
@@ -307,8 +311,8 @@ def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, table: torc
     if q is not None:
         _rows("q", q, tokens, None, cache.head_dim, index)
         heads = q.shape[1]
-        if q.dtype != k.dtype or heads == 0:
-            raise ValueError(f"q {tuple(q.shape)} of {q.dtype} beside k of {k.dtype}")
+        if q.dtype != k.dtype or heads == 0 or heads >> 31:
+            raise ValueError(f"q {tuple(q.shape)} of {q.dtype} beside k of {k.dtype}: 1 to 2^31 - 1 heads of k's type")
         if q_out is None:
             q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
@@ -350,15 +354,17 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
     heads = q.shape[1]
     if q.dtype != cache.dtype:
         raise ValueError(f"q of {q.dtype} over a cache of {cache.dtype}")
-    if heads == 0 or heads % cache.kv_heads:
+    if heads == 0 or heads % cache.kv_heads or heads >> 31:
         raise ValueError(f"{heads} query heads over {cache.kv_heads} key heads")
+    if not 0 <= max_new < 2 ** 31:
+        raise ValueError(f"max_new {max_new}")
     batch = _batch(cache, tokens, table, past, starts)
     mask, mask_stride, mask_width = None, 0, 0
     if key_mask is not None:
         if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.dim() != 2 or key_mask.shape[0] != past.shape[0] or \
                 key_mask.get_device() != index or (key_mask.shape[1] > 1 and key_mask.stride(1) != 1):
             raise ValueError(f"key_mask has to be a bool tensor [{past.shape[0]}, columns] on {cache.device}")
-        mask_width = key_mask.shape[1]
+        mask_width = min(key_mask.shape[1], 2 ** 31 - 1)      # no context reaches the columns behind
         mask, mask_stride = key_mask.data_ptr() if mask_width else None, max(key_mask.stride(0), mask_width)
         if key_mask.shape[0] > 1 and key_mask.stride(0) < mask_width:
             key_mask = key_mask.contiguous()          # one row for every sequence, expanded

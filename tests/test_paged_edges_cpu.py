@@ -219,3 +219,26 @@ def test_the_tensors_of_a_table_stay_those_the_kernels_know():
     table.cos.data = table.cos.data.clone()
     with pytest.raises(ValueError, match="cos has other memory"):
         paged.rotary_embed(x, pos, table)
+
+
+def test_sizes_that_do_not_fit_32_bits_are_refused_not_cut():
+    """(expanded tensors: the sizes without the memory)"""
+    table, big = RotaryTableOnHost(), 2 ** 32
+    pages, pos = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    starts = torch.zeros(3, dtype=torch.int32)
+    cache = StubCache(torch.zeros(1), torch.zeros(1))
+    paged._batch(cache, 2 ** 31 - 1, pages, pos, starts)
+    for tokens in (2 ** 31, big, big + 2):
+        with pytest.raises(ValueError, match="less than 2\\^31"):
+            paged._batch(cache, tokens, pages, pos, starts)
+    x = torch.zeros(1, 1, 64).expand(1, big + 2, 64)
+    with pytest.raises(ValueError, match="less than 2\\^31"):
+        paged.rotary_embed(x, pos[:1], table)
+    cache.__dict__.update(kv_heads=2, head_dim=64, dtype=torch.float32)
+    for max_new in (-1, 2 ** 31, big, big + 1):
+        with pytest.raises(ValueError, match="max_new"):
+            paged.paged_attention(torch.zeros(2, 2, 64), cache, pages, pos, max_new=max_new)
+    for rows in (lambda: paged.paged_attention(x, cache, pages, pos[:1]),
+                 lambda: paged.kv_append(cache, torch.zeros(1, 2, 64), torch.zeros(1, 2, 64), pages[:1], pos[:1], q=x)):
+        with pytest.raises(ValueError, match="heads"):
+            rows()
