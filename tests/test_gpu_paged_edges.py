@@ -253,3 +253,27 @@ def test_the_tensors_of_a_cache_stay_those_the_kernels_know(paged):
     for call in (lambda: paged.paged_attention(q, cache, table, past), lambda: paged.kv_append(cache, q, q, table, past)):
         with pytest.raises(ValueError, match="v has other memory"):
             call()
+
+
+@pytest.mark.parametrize("single", [True, False])
+@pytest.mark.parametrize("n", [5, 100, 200])
+def test_each_kind_of_bad_entry_sets_its_own_bit(paged, n, single):
+    """lengths of -3 and 2^31 - 1, and a bad page, each alone and together: the bits of the status word, and NaN in the rows concerned alone"""
+    dim = 64
+    starts, past, table, pages = ref.make_batch([(1 if single else 1 + i % 4, 30 + i % 50) for i in range(n)], 16)
+    kc, vc, q = rnd(2, pages, 1, 16, dim), rnd(3, pages, 1, 16, dim), rnd(1, starts[-1], 1, dim)
+    want, bound = ref.attend(q, kc, vc, table, past, starts, 0.125)
+    cache = paged.PagedKVCache.from_tensors(kc.cuda(), vc.cuda())
+    for spoiled, bits in (([("page", 1)], 2), ([("past", 2, -3)], 4), ([("past", 3, 2 ** 31 - 1)], 4), ([("page", 0), ("past", n - 1, -3)], 6)):
+        t, p, keep = table.clone(), list(past), torch.ones(starts[-1], dtype=torch.bool)
+        for what in spoiled:
+            if what[0] == "page":
+                t[what[1], 1] = -5
+            else:
+                p[what[1]] = what[2]
+            keep[starts[what[1]]:starts[what[1] + 1]] = False
+        got = paged.paged_attention(q.cuda(), cache, t.cuda(), ints(p), None if single else ints(starts))
+        assert int(cache.status) == bits
+        assert got[~keep.cuda()].isnan().all()
+        close(got[keep.cuda()], want[keep], bound[keep])
+        cache.status.zero_()

@@ -242,3 +242,51 @@ def test_sizes_that_do_not_fit_32_bits_are_refused_not_cut():
                  lambda: paged.kv_append(cache, torch.zeros(1, 2, 64), torch.zeros(1, 2, 64), pages[:1], pos[:1], q=x)):
         with pytest.raises(ValueError, match="heads"):
             rows()
+
+
+def test_single_tokens_over_long_tables_need_a_workspace_and_ask_for_all_of_it(lib):
+    b, c = batch(starts=None, tokens=2, max_pages=4096, table_stride=4096), kv(k=64 * P, v=128 * P)
+    need = lib.ptts_paged_attention_workspace(C.byref(c), C.byref(b), 4, 1)
+    assert need > 0
+    for refused in (dict(wsb=need - 1), dict(ws=4 * P + 4), dict(wsb=0)):
+        assert attend(lib, c, b, max_new=1, **refused) == -1 and b"workspace" in lib.ptts_last_error()
+    if not torch.cuda.is_available():
+        assert attend(lib, c, b, max_new=1, ws=1024 * P, wsb=need) == LAUNCHED
+
+
+def test_calls_run_on_the_device_of_their_cache_and_leave_the_current_one(monkeypatch):
+    """host tensors that say they are on device 1 while device 0 is current, a library that notes what is current when it is called"""
+    current, seen = [0], []
+
+    class device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class library:
+        def __getattr__(self, name):
+            def call(*args):
+                seen.append((name, current[0], args[-1]))
+                return 32 if name == "ptts_paged_attention_workspace" else 0
+
+            return call
+
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 1)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(paged, "_current_device", lambda: current[0])
+    monkeypatch.setattr(paged, "_raw_stream", lambda index: 1000 + index)
+    monkeypatch.setattr(paged._hip, "load_library", lambda: library())
+    table = RotaryTableOnHost()
+    cache = StubCache(torch.zeros(2, 1, 16, 64), torch.zeros(2, 1, 16, 64))
+    cache.__dict__.update(_index=1, kv_heads=1, head_dim=64, dtype=torch.float32, device=torch.device("cpu"), _ref=0, _status=0, _workspace={})
+    x, pages, pos = torch.zeros(2, 1, 64), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    paged.rotary_embed(x, pos, table)
+    paged.kv_append(cache, x, x, pages, pos, rotary=table, q=x)
+    paged.paged_attention(x, cache, pages, pos)
+    assert [s for s in seen if s[0] != "ptts_paged_attention_workspace"] == [
+        (name, 1, 1001) for name in ("ptts_rotary_embed", "ptts_kv_append", "ptts_paged_attention")] and current == [0]
