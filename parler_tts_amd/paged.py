@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from types import SimpleNamespace
 from typing import Any, Dict, Optional
 
 import torch
@@ -41,12 +42,17 @@ def _need(ok: bool, what: str) -> None:
 # the current stream's handle without the object around it (2.6 us of a call that launches in 3); the device likewise
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_changed = getattr(torch._C, "_increment_version", None) or increment_version      # of a tuple of tensors
+
+
+# the level of forward-mode gradients, below 0 where there is none (looking for a tangent there takes 0.3 us a tensor)
+_forward = forward_ad if hasattr(forward_ad, "_current_level") else SimpleNamespace(_current_level=0)
 
 
 def _no_gradient(name: str, t: torch.Tensor) -> None:
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient; this operator has none (torch.no_grad(), or detach it)")
-    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+    if _forward._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
         raise ValueError(f"{name} has a tangent; this operator has no forward-mode gradient")
 
 
@@ -115,7 +121,7 @@ class _Held:
 
     def _hold(self, one: str, two: str) -> None:
         self._names, self._one, self._two = (one, two), getattr(self, one), getattr(self, two)
-        self._at = (self._one.data_ptr(), self._two.data_ptr())
+        self._at_one, self._at_two = self._one.data_ptr(), self._two.data_ptr()
         self._made = frozenset(self.__dict__) | {"_made"}
 
     def __setattr__(self, name, value):
@@ -124,8 +130,8 @@ class _Held:
         object.__setattr__(self, name, value)
 
     def _check_held(self) -> None:
-        if (self._one.data_ptr(), self._two.data_ptr()) != self._at:
-            raise ValueError(f"{self._names[self._one.data_ptr() == self._at[0]]} has other memory than when the {type(self).__name__} was made: "
+        if self._one.data_ptr() != self._at_one or self._two.data_ptr() != self._at_two:
+            raise ValueError(f"{self._names[self._one.data_ptr() == self._at_one]} has other memory than when the {type(self).__name__} was made: "
                              "make another around it")
 
 
@@ -209,7 +215,8 @@ def _rows(name: str, t: torch.Tensor, tokens: Optional[int], heads: Optional[int
         raise ValueError(f"{name} is on {t.device}, not on device {index}")
     if t.stride(2) != 1:
         raise ValueError(f"the features of a row of {name} have to be contiguous")
-    _no_gradient(name, t)
+    if t.requires_grad or _forward._current_level >= 0:
+        _no_gradient(name, t)
 
 
 def _ints(name: str, t: torch.Tensor, dims: int, index: int) -> None:
@@ -220,8 +227,9 @@ def _ints(name: str, t: torch.Tensor, dims: int, index: int) -> None:
 def _batch(cache: PagedKVCache, tokens: int, table: torch.Tensor, past: torch.Tensor, starts: Optional[torch.Tensor]):
     index = cache._index
     cache._check_held()
-    _no_gradient("cache.k", cache.k)
-    _no_gradient("cache.v", cache.v)
+    if cache.k.requires_grad or cache.v.requires_grad or _forward._current_level >= 0:
+        _no_gradient("cache.k", cache.k)
+        _no_gradient("cache.v", cache.v)
     _ints("table", table, 2, index)
     _ints("past", past, 1, index)
     n = past.shape[0]
@@ -245,7 +253,7 @@ def _batch(cache: PagedKVCache, tokens: int, table: torch.Tensor, past: torch.Te
 def rotary_embed(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x`` [tokens, heads, head_dim] (float32 or bfloat16) turned by ``positions`` [tokens] int32 -> ``out`` (may be ``x``).
     A row whose position is outside the table becomes zero, and ``rotary.check()`` raises."""
-    tokens, heads = x.shape[0], x.shape[1] if x.dim() == 3 else None
+    tokens, heads, given = x.shape[0], x.shape[1] if x.dim() == 3 else None, out is not None
     index = rotary._index
     _rows("x", x, None, None, rotary.head_dim, index)
     if x.dtype not in _DTYPES:
@@ -274,7 +282,8 @@ def rotary_embed(x: torch.Tensor, positions: torch.Tensor, rotary: RotaryTable, 
                                                positions.data_ptr(), out.data_ptr(), os[0], os[1], rotary._status, _raw_stream(index))
     if rc:
         _hip.check(rc)
-    increment_version(out)              # what autograd saved of it is no longer there
+    if given:
+        _changed((out,))                # what autograd saved of it is no longer there
     return out
 
 
@@ -286,7 +295,7 @@ def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, table: torc
     and shares no memory with ``k`` or ``v``), which is returned.  float32 rows may be stored in a bfloat16 cache.  Rows behind the last
     sequence are left alone, in ``q_out`` too.  None of the rows may lie in the cache (copy what is to move within it), and ``cache.k`` and
     ``cache.v`` share no memory."""
-    index = cache._index
+    index, written = cache._index, q_out
     tokens = k.shape[0]
     _rows("k", k, tokens, cache.kv_heads, cache.head_dim, index)
     _rows("v", v, tokens, cache.kv_heads, cache.head_dim, index)
@@ -331,7 +340,7 @@ def kv_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, table: torc
                                             rot, at, heads, qp, qs[0], qs[1], qop, qos[0], qos[1], cache._status, _raw_stream(index))
     if rc:
         _hip.check(rc)
-    increment_version((cache.k, cache.v) if q_out is None else (cache.k, cache.v, q_out))      # what autograd saved of them is no longer there
+    _changed((cache.k, cache.v) if written is None else (cache.k, cache.v, written))      # what autograd saved of them is no longer there
     return q_out
 
 
@@ -348,7 +357,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
     Rows of ``q`` and ``out`` start at multiples of 16 bytes; ``out`` shares no memory with ``q`` or the cache.
     Sequences may share pages, or (an expanded ``table``) all of them.  Rows of no sequence (behind the last, or where ``starts`` are wrong)
     are left as they are in ``out``; rows that descending ``starts`` give to several hold the result of one of these."""
-    index, dim = cache._index, cache.head_dim
+    index, dim, given = cache._index, cache.head_dim, out is not None
     tokens = q.shape[0]
     _rows("q", q, None, None, dim, index)
     heads = q.shape[1]
@@ -398,5 +407,6 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
                                   workspace.data_ptr() if need else None, need, cache._status, _raw_stream(index))
     if rc:
         _hip.check(rc)
-    increment_version(out)
+    if given:
+        _changed((out,))
     return out

@@ -277,3 +277,20 @@ def test_each_kind_of_bad_entry_sets_its_own_bit(paged, n, single):
         assert got[~keep.cuda()].isnan().all()
         close(got[keep.cuda()], want[keep], bound[keep])
         cache.status.zero_()
+
+
+def test_inference_mode_and_its_tensors(paged):
+    """they have no version to raise: caches and outputs made inside are served, inside and outside"""
+    k, q, table, past = rnd(1, 4, 2, 16, 64).cuda(), rnd(3, 1, 2, 64).cuda(), ints([[0, 1]]), ints([3])
+    base = paged.PagedKVCache.from_tensors(k.clone(), k.clone())
+    want = paged.paged_attention(paged.kv_append(base, q, q, table, past, q=q), base, table, past)
+    with torch.inference_mode():
+        cache, out, turned = paged.PagedKVCache(4, 16, 2, 64, dtype=F32), torch.empty_like(q), torch.empty_like(q)
+    for inside in (True, False):
+        with torch.inference_mode(inside):
+            if inside:
+                cache.k.copy_(k)
+                cache.v.copy_(k)
+            paged.kv_append(cache, q, q, table, past, q=q, q_out=turned)
+            assert paged.paged_attention(turned, cache, table, past, out=out) is out
+            assert torch.equal(out, want)
