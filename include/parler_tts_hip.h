@@ -348,7 +348,9 @@ int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, in
  * get NaN; rows of no sequence (behind the last, or where starts are wrong) are left as they are, rows that descending starts give to
  * several hold the result of one of these.  Query head h reads key head h / (q_heads / kv_heads).  q, out: [tokens][q_heads][head_dim] of
  * the cache's type; out shares no memory with q or the cache.
- * max_new: an upper bound of the new tokens of one sequence, 0 = not known; it picks the kernel, never the result's validity.
+ * max_new: an upper bound of the new tokens of one sequence, 0 = not known; with max_pages it picks the kernel and the workspace, never the
+ * result's validity (a tight bound and a table no wider than the contexts need are faster).
+ * bf16: the softmax weights are rounded to bf16 before they meet v (half a step of each); scores, sums and out's sum are f32.
  * workspace: ptts_paged_attention_workspace() bytes (may be 0; negative = PTTS_E_*) at a multiple of 16, not shared with another call
  * in flight. */
 int64_t ptts_paged_attention_workspace(const ptts_paged_kv* cache, const ptts_paged_batch* batch, int32_t q_heads, int32_t max_new);

@@ -111,7 +111,8 @@ class ParlerTTSDecoderConfig(_ConfigBase):
         #   norm_type          "layer_norm" | "rms_norm"  (x * rsqrt(mean(x^2) + 1e-5) * weight; the bias tensors are ignored)
         #   position_embedding "sinusoidal" | "rope"      (no additive table; q, k of the SELF-attention rotated per head,
         #                                                  pairs (i, i + head_dim / 2), angle pos * rope_theta^(-2 i / head_dim),
-        #                                                  stretched by rope_scaling: paged.rotary_frequencies)
+        #                                                  stretched by rope_scaling: paged.rotary_frequencies,
+        #                                                  which also says which of the two yarn ramps this is)
         #   mlp_type           "gelu" | "swiglu"          (fc2(silu(fc1(x)) * fc1_up(x)); extra tensor layers.{l}.fc1_up.weight)
         self.norm_type = kwargs.pop("norm_type", "layer_norm")
         self.position_embedding = kwargs.pop("position_embedding", "sinusoidal")

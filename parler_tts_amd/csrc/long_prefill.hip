@@ -7,6 +7,8 @@
 //     keys they meet are rounded); an fp32 cache takes them as they are.
 //   * the additive mask (0 or finfo.min per key) becomes a key mask; a row of padding that sees no key comes out as zeros
 //   * rows leave as MFMA fragments for the out_proj GEMM
+// The status word is the operators', and nobody reads it: page ids are checked where a table is set, lengths and starts are made here, and
+// prompt and generated positions together never exceed the rotary table's, so that no bit of it can be set.
 #include "attn.h"
 #include "paged.h"
 

@@ -62,7 +62,7 @@ template <int N> __device__ inline void unit_offsets(const RotaryArgs& r, int ro
 // Bound by the stream of rows (a product and a sum a feature): a thread moves two 16-byte pieces, the two runs of its pairs, in the widest
 // loads that strides, alignment and the rotated width allow (else element by element); a workgroup takes whole tokens, so that a token's
 // position is one address for many lanes and the table rows stay in the cache.  Measured: 41283 tokens x 24 heads of 64 in f32, 507 MB:
-// 91 - 94 us, 5400 - 5560 GB/s (a copy of 1 GiB reaches 5060, of 256 MiB 5400); 32 tokens x 16 heads in bf16: 3.1 us on the device, 7.5 with the call.
+// 91 - 94 us, 5400 - 5560 GB/s (a copy of 1 GiB reaches 5060, of 256 MiB 5400); 32 tokens x 16 heads in bf16: 3.1 us on the device, 7.8 with the call.
 template <typename T, int N, bool IL>
 __global__ __launch_bounds__(256) void rotary_embed_kernel(RotaryEmbedArgs a, UnitMap m) {
     const int t0 = blockIdx.x * m.tokens_per_block;
@@ -107,8 +107,8 @@ constexpr int APPEND_TOKENS = 64;      // most tokens of one workgroup
 
 // The rows of a block's tokens are looked up once (sequence, page, slot, position), then every thread moves units of q, k and v, as above.
 // Bound by the stream of rows, behind the look-up's dependent trips (starts, length, page id: a chain of 3 us): 24 prompts of 257 to 1500
-// tokens x 24 heads, 389 MB: 86 us, 4530 GB/s; a step of 32 tokens 3.1 us on the device, 10.5 with the call; a ragged batch of 24 chunks of up
-// to 401 tokens x 16/8 heads of 64 10.2 us (8 of them its bytes).  Loads or stores past the caches: 1.3 times as long for the small batches.
+// tokens x 24 heads, 389 MB: 86 us, 4530 GB/s; a step of 32 tokens 3.3 us on the device, 11.7 with the call; a ragged batch of 24 chunks of up
+// to 401 tokens x 16/8 heads of 64 10.2 us (8 of them its bytes; 11.7 profiled beside an attention).  Loads or stores past the caches: 1.3 times as long for the small batches.
 template <typename T, typename TC, int N, bool IL>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, UnitMap m) {
     __shared__ int page_of[APPEND_TOKENS], slot_of[APPEND_TOKENS], pos_of[APPEND_TOKENS];   // page -1: nothing to do, -2: refused

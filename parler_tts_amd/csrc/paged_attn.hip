@@ -580,8 +580,9 @@ template <> __device__ __forceinline__ void store4<PF32>(float* p, float a, floa
 // instruction between two products.  Iterations with less in front of the end are written out apart: they wait for all in flight.
 // =================================================================================================================================
 // Three workgroups on a CU at head dim 64 (48 KiB, 168 registers: four fragments read ahead), two at 128 (64 KiB, 248 registers).
-// Bound: at head dim 128 the matrix unit, under a power limit (prompt of 8191 tokens, 16 heads over 4: 280 - 294 us, 935 - 980 TFLOP/s, where
-// the library's product of 8192^3 reaches 1162 - 1202); at 64 the vector unit beside it (per tile and wave 32 exponentials, 130 other
+// Bound: at head dim 128 the matrix unit, under a power limit (prompt of 8191 tokens, 16 heads over 4: 279 - 294 us a call in a stream of
+// calls, 935 - 985 TFLOP/s; profiled, by the run's median, 305 - 331 us, 830 - 900, its shortest launches 292 - 299; the library's product of 8192^3
+// reaches 1162 - 1202); at 64 the vector unit beside it (per tile and wave 32 exponentials, 130 other
 // operations, 16 products: 8191 tokens, 16 heads: 182 us, 755 TFLOP/s; with two workgroups on a CU 199).  Short chunks: a workgroup's start
 // (lengths, page ids and first tiles are three dependent trips to memory, 5.6 us) and the unequal lengths.
 // Tried and left: the sum of the weights by the matrix unit or by two-element dot products (no change); 64 rows a wave (registers).

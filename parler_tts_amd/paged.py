@@ -6,7 +6,7 @@ the caller owns (grouped heads, head dim 64 or 128, float32 or bfloat16), as cal
     cache  = PagedKVCache(num_pages, page_tokens, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda")
     rotary = RotaryTable(head_dim, max_positions)
     q = kv_append(cache, k, v, table, past, starts, rotary=rotary, q=q)      # store k (turned) and v, turn q
-    o = paged_attention(q, cache, table, past, starts)
+    o = paged_attention(q, cache, table, past, starts, max_new=longest)
 
 ``table`` [sequences, pages] int32 lists every sequence's pages, ``past`` [sequences] int32 how many of its tokens the cache held before
 this call, ``starts`` [sequences + 1] int32 where its new tokens begin in q / k / v (None: one new token each).  They are read on the
@@ -84,7 +84,11 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optiona
       {"type": "ntk", "factor": s}               theta * s^(r / (r - 2)) in theta's place: the slowest pair interpolated, the fastest kept
       {"type": "yarn", "factor": s, "original_positions": L [, "beta_fast": 32, "beta_slow": 1, "attention_factor": a]}
           pairs that turn more than beta_fast times within L positions kept, those below beta_slow interpolated, linear in the number
-          of turns between; cos and sin times a = 0.1 ln s + 1 (Peng et al., "YaRN: Efficient Context Window Extension", 2023)
+          of TURNS between; cos and sin times a = 0.1 ln s + 1 (Peng et al., "YaRN: Efficient Context Window Extension", 2023)
+
+    There are two ramps by the name of yarn.  This is the paper's.  Checkpoints are also trained with one that is linear in the pair's INDEX
+    between the (rounded) indices where a pair turns beta_fast and beta_slow times: it shares the ends, and differs between them (head dim
+    128, s = 16, L = 4096: the paper's frequencies are up to 67 % lower).  Rows of such a checkpoint are not to be turned by these frequencies.
     """
     _need(isinstance(rotary_dim, int) and rotary_dim > 0 and rotary_dim % 2 == 0, f"rotary_dim {rotary_dim}: a positive even number")
     _need(theta > 0 and math.isfinite(theta), f"theta {theta}")
@@ -350,10 +354,14 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
     """softmax(scale * q k^T) v over the cache -> [tokens, heads, head_dim], ``scale`` by default head_dim^-0.5.
 
     causal: token i of sequence s sees the keys 0 .. past[s] + i (its own among them: append first); otherwise every token sees the keys
-    0 .. past[s] - 1 (states that were cached once, as a cross-attention reads them).  ``key_mask`` [sequences, columns] bool: a False
+    0 .. past[s] - 1 (states that were cached once, as a cross-attention reads them).  ``scale`` is positive.  ``key_mask`` [sequences, columns] bool: a False
     column is no key, whatever the cache holds there; keys behind its last column are seen.  A token without keys gets zeros.
     ``q``'s heads are a multiple of the cache's, in groups: head h reads key head h // (heads / kv_heads).
-    ``max_new``: the longest sequence's number of new tokens if the caller knows it (it helps to pick the kernel; 0: unknown).
+    ``max_new``: the longest sequence's number of new tokens if the caller knows it (0: unknown).  Kernel and workspace are picked by it and
+    by the table's WIDTH, before any length is known: rows of unknown number take the kernel for chunks, and a table much wider than the
+    contexts brings room and a launch to join shares that nobody may need.  Results hold either way; a tight table and bound are faster.
+    bfloat16: scores, sums and the output's sum are float32, the softmax weights are rounded to bfloat16 before they meet the values (half
+    a step, 2^-8 of each; the error against 64 bits is 1.3 to 1.4 times that of float32 weights).  float32 rounds nothing more.
     Rows of ``q`` and ``out`` start at multiples of 16 bytes; ``out`` shares no memory with ``q`` or the cache.
     Sequences may share pages, or (an expanded ``table``) all of them.  Rows of no sequence (behind the last, or where ``starts`` are wrong)
     are left as they are in ``out``; rows that descending ``starts`` give to several hold the result of one of these."""

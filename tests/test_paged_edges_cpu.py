@@ -1,5 +1,6 @@
 """Paged-cache operators without a GPU, at their edges: memory that tensors share, strides that address nothing, the wrapper's promises."""
 import ctypes as C
+import math
 import random
 
 import pytest
@@ -290,3 +291,16 @@ def test_calls_run_on_the_device_of_their_cache_and_leave_the_current_one(monkey
     paged.paged_attention(x, cache, pages, pos)
     assert [s for s in seen if s[0] != "ptts_paged_attention_workspace"] == [
         (name, 1, 1001) for name in ("ptts_rotary_embed", "ptts_kv_append", "ptts_paged_attention")] and current == [0]
+
+
+def test_yarn_is_linear_in_turns_as_the_paper_has_it():
+    """not in the pair's index, as others have it: the part of a frequency that is kept, between 1 and 32 turns within the original positions"""
+    base, _ = paged.rotary_frequencies(128)
+    yarn, _ = paged.rotary_frequencies(128, scaling={"type": "yarn", "factor": 16, "original_positions": 4096})
+    turns = 4096 * base / (2 * math.pi)
+    kept = (yarn / base - 1 / 16) / (1 - 1 / 16)
+    between = (turns > 1) & (turns < 32)
+    assert between.sum() > 10
+    # 64-bit roundings: a few of yarn / base (2^-53 of at most 1), over 15 / 16
+    assert (kept - (turns - 1) / 31)[between].abs().max() < 16 * 2.0 ** -53
+    assert "TURNS" in paged.rotary_frequencies.__doc__ and "INDEX" in paged.rotary_frequencies.__doc__
