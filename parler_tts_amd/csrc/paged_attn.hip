@@ -1311,13 +1311,13 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
             top = next;
             sum *= keep;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = keep == 0.f ? 0.f : acc[i] * keep;
+            for (int i = 0; i < 4; ++i) acc[i] *= keep;
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const float f = l[u] == 0.f ? 0.f : exp2_hw(m[u] - mu);
                 sum = fmaf(l[u], f, sum);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[i] = f == 0.f ? acc[i] : fmaf(x[u][i], f, acc[i]);
+                for (int i = 0; i < 4; ++i) acc[i] = l[u] == 0.f ? acc[i] : fmaf(x[u][i], f, acc[i]);
             }
         }
     } else {
@@ -1327,7 +1327,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
         if ((tid & 63) == 0) red[tid >> 6] = top;
         __syncthreads();
         top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float f = l == 0.f ? 0.f : exp2_hw(m - (top == -INFINITY ? 0.f : top));
+        const float f = exp2_hw(m - (top == -INFINITY ? 0.f : top));      // no key: e^-inf
         weight[tid] = f;
         const float part = wave_sum(l * f);
         if ((tid & 63) == 0) red[4 + (tid >> 6)] = part;
@@ -1338,7 +1338,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
             const f32x4 x = *reinterpret_cast<const f32x4*>(part_out<D>(a, s, orow) + piece * 4);
             const float fs = weight[s];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = fs == 0.f ? acc[i] : fmaf(x[i], fs, acc[i]);
+            for (int i = 0; i < 4; ++i) acc[i] = fmaf(x[i], fs, acc[i]);
         }
         pieces[tid] = acc;
         __syncthreads();

@@ -294,3 +294,25 @@ def test_inference_mode_and_its_tensors(paged):
             paged.kv_append(cache, q, q, table, past, q=q, q_out=turned)
             assert paged.paged_attention(turned, cache, table, past, out=out) is out
             assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF, 64), (F32, 64), (BF, 128), (F32, 128)])
+@pytest.mark.parametrize("new", [1, 30])
+@pytest.mark.parametrize("top,spoiled", [(5990, 100), (10, 5000), (3000, 3001)], ids=["behind", "in front", "beside"])
+def test_values_that_are_not_finite_count_however_small_their_weight(paged, top, spoiled, new, dtype, dim):
+    """one key scores 120 more than the rest, whose weights of e^-120 are 0 in float32: 0 times NaN or infinity is still no number, whichever share
+    the value lies in; all else is the top key's value"""
+    starts, past, table, pages = ref.make_batch([(new, 6000)], 64)
+    kc, vc = torch.zeros(pages, 1, 64, dim, dtype=dtype), rnd(3, pages, 1, 64, dim, dtype=dtype)
+    at = lambda key: (int(table[0, key // 64]), 0, key % 64)
+    kc[at(top)] = 120.0 / dim ** 0.5
+    for feature, value in ((3, math.nan), (5, math.inf), (dim - 1, -math.inf)):
+        vc[at(spoiled)][feature] = value
+    cache = paged.PagedKVCache.from_tensors(kc.cuda(), vc.cuda())
+    got = paged.paged_attention(torch.ones(new, 2, dim, dtype=dtype, device="cuda"), cache, table.cuda(), ints(past), ints(starts), max_new=new)
+    lost = [3, 5, dim - 1]
+    rest = [i for i in range(dim) if i not in lost]
+    assert not got[..., lost].isfinite().any()
+    want = vc[at(top)].double()[rest].expand(new, 2, -1)
+    # 6000 weights of e^-119 beside one: nothing; the output's rounding of its one value, and a weight of exp2(0) = 1
+    close(got[..., rest], want, want.abs() * 2.0 ** -20)
