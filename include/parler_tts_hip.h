@@ -344,10 +344,11 @@ int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, in
 
 /* out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j].  causal: token i of sequence s sees the keys 0 .. past[s] + i (the new tokens are in
  * the cache); else all of 0 .. past[s] - 1 (encoder states, say).  key_mask [n_seqs][mask_stride] bytes: keys j < mask_width with a zero
- * are no keys; whatever they hold does not reach the output.  A token that sees no key gets zeros; rows that a bad page or length concerns
- * get NaN; rows of no sequence (behind the last, or where starts are wrong) are left as they are, rows that descending starts give to
- * several hold the result of one of these.  Query head h reads key head h / (q_heads / kv_heads).  q, out: [tokens][q_heads][head_dim] of
- * the cache's type; out shares no memory with q or the cache.
+ * are no keys; whatever they hold does not reach the output.  A token that sees no key (or whose every score is -infinity) gets zeros;
+ * rows that a bad page or length concerns get NaN, and so may rows of the same sequence that are computed with them; rows of no sequence
+ * (behind the last, or where starts are wrong) are left as they are, rows that descending starts give to several hold the result of one
+ * of these.  Query head h reads key head h / (q_heads / kv_heads).  q, out: [tokens][q_heads][head_dim] of the cache's type; out shares
+ * no memory with q or the cache.
  * max_new: an upper bound of the new tokens of one sequence, 0 = not known; with max_pages it picks the kernel and the workspace, never the
  * result's validity (a tight bound and a table no wider than the contexts need are faster).
  * bf16: the softmax weights are rounded to bf16 before they meet v (half a step of each); scores, sums and out's sum are f32.

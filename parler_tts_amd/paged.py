@@ -12,8 +12,8 @@ the caller owns (grouped heads, head dim 64 or 128, float32 or bfloat16), as cal
 this call, ``starts`` [sequences + 1] int32 where its new tokens begin in q / k / v (None: one new token each).  They are read on the
 device when the work runs, so a captured graph serves other lengths after an in-place update.  What they say wrongly is never followed
 out of a buffer: it sets ``cache.status`` / ``rotary.status``, which ``check()`` turns into an error, and the rows concerned come out as
-zeros (``kv_append``, ``rotary_embed``) or NaN (``paged_attention``; where ``starts`` are wrong, as ``out`` held them or one
-of the sequences' that claim them).
+zeros (``kv_append``, ``rotary_embed``) or NaN (``paged_attention``; rows of the same sequence that are computed with them may be NaN too).
+Where ``starts`` are wrong, rows are as ``out`` held them or of one of the sequences that claim them.
 
 Work goes to the current stream of the tensors' device and nothing is synchronised.  No gradients: forward only (tensors that ask for one are
 refused, those of the cache too); what a call writes counts as changed in place.
@@ -355,7 +355,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, table: torch.Tensor, p
 
     causal: token i of sequence s sees the keys 0 .. past[s] + i (its own among them: append first); otherwise every token sees the keys
     0 .. past[s] - 1 (states that were cached once, as a cross-attention reads them).  ``scale`` is positive.  ``key_mask`` [sequences, columns] bool: a False
-    column is no key, whatever the cache holds there; keys behind its last column are seen.  A token without keys gets zeros.
+    column is no key, whatever the cache holds there; keys behind its last column are seen.  A token without keys
+    (or with every score -infinity) gets zeros.
     ``q``'s heads are a multiple of the cache's, in groups: head h reads key head h // (heads / kv_heads).
     ``max_new``: the longest sequence's number of new tokens if the caller knows it (0: unknown).  Kernel and workspace are picked by it and
     by the table's WIDTH, before any length is known: rows of unknown number take the kernel for chunks, and a table much wider than the
