@@ -33,7 +33,7 @@ def layout(rng, n, inner=64):
     return st
 
 
-def verdict(lib, rc, words):
+def is_refused(lib, rc, words):
     assert rc in (-1, LAUNCHED), (rc, lib.ptts_last_error())
     if rc == -1:
         assert words in lib.ptts_last_error(), lib.ptts_last_error()
@@ -61,15 +61,15 @@ def test_rows_that_share_memory_are_told_from_rows_beside_each_other(lib, seed):
         same = off == 0 and a == b
         r = rotary()
         rc = lib.ptts_rotary_embed(C.byref(r), int(bf16), tokens, heads, 64, 4 * P, *a, P, at, *b, P, None)
-        assert verdict(lib, rc, b"share memory") == (meets and not same)
+        assert is_refused(lib, rc, b"share memory") == (meets and not same)
         far = kv(dtype=int(bf16), k=64 * P, v=128 * P)
         one = batch(starts=None, tokens=tokens, n_seqs=tokens)
         rc = append(lib, far, one, int(bf16), 256 * P, (128, 64), 512 * P, (128, 64), None, heads, 4 * P, a, at, b)
-        assert verdict(lib, rc, b"share memory") == (meets and not same)
+        assert is_refused(lib, rc, b"share memory") == (meets and not same)
         if all(x % (16 // esz) == 0 for x in a + b) and off % 16 == 0:
             c = kv(dtype=int(bf16), k=64 * P, v=128 * P, kv_heads=1)
             rc = attend(lib, c, one, heads, 4 * P, a, at, b, ws=1024 * P)
-            assert verdict(lib, rc, b"share memory") == meets
+            assert is_refused(lib, rc, b"share memory") == meets
         # two key heads beside the query heads
         nk, sk = [tokens, 2], layout(rng, [tokens, 2])
         if rng.random() < 0.6:
@@ -78,7 +78,7 @@ def test_rows_that_share_memory_are_told_from_rows_beside_each_other(lib, seed):
         for first in (True, False):
             rows = (4 * P, sk, 512 * P, (128, 64)) if first else (512 * P, (128, 64), 4 * P, sk)
             rc = append(lib, far, one, int(bf16), *rows, None, heads, 256 * P, (1 << 12, 64), at, b)
-            assert verdict(lib, rc, b"q_out shares memory with k or v") == over
+            assert is_refused(lib, rc, b"q_out shares memory with k or v") == over
     assert 50 < shared < 250
 
 
@@ -108,15 +108,15 @@ def test_rows_within_the_cache_are_told_from_rows_beside_it(lib, seed):
             pools = dict(k=64 * P, v=512 * P) if which == "k" else dict(k=512 * P, v=64 * P)
             c = kv(dtype=int(bf16), k_strides=strides(*st), v_strides=strides(*st), n_pages=pages, page_tokens=16, **pools)
             rc = attend(lib, c, one, 2, 128 * P, (128, 64), at, rows, ws=1024 * P)
-            assert verdict(lib, rc, b"out shares memory with the cache") == meets
+            assert is_refused(lib, rc, b"out shares memory with the cache") == meets
             clear = [(128 * P, (128, 64)), (136 * P, (128, 64)), (144 * P, (128, 64)), (152 * P, (128, 64))]
             for i in range(4):                            # k, v, q, q_out
                 k, v, q, qo = clear[:i] + [(at, rows)] + clear[i + 1:]
                 rc = append(lib, c, one, int(bf16), *k, *v, None, 2, *q, *qo)
-                assert verdict(lib, rc, b"share memory with the cache") == meets
+                assert is_refused(lib, rc, b"share memory with the cache") == meets
         c = kv(dtype=int(bf16), k=64 * P, v=at, k_strides=strides(*st), v_strides=strides(*st), n_pages=pages, page_tokens=16)
         rc = append(lib, c, one, int(bf16), 512 * P, (128, 64), 520 * P, (128, 64))
-        assert verdict(lib, rc, b"keys and values of the cache share memory") == bool(cached & places(at, st, nc, esz))
+        assert is_refused(lib, rc, b"keys and values of the cache share memory") == bool(cached & places(at, st, nc, esz))
     assert 5 < refused < 55, refused
 
 
