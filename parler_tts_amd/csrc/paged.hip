@@ -385,7 +385,15 @@ bool share_memory(const Strided& a, const Strided& b) {
     return m.reaches((int64_t)(pb - pa), m.dims - k);
 }
 
-// whether a tensor and the cache's keys or values do
+// the same rows at the same places
+bool in_place(const Strided& a, const Strided& b) {
+    if (a.p != b.p) return false;
+    for (int i = 0; i < a.dims; ++i)
+        if (a.n[i] > 1 && a.st[i] != b.st[i]) return false;
+    return true;
+}
+
+// whether a tensor and the cache's keys or values share memory
 bool in_cache(const ptts_paged_kv* c, const Strided& t) {
     const int esz = c->dtype == PTTS_DTYPE_BF16 ? 2 : 4;
     const int64_t n[3] = {c->n_pages, c->kv_heads, c->page_tokens};
@@ -439,8 +447,8 @@ int ptts_rotary_embed(const ptts_rotary* rot, int32_t dtype, int32_t tokens, int
     TRY(check_rows("out", out, a.os, tokens, heads, head_dim, true));
     const int esz = dtype == PTTS_DTYPE_BF16 ? 2 : 4;
     const int64_t n[2] = {tokens, heads};
-    if (!(x == out && a.xs[0] == a.os[0] && a.xs[1] == a.os[1]) &&
-        share_memory(Strided{x, a.xs, n, 2, esz, head_dim}, Strided{out, a.os, n, 2, esz, head_dim}))
+    const Strided xs = {x, a.xs, n, 2, esz, head_dim}, os = {out, a.os, n, 2, esz, head_dim};
+    if (!in_place(xs, os) && share_memory(xs, os))
         REFUSE(PTTS_E_INVALID, "x and out share memory in another layout than in place");
     a.pos = positions; a.rot = rotary_args(rot); a.status = status; a.tokens = tokens; a.heads = heads; a.head_dim = head_dim;
     return launched("ptts_rotary_embed", rotary_embed_launch(a, dtype, (hipStream_t)stream));
@@ -474,7 +482,7 @@ int ptts_kv_append(const ptts_paged_kv* cache, const ptts_paged_batch* batch, in
         TRY(check_rows("q", q, a.qs, T, q_heads, D, false));
         TRY(check_rows("q_out", q_out, a.qos, T, q_heads, D, true));
         const Strided qs = {q, a.qs, nq, 2, esz, D}, qos = {q_out, a.qos, nq, 2, esz, D};
-        if (!(q == q_out && a.qs[0] == a.qos[0] && a.qs[1] == a.qos[1]) && share_memory(qs, qos))
+        if (!in_place(qs, qos) && share_memory(qs, qos))
             REFUSE(PTTS_E_INVALID, "q and q_out share memory in another layout than in place");
         if (share_memory(ks, qos) || share_memory(vs, qos)) REFUSE(PTTS_E_INVALID, "q_out shares memory with k or v");
         if (in_cache(cache, qs) || in_cache(cache, qos)) REFUSE(PTTS_E_INVALID, "q or q_out share memory with the cache");

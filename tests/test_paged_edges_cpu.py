@@ -304,3 +304,15 @@ def test_yarn_is_linear_in_turns_as_the_paper_has_it():
     # 64-bit roundings: a few of yarn / base (2^-53 of at most 1), over 15 / 16
     assert (kept - (turns - 1) / 31)[between].abs().max() < 16 * 2.0 ** -53
     assert "TURNS" in paged.rotary_frequencies.__doc__ and "INDEX" in paged.rotary_frequencies.__doc__
+
+
+@no_gpu
+def test_rows_in_place_may_differ_in_strides_of_a_single_entry(lib):
+    """one token, or one head: the stride that differs addresses nothing"""
+    r, far = rotary(), kv(k=64 * P, v=128 * P)
+    one = batch(starts=None, tokens=1, n_seqs=1)
+    for tokens, heads, a, b, ok in ((1, 4, (256, 64), (999, 64), True), (3, 1, (64, 64), (64, 7), True), (2, 4, (256, 64), (300, 64), False)):
+        rc = lib.ptts_rotary_embed(C.byref(r), 1, tokens, heads, 64, P, *a, P, P, *b, P, None)
+        assert rc == (LAUNCHED if ok else -1)
+    assert append(lib, far, one, 1, 256 * P, (128, 64), 512 * P, (128, 64), None, 4, P, (256, 64), P, (999, 64)) == LAUNCHED
+    assert append(lib, far, one, 1, 256 * P, (128, 64), 512 * P, (128, 64), None, 4, P, (256, 64), P, (256, 65)) == -1
