@@ -60,9 +60,10 @@ template <int N> __device__ inline void unit_offsets(const RotaryArgs& r, int ro
 }
 
 // Bound by the stream of rows (a product and a sum a feature): a thread moves two 16-byte pieces, the two runs of its pairs, in the widest
-// loads that strides, alignment and the rotated width allow (else element by element: a rotated width that is no multiple of 8 features in f32,
-// 16 in bf16, takes 120 us for 87 in f32 and 99 for 46 in bf16 at 41283 tokens x 24 heads of 64, an append of 21 thousand 235 for 151 and 205 for 88); a workgroup takes whole tokens, so that a token's
-// position is one address for many lanes and the table rows stay in the cache.  Measured: 41283 tokens x 24 heads of 64 in f32, 507 MB:
+// loads that strides, alignment and the rotated width allow (else element by element: a width that is no multiple of 8 features in f32, 16 in
+// bf16, makes a rotation of 41283 tokens x 24 heads of 64 take 120 us instead of 87 in f32, 99 instead of 46 in bf16, and an append of 21
+// thousand 235 instead of 151, 205 instead of 88).  A workgroup takes whole tokens, so that a token's position is one address for many
+// lanes and the table rows stay in the cache.  Measured: 41283 tokens x 24 heads of 64 in f32, 507 MB:
 // 91 - 94 us, 5400 - 5560 GB/s (a copy of 1 GiB reaches 5060, of 256 MiB 5400); 32 tokens x 16 heads in bf16: 3.1 us on the device, 7.8 with the call.
 template <typename T, int N, bool IL>
 __global__ __launch_bounds__(256) void rotary_embed_kernel(RotaryEmbedArgs a, UnitMap m) {
